@@ -11,7 +11,7 @@
  * do not depend on the head range, the query batch, the KV-head range or the
  * kernel chosen: every (query, head) row is computed by the same arithmetic.
  *
- * Three layers, all plain C types:
+ * Its parts, all plain C types:
  *   1. kernel entry points with the engine's function-pointer signatures
  *      (host pointers, bool result, false = error);
  *   2. checked wrappers with the reference wrappers' validation and error
@@ -21,7 +21,9 @@
  *   4. a device-resident layer cache whose rows the entry of 3 reads in
  *      place;
  *   5. the head transform that prepares Q, K and V rows for 3 and 4;
- *   6. the attention output block (projection, post-norm, residual).
+ *   6. the attention output block (projection, post-norm, residual);
+ *   7. batches of requests over a paged cache: page bookkeeping, appends and
+ *      single-token attention.
  */
 #ifndef PCL_ATTENTION_H
 #define PCL_ATTENTION_H
@@ -227,7 +229,8 @@ int pcl_context_reserve(pcl_context *ctx, size_t bytes);
 /* Wait for the stream; *device_error receives the error flag (bit 0: a
  * non-finite allowed score, bit 1: a non-finite output, bit 2: a non-finite
  * head-transform value, bit 3: a non-finite output-block value, bit 4: a
- * wait between workgroups ran out, pcl_context_set_wait_limit) and is
+ * wait between workgroups ran out, pcl_context_set_wait_limit, bit 5: a page
+ * step that does not fit or page data out of range, section 7) and is
  * cleared. */
 int pcl_context_sync(pcl_context *ctx, int *device_error);
 /* Kernel the descriptor resolves to under PCL_KERNEL_AUTO. */
@@ -452,6 +455,156 @@ int pcl_attention_output(pcl_context *ctx, const float *attended, int64_t n, int
  * few-token kernel with so many tokens a workgroup, else the output block of
  * a wave (16016) or tile of a workgroup as tokens * 1000 + rows. */
 int pcl_debug_projection_form(int64_t n, int64_t in, int64_t out, int cus);
+
+/* ---- 7. batches of requests over a paged cache ------------------------------
+ *
+ * Several requests share pools of pages: a page holds page_tokens consecutive
+ * tokens of one request for one layer's K and V, a request's block table names
+ * its pages in order, and slot = page * page_tokens + offset names a token's
+ * row. One pcl_page_batch serves every layer of a model (all pools have the
+ * same pages). A step of the batch is
+ *
+ *   pcl_page_step            pages for every request's new tokens; the slot,
+ *                            position and request of every row of the step
+ *   per layer:
+ *     pcl_paged_append[_transformed]   the step's K and V rows into the pages
+ *     pcl_paged_attention              the newest token of every request
+ *   pcl_page_commit          the step's tokens count as held
+ *
+ * Rows are in request order: the new tokens of request 0, then of request 1,
+ * and so on; the other entries of a layer (head transform, output block) take
+ * the same rows. All state is the caller's device memory and everything is
+ * asynchronous on the context's stream with no host read, so a whole step can
+ * be captured into a graph and replayed with other lengths (see each entry for
+ * what must exist before the capture). Replays of graphs captured from one
+ * context share its workspace, and must not overlap with each other or with the
+ * context's launches. Nothing here has a counterpart in the reference, whose
+ * caches hold one sequence each.
+ *
+ * What the host cannot see is checked on the device: bit 5 (32) of the error
+ * flag (pcl_context_sync) reports it. */
+
+/* Values of the pages. Rows are rounded to bf16 when they are written (nearest,
+ * ties to even) and widened (exactly) when they are read; all arithmetic is
+ * that of f32 pages. */
+enum pcl_cache_type {
+    PCL_CACHE_F32 = 0,
+    PCL_CACHE_BF16 = 1,
+};
+
+/* The pages of one layer: k and v [pages][page_tokens][kvheads][dim], device
+ * memory, 16-byte aligned. pages * page_tokens below 2^31, page_tokens at most
+ * 4096 (any size, not only powers of two), kvheads at most 4096, dim a multiple
+ * of 16 up to 512. */
+typedef struct pcl_page_pools {
+    void *k, *v;
+    int32_t type; /* enum pcl_cache_type */
+    int64_t pages, page_tokens, kvheads, dim;
+} pcl_page_pools;
+
+/* Page bookkeeping of a batch of `requests` (at most 2048), all arrays device
+ * memory of the caller. State (pcl_page_reset writes an empty batch; a caller
+ * may fill it in itself): */
+typedef struct pcl_page_batch {
+    int64_t requests;
+    int64_t table_stride; /* pages a block table holds */
+    int64_t page_tokens;
+    int64_t pages;
+    int64_t step_rows;    /* rows a step may have, below 2^20 */
+    int32_t *lengths;     /* [requests] tokens held (committed) */
+    int32_t *table;       /* [requests][table_stride] pages of each request */
+    int32_t *free_pages;  /* [pages] a stack: the last free entry is taken first */
+    int32_t *counters;    /* [4] free pages; of the step: its rows, the pages it
+                             takes, 1 while it stands uncommitted */
+    /* what a step writes: */
+    int32_t *step_lengths; /* [requests] tokens held with the step's */
+    int32_t *newest;       /* [requests] row of the newest token, -1 for none */
+    int32_t *slots;        /* [step_rows] slot of each row, -1 behind the last */
+    int32_t *positions;    /* [step_rows] position of each row, -1 behind it */
+    int32_t *row_request;  /* [step_rows] request of each row, -1 behind it */
+} pcl_page_batch;
+
+/* An empty batch: no tokens, every page free, no step. */
+int pcl_page_reset(pcl_context *ctx, const pcl_page_batch *batch);
+/* Opens a step with new_tokens[b] (device, [requests], 0 allowed) more tokens
+ * of every request: pages for them from the free list in request order, their
+ * entries behind the held ones of the block tables, and the step's arrays. The
+ * held state (lengths, held entries, free list) is not changed, so a step that
+ * is not committed is simply replaced by the next one. A step that does not
+ * fit (negative or too many tokens for the table or step_rows, too few free
+ * pages, a length outside the table) is refused as a whole: bit 5 of the error
+ * flag, no rows, slots all -1, counters[3] = 0. A page number outside the pools
+ * in the table or the free list leaves that row's slot -1, with the error. */
+int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *new_tokens);
+/* The standing step's tokens count as held: all of them, or the first kept[b]
+ * of each request (device, [requests]; speculative tokens that were refused);
+ * pages that hold only tokens not kept go back to the free list. Without a
+ * standing step nothing happens; a count outside 0..new tokens, like step data
+ * out of range, is bit 5 of the error flag and changes nothing. */
+int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *kept);
+/* Requests with finished[b] != 0 (device, [requests]) give all their pages back
+ * and hold no tokens; a standing step is dropped. */
+int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *finished);
+
+/* K and V rows [n][kvheads][dim] (f32, device, 16-byte aligned) into the slots
+ * of the pools; a row with a negative slot is left out, one past the pools too,
+ * with bit 5 of the error flag. Slots must differ from each other. */
+int pcl_paged_append(pcl_context *ctx, const pcl_page_pools *pools, const int32_t *slots,
+                     const float *keys, const float *values, int64_t n);
+/* The same from raw projections: pcl_head_transform_prepare for n rows, each
+ * at its own position, with K and V written into their slots and the prepared
+ * queries into q_out [n][qheads][dim] (a row that is left out keeps its q_out).
+ * Positions lie in [0, position_limit), or the row is left out with bit 5 of
+ * the error flag; the rotation table for them is built on the host at the first
+ * call (before a capture: inside one a table that is too short is
+ * PCL_RESOURCE_LIMIT). raw_v NULL as in pcl_head_transform_prepare. On the
+ * transform's context. */
+int pcl_paged_append_transformed(pcl_head_transform *transform, const pcl_page_pools *pools,
+                                 const int32_t *slots, const int32_t *positions,
+                                 int64_t position_limit, const float *raw_q, const float *raw_k,
+                                 const float *raw_v, int64_t n, float *q_out);
+
+/* Attention of the newest token of every request over its pages. Request b
+ * with row r = rows[b] (rows NULL: r = b) attends keys [0, lengths[b]) or, with
+ * a window, the last `window` of them; its query heads are at q + r * q_stride
+ * and its output goes to out + r * o_stride, [qheads][dim] each. A request with
+ * a negative row or no keys is left out: its output row stays as it was. With a
+ * step's arrays (lengths = step_lengths, rows = newest) the requests without a
+ * new token are left out. The query is scaled by q_scale, and scores are capped
+ * by softcap, as in pcl_attention_desc. A request's output has the bits that
+ * pcl_attention_launch gives for its keys and values in one segment (causal, the
+ * same window, first_key 0, first_query lengths[b] - 1; bf16 pages: for the
+ * widened rows), whatever else is in the batch; only a zero's sign may differ.
+ * max_length bounds the lengths (it sizes the workspace); a longer request or a
+ * row at or past q_rows is left out with bit 5 of the error flag, and a page
+ * outside the pools is read as page 0, with bit 5. Rows must differ from each
+ * other. Several requests may share pages. */
+typedef struct pcl_paged_desc {
+    pcl_page_pools pools;
+    const float *q;
+    int64_t q_stride, q_rows; /* q_rows: rows that q and out hold */
+    int64_t qheads;           /* at most 4096 */
+    const int32_t *table;     /* [requests][table_stride] */
+    int64_t table_stride;
+    const int32_t *lengths; /* [requests] */
+    const int32_t *rows;    /* [requests] or NULL */
+    int64_t requests;       /* at most 2048 */
+    int64_t max_length;     /* at most table_stride * page_tokens */
+    int64_t window;         /* 0 = all keys */
+    float q_scale;
+    float softcap; /* 0 = off */
+    float *out;
+    int64_t o_stride;
+} pcl_paged_desc;
+
+/* Launch asynchronously; PCL_OK, PCL_INVALID_SHAPE, PCL_INVALID_PARAMETER,
+ * PCL_RESOURCE_LIMIT when the workspace cannot be had (inside a capture it is
+ * not grown: pcl_context_reserve the bytes before) or PCL_NON_FINITE_VALUE for
+ * a launch failure. Non-finite scores and outputs are bits 0 and 1 of the error
+ * flag. */
+int pcl_paged_attention(pcl_context *ctx, const pcl_paged_desc *desc);
+/* Workspace bytes a descriptor needs (0 when it is refused). */
+size_t pcl_paged_workspace_bytes(const pcl_paged_desc *desc);
 
 /* Library identification (for loaders). */
 const char *pcl_version(void);

@@ -19,6 +19,10 @@ error behaviour:
   HeadTransform
       the engine's HeadTransform (src/engine/attention.rs:51-243): Q/K/V head
       norms and rotary positions on the device, fused with the cache append.
+  PclPageBatch, PclPagePools, PclPagedDesc
+      batches of requests over a paged cache: Context.page_reset / page_step /
+      page_commit / page_release, Context.paged_append,
+      HeadTransform.append_paged and Context.paged_attention.
 
 There is no CPU fallback: without the built library every entry raises.
 """
@@ -42,6 +46,9 @@ KERNELS = (KERNEL_SPLIT_KV, KERNEL_TILED, KERNEL_TILED_SPLIT, KERNEL_PIPE_KV, KE
 KERNEL_NAMES = {KERNEL_SPLIT_KV: "split_kv", KERNEL_TILED: "tiled",
                 KERNEL_TILED_SPLIT: "tiled_split", KERNEL_PIPE_KV: "pipe_kv",
                 KERNEL_SPREAD_KV: "spread_kv", KERNEL_FAN_KV: "fan_kv"}
+
+# values of a paged cache's pages
+CACHE_F32, CACHE_BF16 = 0, 1
 
 # Every symbol include/pcl_attention.h declares.
 EXPORTS = (
@@ -87,6 +94,14 @@ EXPORTS = (
     "pcl_kv_cache_attend_token",
     "pcl_attention_output",
     "pcl_debug_projection_form",
+    "pcl_page_reset",
+    "pcl_page_step",
+    "pcl_page_commit",
+    "pcl_page_release",
+    "pcl_paged_append",
+    "pcl_paged_append_transformed",
+    "pcl_paged_attention",
+    "pcl_paged_workspace_bytes",
     "pcl_version",
 )
 
@@ -121,6 +136,44 @@ class PclDesc(ctypes.Structure):
 class PclPending(ctypes.Structure):
     """pcl_kv_pending (PendingKv, src/engine/attention.rs:263-266), in tokens."""
     _fields_ = [("old_len", ctypes.c_int64), ("old_total", ctypes.c_int64)]
+
+
+class PclPagePools(ctypes.Structure):
+    """pcl_page_pools: one layer's pages."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int32),
+                ("pages", ctypes.c_int64), ("page_tokens", ctypes.c_int64),
+                ("kvheads", ctypes.c_int64), ("dim", ctypes.c_int64)]
+
+
+class PclPageBatch(ctypes.Structure):
+    """pcl_page_batch: page bookkeeping of a batch of requests."""
+    _fields_ = [(n, ctypes.c_int64) for n in ("requests", "table_stride", "page_tokens", "pages",
+                                              "step_rows")] + \
+               [(n, ctypes.c_void_p) for n in ("lengths", "table", "free_pages", "counters",
+                                               "step_lengths", "newest", "slots", "positions",
+                                               "row_request")]
+
+
+class PclPagedDesc(ctypes.Structure):
+    """pcl_paged_desc: one layer's single-token attention of a batch."""
+    _fields_ = [
+        ("pools", PclPagePools),
+        ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("q_rows", ctypes.c_int64),
+        ("qheads", ctypes.c_int64), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p), ("rows", ctypes.c_void_p), ("requests", ctypes.c_int64),
+        ("max_length", ctypes.c_int64), ("window", ctypes.c_int64), ("q_scale", ctypes.c_float),
+        ("softcap", ctypes.c_float), ("out", ctypes.c_void_p), ("o_stride", ctypes.c_int64),
+    ]
+
+
+def page_pools(**kw):
+    """A PclPagePools with the given fields."""
+    return PclPagePools(**kw)
+
+
+def page_batch(**kw):
+    """A PclPageBatch with the given fields."""
+    return PclPageBatch(**kw)
 
 
 _lib = None
@@ -192,6 +245,7 @@ def load():
     i64, i64p = ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)
     pend = ctypes.POINTER(PclPending)
     dp = ctypes.POINTER(PclDesc)
+    batch, pools = ctypes.POINTER(PclPageBatch), ctypes.POINTER(PclPagePools)
     for name, res, args in (
             ("pcl_kv_cache_create", ctypes.c_int, [vp, i64, i64, i64, i64, sz,
                                                    ctypes.POINTER(vp)]),
@@ -222,7 +276,16 @@ def load():
              [vp, vp, vp, vp, vp, ctypes.c_float, ctypes.c_int, vp, vp, pend]),
             ("pcl_attention_output", ctypes.c_int,
              [vp, vp, i64, i64, vp, i64, vp, ctypes.c_float, vp, vp, vp]),
-            ("pcl_debug_projection_form", ctypes.c_int, [i64, i64, i64, ctypes.c_int])):
+            ("pcl_debug_projection_form", ctypes.c_int, [i64, i64, i64, ctypes.c_int]),
+            ("pcl_page_reset", ctypes.c_int, [vp, batch]),
+            ("pcl_page_step", ctypes.c_int, [vp, batch, vp]),
+            ("pcl_page_commit", ctypes.c_int, [vp, batch, vp]),
+            ("pcl_page_release", ctypes.c_int, [vp, batch, vp]),
+            ("pcl_paged_append", ctypes.c_int, [vp, pools, vp, vp, vp, i64]),
+            ("pcl_paged_append_transformed", ctypes.c_int,
+             [vp, pools, vp, vp, i64, vp, vp, vp, i64, vp]),
+            ("pcl_paged_attention", ctypes.c_int, [vp, ctypes.POINTER(PclPagedDesc)]),
+            ("pcl_paged_workspace_bytes", sz, [ctypes.POINTER(PclPagedDesc)])):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
@@ -457,6 +520,52 @@ class Context:
         if rc != OK:
             raise AttentionError(rc)
 
+    def _check(self, rc):
+        if rc != OK:
+            raise AttentionError(rc)
+
+    def page_reset(self, batch):
+        """An empty batch: no tokens, every page free, no step."""
+        self._check(self.lib.pcl_page_reset(self.handle, ctypes.byref(batch)))
+
+    def page_step(self, batch, new_tokens_ptr):
+        """Opens a step: pages, slots, positions and newest rows for the new
+        tokens of every request (device int32 [requests])."""
+        self._check(self.lib.pcl_page_step(self.handle, ctypes.byref(batch),
+                                           ctypes.c_void_p(new_tokens_ptr)))
+
+    def page_commit(self, batch, kept_ptr=None):
+        """The standing step's tokens count as held: all, or the first kept[b]
+        of each request."""
+        self._check(self.lib.pcl_page_commit(self.handle, ctypes.byref(batch),
+                                             ctypes.c_void_p(kept_ptr)))
+
+    def page_release(self, batch, finished_ptr):
+        """Requests with a nonzero flag give their pages back."""
+        self._check(self.lib.pcl_page_release(self.handle, ctypes.byref(batch),
+                                              ctypes.c_void_p(finished_ptr)))
+
+    def paged_append(self, pools, slots_ptr, keys_ptr, values_ptr, n):
+        """K and V rows [n][kv_heads][head_dim] into their slots."""
+        self._check(self.lib.pcl_paged_append(
+            self.handle, ctypes.byref(pools), ctypes.c_void_p(slots_ptr),
+            ctypes.c_void_p(keys_ptr), ctypes.c_void_p(values_ptr), int(n)))
+
+    @staticmethod
+    def paged_desc(**kw):
+        d = PclPagedDesc()
+        d.q_scale = 1.0
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def paged_attention(self, desc):
+        """The newest token of every request over its pages."""
+        self._check(self.lib.pcl_paged_attention(self.handle, ctypes.byref(desc)))
+
+    def paged_workspace_bytes(self, desc):
+        return self.lib.pcl_paged_workspace_bytes(ctypes.byref(desc))
+
     def sync(self):
         """Wait; returns the device error flag (cleared)."""
         err = ctypes.c_int(0)
@@ -643,5 +752,17 @@ class HeadTransform:
     def query(self, raw_q_ptr, n, position, q_out_ptr):
         rc = self.lib.pcl_head_transform_query(self.handle, ctypes.c_void_p(raw_q_ptr), int(n),
                                                int(position), ctypes.c_void_p(q_out_ptr))
+        if rc != OK:
+            raise AttentionError(rc)
+
+    def append_paged(self, pools, slots_ptr, positions_ptr, position_limit, raw_q_ptr, raw_k_ptr,
+                     raw_v_ptr, n, q_out_ptr):
+        """Raw projections of n rows, each at its own position, into their
+        slots of the pages; prepared queries to q_out."""
+        rc = self.lib.pcl_paged_append_transformed(
+            self.handle, ctypes.byref(pools), ctypes.c_void_p(slots_ptr),
+            ctypes.c_void_p(positions_ptr), int(position_limit), ctypes.c_void_p(raw_q_ptr),
+            ctypes.c_void_p(raw_k_ptr), ctypes.c_void_p(raw_v_ptr or None), int(n),
+            ctypes.c_void_p(q_out_ptr))
         if rc != OK:
             raise AttentionError(rc)

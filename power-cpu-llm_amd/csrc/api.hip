@@ -364,7 +364,10 @@ int ensure_workspace(pcl_context *ctx, size_t bytes)
         return PCL_OK;
     if (ctx->ws) {
         (void)hipStreamSynchronize(ctx->stream);
-        (void)hipFree(ctx->ws);
+        if (ctx->ws_captured)
+            ctx->ws_retired.push_back(ctx->ws);
+        else
+            (void)hipFree(ctx->ws);
         ctx->ws = nullptr;
         ctx->ws_bytes = 0;
     }
@@ -815,6 +818,8 @@ void pcl_context_destroy(pcl_context *ctx)
             (void)hipFree(ctx->stage[i]);
     if (ctx->ws)
         (void)hipFree(ctx->ws);
+    for (void *old : ctx->ws_retired)
+        (void)hipFree(old);
     if (ctx->err)
         (void)hipFree(ctx->err);
     if (ctx->own_stream && ctx->stream)
@@ -925,6 +930,30 @@ int launch_plan(pcl_context *ctx, const pcl_attention_desc &desc, Plan *plan)
 }
 
 } // namespace
+
+bool pcl::stream_capturing(hipStream_t stream)
+{
+    return capturing(stream);
+}
+
+size_t pcl::workspace_bytes_for(size_t body)
+{
+    return body ? kTagFloats * sizeof(float) + body : 0;
+}
+
+int pcl::workspace_body(pcl_context *ctx, size_t bytes, float **body)
+{
+    const size_t all = workspace_bytes_for(bytes);
+    if (capturing(ctx->stream)) {
+        if (all > ctx->ws_bytes)
+            return PCL_RESOURCE_LIMIT;
+        ctx->ws_captured = true;
+    }
+    const int rc = ensure_workspace(ctx, all);
+    if (rc == PCL_OK)
+        *body = static_cast<float *>(ctx->ws) + kTagFloats;
+    return rc;
+}
 
 int pcl::launch_step(pcl_context *ctx, const pcl_attention_desc &desc, const StepFold &f,
                      const std::function<int()> &separate)

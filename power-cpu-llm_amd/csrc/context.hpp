@@ -28,6 +28,10 @@ struct pcl_context {
     // epoch generation for which the workspace's published-word region was
     // last zeroed
     uint32_t ws_tag_gen = 0;
+    // a captured paged attention holds the workspace's address: workspaces
+    // outgrown after such a capture are kept until the context is destroyed
+    bool ws_captured = false;
+    std::vector<void *> ws_retired;
     int *err = nullptr;
     // this device's scratch of pcl_attention_launch_noalloc (never freed)
     void *noalloc_scratch = nullptr;
@@ -65,6 +69,16 @@ namespace pcl {
 int kv_cache_reserve(pcl_kv_cache *c, int64_t n);
 // Records the step in *pending and counts its n rows (written at row len).
 void kv_cache_advance_rows(pcl_kv_cache *c, int64_t n, pcl_kv_pending *pending);
+
+// True while `stream` is being captured into a graph.
+bool stream_capturing(hipStream_t stream);
+
+// The context's workspace with room for `bytes` of partials, as *body (behind
+// its region of published words, which no other data enters). Grows it when
+// needed; in a capture it is refused instead (PCL_RESOURCE_LIMIT).
+int workspace_body(pcl_context *ctx, size_t bytes, float **body);
+// The workspace bytes that such a call needs.
+size_t workspace_bytes_for(size_t body);
 
 // A one-token decode step's head transform (the token's raw rows, the
 // learned scales, the (sin, cos) pairs of its position, the norm epsilon)

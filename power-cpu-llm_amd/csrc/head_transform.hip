@@ -26,6 +26,7 @@
 // step's heads run on many CUs at once.
 #include "attention_device.hpp"
 #include "context.hpp"
+#include "paged.hpp"
 #include "pcl_attention.h"
 #include "rotation.hpp"
 #include "step_prologue.hpp"
@@ -49,6 +50,11 @@ struct TransformParams {
     int n, qheads, kvh, dim, slots;
     float eps;
     int *err;
+    // the paged form: every row's slot and position, the pools' slots and the
+    // bound of the positions (the table holds them all)
+    const int32_t *slots_of, *positions;
+    void *kp, *vp;
+    int total, limit;
 };
 
 // Heads per workgroup: about 16 KiB of staged rows, so that several
@@ -59,9 +65,12 @@ constexpr int transform_items()
     return 4096 / DK < 64 ? 4096 / DK : 64;
 }
 
-// Workgroup (token t, slot group y): heads y*ITEMS.. of token t.
-template <int DK, int ITEMS>
-__global__ __launch_bounds__(64) void head_transform_kernel(TransformParams p)
+// Workgroup (token t, slot group y): heads y*ITEMS.. of token t. KV: the type
+// of the K and V rows written. PAGED: token t is at positions[t], its K and V
+// rows go to slot slots_of[t] of the pools; a token with a negative slot is
+// left out, one whose slot or position is out of range too, with an error.
+template <int DK, int ITEMS, typename KV, bool PAGED>
+__device__ __forceinline__ void transform_rows(const TransformParams &p)
 {
     constexpr int kItems = ITEMS;
     constexpr int kStride = DK + 4; // 16-byte aligned rows
@@ -80,7 +89,20 @@ __global__ __launch_bounds__(64) void head_transform_kernel(TransformParams p)
     constexpr int kRowLanes = kHalf / 4;
     constexpr int kPassRows = 64 / kRowLanes;
     const int j0 = 4 * (lane % kRowLanes);
-    const float *tab = p.tab + (p.pos0 + t) * DK;
+    int64_t position = p.pos0 + t, slot = 0;
+    bool live = true;
+    if constexpr (PAGED) {
+        slot = p.slots_of[t];
+        position = p.positions[t];
+        live = slot >= 0;
+        if (live && (slot >= p.total || position < 0 || position >= p.limit)) {
+            live = false;
+            if (lane == 0 && s0 == 0)
+                atomicOr(p.err, kErrPages);
+        }
+        position = live ? position : 0;
+    }
+    const float *tab = p.tab + position * DK;
     const f4 sc0 = ldg4(tab + 2 * j0), sc1 = ldg4(tab + 2 * j0 + 4);
     const f4 qa4 = ldg4(p.qs + j0), qb4 = ldg4(p.qs + j0 + kHalf);
     const f4 ka4 = ldg4(p.ks + j0), kb4 = ldg4(p.ks + j0 + kHalf);
@@ -125,7 +147,8 @@ __global__ __launch_bounds__(64) void head_transform_kernel(TransformParams p)
     for (int r = lane / kRowLanes; r < count; r += kPassRows) {
         const int s = s0 + r;
         const int kind = s < p.qheads ? 0 : s < p.qheads + p.kvh ? 1 : 2;
-        float *out = kind == 0   ? p.oq + (t * p.qheads + s) * DK
+        float *out = PAGED       ? p.oq + (t * p.qheads + s) * DK
+                     : kind == 0 ? p.oq + (t * p.qheads + s) * DK
                      : kind == 1 ? p.ok + t * p.o_kv_stride + (int64_t)(s - p.qheads) * DK
                                  : p.ov + t * p.o_kv_stride + (int64_t)(s - p.qheads - p.kvh) * DK;
         const double iv = inv[r];
@@ -146,11 +169,34 @@ __global__ __launch_bounds__(64) void head_transform_kernel(TransformParams p)
             ya[e] = a;
             yb[e] = b;
         }
+        if constexpr (PAGED) {
+            if (!live)
+                continue;
+            if (kind) {
+                KV *row = static_cast<KV *>(kind == 1 ? p.kp : p.vp) +
+                          (slot * p.kvh + (s - p.qheads - (kind == 1 ? 0 : p.kvh))) * DK;
+                store_row4(row + j0, ya);
+                store_row4(row + j0 + kHalf, yb);
+                continue;
+            }
+        }
         stg4(out + j0, ya);
         stg4(out + j0 + kHalf, yb);
     }
-    if (bad)
+    if (bad && live)
         atomicOr(p.err, kErrTransform);
+}
+
+template <int DK, int ITEMS>
+__global__ __launch_bounds__(64) void head_transform_kernel(TransformParams p)
+{
+    transform_rows<DK, ITEMS, float, false>(p);
+}
+
+template <int DK, int ITEMS, typename KV>
+__global__ __launch_bounds__(64) void paged_transform_kernel(TransformParams p)
+{
+    transform_rows<DK, ITEMS, KV, true>(p);
 }
 
 // Workgroups a launch should at least fill before its heads are packed
@@ -159,7 +205,16 @@ __global__ __launch_bounds__(64) void head_transform_kernel(TransformParams p)
 // workgroup, so fewer heads per workgroup spread it over more CUs.
 constexpr int64_t kTransformSpreadGroups = 256;
 
-template <int DK> static hipError_t launch_dk(const TransformParams &p, hipStream_t stream)
+template <int DK, typename KV, bool PAGED, int ITEMS> constexpr auto transform_kernel()
+{
+    if constexpr (PAGED)
+        return paged_transform_kernel<DK, ITEMS, KV>;
+    else
+        return head_transform_kernel<DK, ITEMS>;
+}
+
+template <int DK, typename KV = float, bool PAGED = false>
+static hipError_t launch_dk(const TransformParams &p, hipStream_t stream)
 {
     auto go = [&](auto kernel, int per) {
         const dim3 grid((unsigned)p.n, (unsigned)((p.slots + per - 1) / per));
@@ -169,21 +224,22 @@ template <int DK> static hipError_t launch_dk(const TransformParams &p, hipStrea
     constexpr int full = transform_items<DK>();
     auto groups = [&](int per) { return (int64_t)p.n * ((p.slots + per - 1) / per); };
     if (groups(full) >= kTransformSpreadGroups || full <= 4)
-        return go(head_transform_kernel<DK, full>, full);
+        return go(transform_kernel<DK, KV, PAGED, full>(), full);
     if (groups(4) >= kTransformSpreadGroups)
-        return go(head_transform_kernel<DK, 4>, 4);
-    return go(head_transform_kernel<DK, 1>, 1);
+        return go(transform_kernel<DK, KV, PAGED, 4>(), 4);
+    return go(transform_kernel<DK, KV, PAGED, 1>(), 1);
 }
 
-hipError_t launch_head_transform(const TransformParams &p, hipStream_t stream)
+template <typename KV = float, bool PAGED = false>
+static hipError_t launch_head_transform(const TransformParams &p, hipStream_t stream)
 {
     switch (p.dim) {
-    case 16: return launch_dk<16>(p, stream);
-    case 32: return launch_dk<32>(p, stream);
-    case 64: return launch_dk<64>(p, stream);
-    case 128: return launch_dk<128>(p, stream);
-    case 256: return launch_dk<256>(p, stream);
-    case 512: return launch_dk<512>(p, stream);
+    case 16: return launch_dk<16, KV, PAGED>(p, stream);
+    case 32: return launch_dk<32, KV, PAGED>(p, stream);
+    case 64: return launch_dk<64, KV, PAGED>(p, stream);
+    case 128: return launch_dk<128, KV, PAGED>(p, stream);
+    case 256: return launch_dk<256, KV, PAGED>(p, stream);
+    case 512: return launch_dk<512, KV, PAGED>(p, stream);
     default: return hipErrorInvalidValue;
     }
 }
@@ -199,6 +255,10 @@ struct pcl_head_transform {
     float *scales = nullptr;    // device [2][dim]: query, key
     float *tab = nullptr;       // device (sin, cos) pairs [rows][dim/2][2]
     int64_t tab_rows = 0;
+    // a captured graph holds the table's address: a table that grows after
+    // such a capture is kept until the transform is destroyed
+    bool captured = false;
+    std::vector<float *> retired;
 };
 
 namespace {
@@ -281,7 +341,9 @@ int ensure_table(pcl_head_transform *t, int64_t end)
             (void)hipFree(tab);
         return PCL_RESOURCE_LIMIT;
     }
-    if (t->tab)
+    if (t->tab && t->captured)
+        t->retired.push_back(t->tab);
+    else if (t->tab)
         (void)hipFree(t->tab);
     t->tab = tab;
     t->tab_rows = rows;
@@ -395,6 +457,8 @@ void pcl_head_transform_destroy(pcl_head_transform *t)
         (void)hipFree(t->scales);
     if (t->tab)
         (void)hipFree(t->tab);
+    for (float *old : t->retired)
+        (void)hipFree(old);
     delete t;
 }
 
@@ -413,6 +477,62 @@ int pcl_head_transform_query(pcl_head_transform *t, const float *raw_q, int64_t 
     if (!t)
         return PCL_INVALID_SHAPE;
     return run(t, raw_q, nullptr, nullptr, n, position, q_out, nullptr, nullptr, 0);
+}
+
+int pcl_paged_append_transformed(pcl_head_transform *t, const pcl_page_pools *pools,
+                                 const int32_t *slots, const int32_t *positions,
+                                 int64_t position_limit, const float *raw_q, const float *raw_k,
+                                 const float *raw_v, int64_t n, float *q_out)
+{
+    if (!t || !pools || !pcl::valid_pools(*pools) || n < 0 || n > pcl::kMaxStepRows ||
+        pools->kvheads != t->kvheads || pools->dim != t->dim)
+        return PCL_INVALID_SHAPE;
+    if (position_limit <= 0 || position_limit > kMaxPositions)
+        return PCL_RESOURCE_LIMIT;
+    if (n == 0)
+        return PCL_OK;
+    if (!slots || !positions || !raw_q || !raw_k || !q_out || (!raw_v && t->sliding) ||
+        ((uintptr_t)slots | (uintptr_t)positions) % 4 ||
+        ((uintptr_t)raw_q | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)q_out) % 16)
+        return PCL_INVALID_SHAPE;
+    (void)hipSetDevice(t->ctx->device);
+    if (pcl::stream_capturing(t->ctx->stream)) {
+        if (position_limit > t->tab_rows) // the table cannot be built in a capture
+            return PCL_RESOURCE_LIMIT;
+        t->captured = true;
+    }
+    const int rc = ensure_table(t, position_limit);
+    if (rc != PCL_OK)
+        return rc;
+    TransformParams p{};
+    p.rq = raw_q;
+    p.rk = raw_k;
+    p.rv = raw_v;
+    p.oq = q_out;
+    p.qs = t->scales;
+    p.ks = t->scales + t->dim;
+    p.tab = t->tab;
+    p.n = (int)n;
+    p.qheads = (int)t->qheads;
+    p.kvh = (int)t->kvheads;
+    p.dim = (int)t->dim;
+    p.slots = (int)(t->qheads + 2 * t->kvheads);
+    p.eps = t->eps;
+    p.err = t->ctx->err;
+    p.slots_of = slots;
+    p.positions = positions;
+    p.kp = pools->k;
+    p.vp = pools->v;
+    p.total = (int)(pools->pages * pools->page_tokens);
+    p.limit = (int)position_limit;
+    const hipError_t e = pools->type == PCL_CACHE_F32
+                             ? pcl::launch_head_transform<float, true>(p, t->ctx->stream)
+                             : pcl::launch_head_transform<__bf16, true>(p, t->ctx->stream);
+    if (e != hipSuccess) {
+        report("paged launch", e);
+        return PCL_NON_FINITE_VALUE;
+    }
+    return PCL_OK;
 }
 
 int pcl_kv_cache_append_transformed(pcl_kv_cache *c, pcl_head_transform *t, const float *raw_q,

@@ -1,0 +1,421 @@
+// Page bookkeeping of a batch of requests on gfx950: block tables, slot map,
+// positions and newest rows of a step, built from the requests' lengths, and
+// the plain append of a step's K and V rows through the slot map.
+//
+// With L_b the committed tokens of request b, n_b its new ones, P tokens a
+// page and F free pages:
+//   off_b   = n_0 + .. + n_{b-1}            first row of request b
+//   held_b  = ceil(L_b / P)                 pages it holds
+//   need_b  = ceil((L_b + n_b) / P) - held_b
+//   first_b = need_0 + .. + need_{b-1}
+//   table[b][held_b + i] = free[F - 1 - (first_b + i)],  0 <= i < need_b
+//   row t in [off_b, off_b + n_b): position p = L_b + t - off_b,
+//   slot = table[b][p div P] * P + p mod P.
+// Both sums run in request order, so a step's result is the same in every
+// run. Nothing that a step reads is written by it (the table's new entries
+// lie behind the held ones, the free list stands until the commit), so its
+// workgroups need no order among them and a repeated step repeats its result.
+#include "context.hpp"
+#include "paged.hpp"
+
+#include <algorithm>
+#include <cstdio>
+
+namespace pcl {
+
+constexpr int kPageThreads = 256;
+
+enum { kCountFree, kCountRows, kCountTaken, kCountState, kCounters };
+
+struct PageParams {
+    int32_t *lengths, *table, *free_pages, *counters, *step_lengths, *newest;
+    int32_t *slots, *positions, *row_request;
+    const int32_t *in; // new tokens, kept tokens or finished flags per request
+    int64_t table_stride;
+    int requests, pages, step_rows;
+    uint32_t page_tokens, max_tokens; // tokens a request may hold
+    int *err;
+};
+
+// Tokens request i holds, or ~0 when its length is outside the table.
+__device__ __forceinline__ uint32_t held_tokens(const PageParams &p, const int32_t *lengths,
+                                                int i)
+{
+    const int32_t n = lengths[i];
+    return n >= 0 && (uint32_t)n <= p.max_tokens ? (uint32_t)n : ~0u;
+}
+
+// One thread per row of the step; every workgroup forms the sums over all
+// requests by itself (they are a few loads a thread), the first one also
+// writes the words of each request. A decode step is a chain of latencies:
+// the lengths' load, the two scans in one 64-bit sum, the search, the page's
+// load.
+__global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
+{
+    extern __shared__ uint32_t offsets[]; // rows [requests + 1], pages [requests]
+    __shared__ uint64_t waves[kPageThreads / 64];
+    uint32_t *row_off = offsets, *page_off = offsets + p.requests + 1;
+    const int tid = threadIdx.x;
+    const int per = (p.requests + kPageThreads - 1) / kPageThreads;
+    const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
+    const int free_count = p.counters[kCountFree];
+    uint64_t sum = 0; // rows in the low half, pages in the high half
+    bool bad = false;
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t len = held_tokens(p, p.lengths, i);
+        const int32_t n = p.in[i];
+        const bool fits = len != ~0u && n >= 0 && n <= p.step_rows &&
+                          (uint32_t)n <= p.max_tokens - len;
+        bad |= !fits;
+        const uint32_t rows = fits ? (uint32_t)n : 0;
+        const uint32_t need =
+            fits ? pages_of(len + rows, p.page_tokens) - pages_of(len, p.page_tokens) : 0;
+        row_off[i] = rows;
+        page_off[i] = need;
+        sum += (uint64_t)need << 32 | rows;
+    }
+    uint64_t total;
+    uint64_t at = block_offsets(sum, waves, &total);
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t rows = row_off[i], need = page_off[i];
+        row_off[i] = (uint32_t)at;
+        page_off[i] = (uint32_t)(at >> 32);
+        at += (uint64_t)need << 32 | rows;
+    }
+    const uint32_t rows = (uint32_t)total, taken = (uint32_t)(total >> 32);
+    if (tid == 0)
+        row_off[p.requests] = rows;
+    bad |= free_count < 0 || free_count > p.pages || (int64_t)taken > free_count ||
+           rows > (uint32_t)p.step_rows;
+    const bool ok = !__syncthreads_or(bad);
+
+    if (blockIdx.x == 0) {
+        for (int i = tid; i < p.requests; i += kPageThreads) {
+            const uint32_t n = ok ? row_off[i + 1] - row_off[i] : 0;
+            p.step_lengths[i] = (int32_t)((uint32_t)p.lengths[i] + n);
+            p.newest[i] = n ? (int32_t)(row_off[i] + n - 1) : -1;
+        }
+        if (tid == 0) {
+            p.counters[kCountRows] = ok ? (int32_t)rows : 0;
+            p.counters[kCountTaken] = ok ? (int32_t)taken : 0;
+            p.counters[kCountState] = ok;
+            if (!ok)
+                atomicOr(p.err, kErrPages);
+        }
+    }
+    const uint32_t t = blockIdx.x * kPageThreads + tid;
+    if (t >= (uint32_t)p.step_rows)
+        return;
+    int32_t slot = -1, position = -1, request = -1;
+    if (ok && t < rows) {
+        request = find_range(row_off, p.requests, t);
+        const uint32_t len = (uint32_t)p.lengths[request];
+        const uint32_t pos = len + (t - row_off[request]);
+        const uint32_t column = pos / p.page_tokens, held = pages_of(len, p.page_tokens);
+        int32_t *entry = p.table + request * p.table_stride + column;
+        const int32_t page =
+            column < held
+                ? *entry
+                : p.free_pages[free_count - 1 - (int)(page_off[request] + column - held)];
+        position = (int32_t)pos;
+        if (page < 0 || page >= p.pages) {
+            atomicOr(p.err, kErrPages); // the caller's table or free list is damaged
+        } else {
+            slot = page * (int32_t)p.page_tokens + (int32_t)(pos % p.page_tokens);
+            // a new page's first token is its first row
+            if (column >= held && pos % p.page_tokens == 0)
+                *entry = page;
+        }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = position;
+    p.row_request[t] = request;
+}
+
+// The pages behind the kept ones of every request go back on the free list,
+// in the order of the requests and of their pages: one workgroup. KEEP: the
+// step's commit (`in`: the tokens kept of each request's new ones, null for
+// all); otherwise the release of the requests whose flag is set.
+template <bool KEEP> __global__ __launch_bounds__(kPageThreads) void page_return_kernel(PageParams p)
+{
+    extern __shared__ uint32_t offsets[]; // returned pages before a request [requests + 1]
+    __shared__ uint32_t waves[kPageThreads / 64];
+    const int tid = threadIdx.x;
+    if (KEEP && p.counters[kCountState] != 1)
+        return; // no step stands
+    const int per = (p.requests + kPageThreads - 1) / kPageThreads;
+    const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
+    const int64_t free_count = (int64_t)p.counters[kCountFree] - (KEEP ? p.counters[kCountTaken] : 0);
+    uint32_t sum = 0;
+    bool bad = false;
+    // tokens request i holds before the call (with the step's) and after it
+    auto tokens = [&](int i, uint32_t *now, uint32_t *after) {
+        const uint32_t len = held_tokens(p, p.lengths, i);
+        *now = KEEP ? held_tokens(p, p.step_lengths, i) : len;
+        bool in = len != ~0u && *now != ~0u && *now >= len;
+        if (KEEP) {
+            const int32_t kept = p.in ? p.in[i] : (int32_t)(*now - len);
+            in = in && kept >= 0 && (uint32_t)kept <= *now - len;
+            *after = len + (uint32_t)kept;
+        } else {
+            *after = p.in[i] ? 0 : len;
+        }
+        return in;
+    };
+    for (int i = i0; i < i1; ++i) {
+        uint32_t now, after;
+        const bool in = tokens(i, &now, &after);
+        bad |= !in;
+        const uint32_t n =
+            in ? pages_of(now, p.page_tokens) - pages_of(after, p.page_tokens) : 0;
+        offsets[i] = n;
+        sum += n;
+    }
+    uint32_t total;
+    uint32_t at = block_offsets(sum, waves, &total);
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t n = offsets[i];
+        offsets[i] = at;
+        at += n;
+    }
+    if (tid == 0)
+        offsets[p.requests] = total;
+    bad |= free_count < 0 || free_count + total > p.pages;
+    if (__syncthreads_or(bad)) {
+        if (tid == 0)
+            atomicOr(p.err, kErrPages);
+        return; // nothing changes
+    }
+    for (uint32_t u = tid; u < total; u += kPageThreads) {
+        const int i = find_range(offsets, p.requests, u);
+        uint32_t now, after;
+        tokens(i, &now, &after);
+        p.free_pages[free_count + u] =
+            p.table[i * p.table_stride + pages_of(after, p.page_tokens) + (u - offsets[i])];
+    }
+    __syncthreads(); // the lengths are read above
+    for (int i = i0; i < i1; ++i) {
+        uint32_t now, after;
+        tokens(i, &now, &after);
+        p.lengths[i] = (int32_t)after;
+    }
+    if (tid == 0) {
+        p.counters[kCountFree] = (int32_t)(free_count + total);
+        p.counters[kCountState] = 0;
+    }
+}
+
+// An empty batch: no tokens, every page free (page 0 is taken first), no step.
+__global__ __launch_bounds__(kPageThreads) void page_reset_kernel(PageParams p)
+{
+    const int64_t step = (int64_t)gridDim.x * kPageThreads;
+    const int64_t t0 = (int64_t)blockIdx.x * kPageThreads + threadIdx.x;
+    for (int64_t i = t0; i < p.requests * p.table_stride; i += step)
+        p.table[i] = -1;
+    for (int64_t i = t0; i < p.pages; i += step)
+        p.free_pages[i] = p.pages - 1 - (int32_t)i;
+    for (int64_t i = t0; i < p.requests; i += step) {
+        p.lengths[i] = 0;
+        p.step_lengths[i] = 0;
+        p.newest[i] = -1;
+    }
+    for (int64_t i = t0; i < p.step_rows; i += step) {
+        p.slots[i] = -1;
+        p.positions[i] = -1;
+        p.row_request[i] = -1;
+    }
+    if (t0 < kCounters)
+        p.counters[t0] = t0 == kCountFree ? p.pages : 0;
+}
+
+struct RowsParams {
+    const float *keys, *values; // [n][width]
+    void *k, *v;                // pools
+    const int32_t *slots;
+    int n, width;
+    int total; // slots of the pools
+    int *err;
+};
+
+// One wave per row and array: the row's loads go out before its slot is
+// needed. HBM-bound on a prompt's rows.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_rows_kernel(RowsParams p)
+{
+    constexpr int kAhead = 8; // 16-byte pieces a lane has in flight
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= p.n)
+        return;
+    const float *src = (blockIdx.y ? p.values : p.keys) + (int64_t)row * p.width;
+    T *pool = static_cast<T *>(blockIdx.y ? p.v : p.k);
+    const int slot = p.slots[row];
+    if (slot < 0)
+        return;
+    if (slot >= p.total) {
+        if (lane == 0)
+            atomicOr(p.err, kErrPages);
+        return;
+    }
+    T *dst = pool + (int64_t)slot * p.width;
+    for (int c = 4 * lane; c < p.width; c += 256 * kAhead) {
+        f4 v[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            v[i] = c + 256 * i < p.width ? ldg4_stream(src + c + 256 * i) : f4{};
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (c + 256 * i < p.width)
+                store_row4(dst + c + 256 * i, v[i]);
+    }
+}
+
+bool valid_pools(const pcl_page_pools &s)
+{
+    return s.k && s.v && (s.type == PCL_CACHE_F32 || s.type == PCL_CACHE_BF16) && s.pages > 0 &&
+           s.page_tokens > 0 && s.page_tokens <= kMaxPageTokens &&
+           s.pages <= kMaxSlots / s.page_tokens && s.kvheads > 0 && s.kvheads <= 4096 &&
+           s.dim > 0 && s.dim % 16 == 0 && s.dim <= 512 &&
+           ((uintptr_t)s.k | (uintptr_t)s.v) % 16 == 0;
+}
+
+} // namespace pcl
+
+namespace {
+
+using pcl::PageParams;
+
+int launched(const char *what)
+{
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess)
+        return PCL_OK;
+    std::fprintf(stderr, "pcl_page: %s: %s\n", what, hipGetErrorString(e));
+    return PCL_NON_FINITE_VALUE;
+}
+
+int page_params(pcl_context *ctx, const pcl_page_batch *b, PageParams *p)
+{
+    if (!ctx || !b || b->requests <= 0 || b->requests > pcl::kMaxRequests || b->table_stride <= 0 ||
+        b->table_stride > pcl::kMaxSlots || b->page_tokens <= 0 ||
+        b->page_tokens > pcl::kMaxPageTokens || b->pages <= 0 ||
+        b->pages > pcl::kMaxSlots / b->page_tokens || b->step_rows <= 0 ||
+        b->step_rows > pcl::kMaxStepRows)
+        return PCL_INVALID_SHAPE;
+    const void *words[] = {b->lengths,      b->table,  b->free_pages, b->counters,   b->step_lengths,
+                           b->newest,       b->slots,  b->positions,  b->row_request};
+    for (const void *w : words)
+        if (!w || (uintptr_t)w % 4)
+            return PCL_INVALID_SHAPE;
+    p->lengths = b->lengths;
+    p->table = b->table;
+    p->free_pages = b->free_pages;
+    p->counters = b->counters;
+    p->step_lengths = b->step_lengths;
+    p->newest = b->newest;
+    p->slots = b->slots;
+    p->positions = b->positions;
+    p->row_request = b->row_request;
+    p->in = nullptr;
+    p->table_stride = b->table_stride;
+    p->requests = (int)b->requests;
+    p->pages = (int)b->pages;
+    p->step_rows = (int)b->step_rows;
+    p->page_tokens = (uint32_t)b->page_tokens;
+    p->max_tokens =
+        (uint32_t)std::min<int64_t>(b->table_stride * b->page_tokens, pcl::kMaxSlots);
+    p->err = ctx->err;
+    (void)hipSetDevice(ctx->device);
+    return PCL_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int pcl_page_reset(pcl_context *ctx, const pcl_page_batch *batch)
+{
+    PageParams p;
+    const int rc = page_params(ctx, batch, &p);
+    if (rc != PCL_OK)
+        return rc;
+    const int64_t words = std::max<int64_t>(
+        {batch->requests * batch->table_stride, batch->pages, batch->step_rows});
+    const int64_t groups = std::min<int64_t>((words + 255) / 256, 1024);
+    pcl::page_reset_kernel<<<(unsigned)groups, pcl::kPageThreads, 0, ctx->stream>>>(p);
+    return launched("reset");
+}
+
+int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *new_tokens)
+{
+    PageParams p;
+    const int rc = page_params(ctx, batch, &p);
+    if (rc != PCL_OK)
+        return rc;
+    if (!new_tokens || (uintptr_t)new_tokens % 4)
+        return PCL_INVALID_SHAPE;
+    p.in = new_tokens;
+    const int groups = (p.step_rows + pcl::kPageThreads - 1) / pcl::kPageThreads;
+    const size_t lds = (2 * (size_t)p.requests + 1) * sizeof(uint32_t);
+    pcl::page_step_kernel<<<groups, pcl::kPageThreads, lds, ctx->stream>>>(p);
+    return launched("step");
+}
+
+int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *kept)
+{
+    PageParams p;
+    const int rc = page_params(ctx, batch, &p);
+    if (rc != PCL_OK)
+        return rc;
+    if ((uintptr_t)kept % 4)
+        return PCL_INVALID_SHAPE;
+    p.in = kept;
+    const size_t lds = ((size_t)p.requests + 1) * sizeof(uint32_t);
+    pcl::page_return_kernel<true><<<1, pcl::kPageThreads, lds, ctx->stream>>>(p);
+    return launched("commit");
+}
+
+int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *finished)
+{
+    PageParams p;
+    const int rc = page_params(ctx, batch, &p);
+    if (rc != PCL_OK)
+        return rc;
+    if (!finished || (uintptr_t)finished % 4)
+        return PCL_INVALID_SHAPE;
+    p.in = finished;
+    const size_t lds = ((size_t)p.requests + 1) * sizeof(uint32_t);
+    pcl::page_return_kernel<false><<<1, pcl::kPageThreads, lds, ctx->stream>>>(p);
+    return launched("release");
+}
+
+int pcl_paged_append(pcl_context *ctx, const pcl_page_pools *pools, const int32_t *slots,
+                     const float *keys, const float *values, int64_t n)
+{
+    if (!ctx || !pools || !pcl::valid_pools(*pools) || n < 0 || n > pcl::kMaxStepRows)
+        return PCL_INVALID_SHAPE;
+    if (n == 0)
+        return PCL_OK;
+    if (!slots || !keys || !values || (uintptr_t)slots % 4 ||
+        ((uintptr_t)keys | (uintptr_t)values) % 16)
+        return PCL_INVALID_SHAPE;
+    pcl::RowsParams p;
+    p.keys = keys;
+    p.values = values;
+    p.k = pools->k;
+    p.v = pools->v;
+    p.slots = slots;
+    p.n = (int)n;
+    p.width = (int)(pools->kvheads * pools->dim);
+    p.total = (int)(pools->pages * pools->page_tokens);
+    p.err = ctx->err;
+    (void)hipSetDevice(ctx->device);
+    const dim3 grid((unsigned)((n + 3) / 4), 2);
+    if (pools->type == PCL_CACHE_F32)
+        pcl::paged_rows_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
+    else
+        pcl::paged_rows_kernel<__bf16><<<grid, 256, 0, ctx->stream>>>(p);
+    return launched("append");
+}
+
+} // extern "C"
