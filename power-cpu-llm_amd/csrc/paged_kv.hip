@@ -12,11 +12,17 @@
 //
 // The lengths live on the device, so the launch is a fixed grid whose
 // workgroups form the chunk counts' sums over the requests themselves and
-// take (chunk, KV head, 16-row unit) items in turn. An item's chunk is scored
-// by NW waves (8 / NW tiles each), the running maxima meet in LDS, and every
-// wave then runs the P.V chains of its DK / NW output dims over all eight
-// tiles. A request of one chunk is written at once; the others leave chunk
+// take (chunk, KV head, unit of query rows) items in turn. Scores: a lane is a
+// key, its K row loaded by itself and multiplied with four query rows a matrix
+// instruction. The running maxima meet in LDS, and every wave then runs the
+// P.V chains of its own output dims over the whole chunk, a lane holding VL of
+// them. A request of one chunk is written at once; the others leave chunk
 // partials in the workspace for paged_combine_kernel.
+//
+// A lane's K row is read 16 bytes at a time, eight loads to a 128-byte line, so
+// these are plain loads: streaming ones left nothing of a line in the L1 cache
+// and read it again for each (64 requests of up to 8192 keys, 16 x 8 x 256 heads
+// in bf16: 4.6 times the lines and 345 us, plain 209 us).
 #include "context.hpp"
 #include "launch.hpp"
 #include "paged.hpp"
@@ -25,6 +31,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdio>
+#include <type_traits>
 
 namespace pcl {
 
@@ -100,105 +107,144 @@ __device__ __forceinline__ void chunk_offsets(const PagedParams &p, uint32_t *of
     __syncthreads();
 }
 
-// Eight consecutive values of a K row (16 or 32 bytes), widened to f32.
-template <typename T> struct Piece8;
-template <> struct Piece8<float> {
-    f4 v[2];
-    __device__ __forceinline__ void load(const float *p)
-    {
-        v[0] = ldg4_stream(p);
-        v[1] = ldg4_stream(p + 4);
+// f(std::integral_constant<int, i>) for i = 0 .. N - 1, in order.
+template <int N, int I = 0, typename F> __device__ __forceinline__ void each(F &&f)
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each<N, I + 1>(f);
     }
-    __device__ __forceinline__ float operator[](int j) const { return v[j >> 2][j & 3]; }
-};
+}
+
+// acc + a b for 64 columns and four rows: every lane is a column with its own
+// b, the four rows' a are those of lanes 4 BLOCK .. 4 BLOCK + 3. The f32 MFMAs
+// are chains of fmas over their k slots (checked bit for bit on MI355X), so 4 of
+// these in the order of the slots equal one v_mfma_f32_16x16x4f32 of the
+// canonical chains, at an eighth of its matrix time for four rows.
+template <int BLOCK> __device__ __forceinline__ f4 mfma_rows4(float a, float b, f4 acc)
+{
+    return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, acc, 4, BLOCK, 0);
+}
+
+// Head dim of the n-th step of the canonical score chain (u, jj, g), and the
+// key of a tile at the n-th step of the canonical P.V chain (b, r, g).
+__host__ __device__ constexpr int chain_dim(int n)
+{
+    return 32 * (n / 32) + 8 * (n % 4) + n % 32 / 4;
+}
+
+__host__ __device__ constexpr int chain_key(int n)
+{
+    return 16 * (n / 16) + 4 * (n % 4) + n % 16 / 4;
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp(float x)
+{
+    return __uint_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
+constexpr int kDppXor1 = 0xb1, kDppXor2 = 0x4e, kDppMirror16 = 0x140, kDppMirror8 = 0x141;
+
+// The maximum of 32 lanes (a tile's keys), on each of them.
+__device__ __forceinline__ float max_tile(float x)
+{
+    x = fmaxf(x, dpp<kDppXor1>(x));
+    x = fmaxf(x, dpp<kDppXor2>(x));
+    x = fmaxf(x, dpp<kDppMirror8>(x));
+    x = fmaxf(x, dpp<kDppMirror16>(x));
+    return max_xor16(x);
+}
+
+// The canonical row sum of 32 lanes: the tree over the key's bits 0, 1, 4, 2
+// and 3 (a mirror of 8 or 16 lanes is the flip of bit 2 or 3 once the lanes
+// below that bit agree).
+__device__ __forceinline__ float sum_tile(float x)
+{
+    x = x + dpp<kDppXor1>(x);
+    x = x + dpp<kDppXor2>(x);
+    x = add_xor16(x);
+    x = x + dpp<kDppMirror8>(x);
+    return x + dpp<kDppMirror16>(x);
+}
+
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-template <> struct Piece8<__bf16> {
-    u4 v;
-    __device__ __forceinline__ void load(const __bf16 *p)
-    {
-        v = __builtin_nontemporal_load((const __attribute__((address_space(1))) u4 *)p);
-    }
-    __device__ __forceinline__ float operator[](int j) const
-    {
-        return j & 1 ? bf16_high(v[j >> 1]) : bf16_low(v[j >> 1]);
-    }
-};
+typedef const __attribute__((address_space(1))) u4 *gu4_cptr;
+typedef const __attribute__((address_space(1))) u2 *gu2_cptr;
+typedef const __attribute__((address_space(1))) uint32_t *gu1_cptr;
+typedef const __attribute__((address_space(1))) uint16_t *gu16_cptr;
 
-// N consecutive values of a V row, widened to f32.
-template <typename T, int N> struct PieceN;
-template <int N> struct PieceN<float, N> {
-    float v[N];
-    __device__ __forceinline__ void load(const float *p)
+// Value j of loaded words, widened to f32.
+template <typename T> __device__ __forceinline__ float value_of(const uint32_t *words, int j)
+{
+    if constexpr (sizeof(T) == 4)
+        return __uint_as_float(words[j]);
+    else
+        return j & 1 ? bf16_high(words[j / 2]) : bf16_low(words[j / 2]);
+}
+
+// One lane's N consecutive values of a V row.
+template <typename T, int N> struct Values {
+    static constexpr int kWords = (N * (int)sizeof(T) + 3) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T *p)
     {
-        if constexpr (N >= 4) {
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const f4 x = ldg4_stream(p + 4 * i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[4 * i + e] = x[e];
-            }
-        } else if constexpr (N == 2) {
-            const f2 x = ldg2(p);
-            v[0] = x.x;
-            v[1] = x.y;
-        } else {
-            v[0] = ldg(p);
-        }
-    }
-    __device__ __forceinline__ float operator[](int j) const { return v[j]; }
-};
-template <int N> struct PieceN<__bf16, N> {
-    uint32_t v[(N + 1) / 2];
-    __device__ __forceinline__ void load(const __bf16 *p)
-    {
-        if constexpr (N == 8) {
-            const u4 x = __builtin_nontemporal_load((const __attribute__((address_space(1))) u4 *)p);
+        if constexpr (kWords == 4) {
+            const u4 x = __builtin_nontemporal_load((gu4_cptr)p);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                v[e] = x[e];
-        } else if constexpr (N == 4) {
-            const u2 x = __builtin_nontemporal_load((const __attribute__((address_space(1))) u2 *)p);
-            v[0] = x.x;
-            v[1] = x.y;
-        } else if constexpr (N == 2) {
-            v[0] = *(const __attribute__((address_space(1))) uint32_t *)p;
+                w[e] = x[e];
+        } else if constexpr (kWords == 2) {
+            const u2 x = __builtin_nontemporal_load((gu2_cptr)p);
+            w[0] = x.x;
+            w[1] = x.y;
+        } else if constexpr (N * sizeof(T) == 4) {
+            w[0] = __builtin_nontemporal_load((gu1_cptr)p);
         } else {
-            v[0] = *(const __attribute__((address_space(1))) uint16_t *)p;
+            w[0] = __builtin_nontemporal_load((gu16_cptr)p);
         }
-    }
-    __device__ __forceinline__ float operator[](int j) const
-    {
-        return j & 1 ? bf16_high(v[j >> 1]) : bf16_low(v[j >> 1]);
     }
 };
 
-template <int DK, int NW> struct PagedCfg {
+// Shape of a workgroup: NW waves, 64 KG keys scored by each; the first PVW of
+// them run the P.V chains of 64 VL output dims. R sets of four query rows.
+template <int DK, typename T, int R> struct PagedCfg {
+    static constexpr int NW = DK >= 256 ? 4 : DK / 64;
+    static constexpr int VL = DK / 64 / NW;
+    static constexpr int PVW = NW;
+    static constexpr int KG = 4 / NW;
     static constexpr int kThreads = 64 * NW;
-    static constexpr int NU = DK / 32;                  // score chain steps
-    static constexpr int TPW = kTilesPerChunk / NW;     // tiles a wave scores
-    static constexpr int VD = DK / NW;                  // output dims of a wave
-    static constexpr int VW = VD / 16;                  // output blocks of a wave
-    static constexpr int kQ = DK + 4;                   // padded Q row
-    static_assert(VW >= 1 && VW * 16 * NW == DK, "whole 16-dim output blocks");
+    // K in pieces of a 128-byte line of each of 64 rows, KB of them in flight
+    static constexpr int kLine = 128 / (int)sizeof(T);
+    static constexpr int KP = DK / kLine; // pieces of a row
+    static constexpr int KB = KP < 2 ? KP : 2;
+    // V tiles in flight
+    static constexpr int VB = 2;
+    static constexpr int kRowsUnit = 4 * R;
+};
+
+// LDS of a workgroup: the query rows and the probabilities in the order in
+// which the MFMAs' A registers take them, and each tile's per-row words.
+template <int DK, int R> struct PagedLds {
+    float q[R][DK][4];                  // [row set][chain step][row]
+    float p[R][kTilesPerChunk][kTile][4]; // [row set][tile][chain step][row]
+    f4 max[kTilesPerChunk][R], alpha[kTilesPerChunk][R], sum[kTilesPerChunk][R];
+    int32_t slots[kChunk];
 };
 
 // FULL: the head dim equals the padded head dim DK.
-template <int DK, typename T, bool FULL, bool CAP, int NW>
-__global__ __launch_bounds__(64 * NW) void paged_kv_kernel(PagedParams p)
+template <int DK, typename T, bool FULL, bool CAP, int R>
+__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kernel(PagedParams p)
 {
-    using C = PagedCfg<DK, NW>;
-    constexpr int NU = C::NU, TPW = C::TPW, VW = C::VW;
-    __shared__ __attribute__((aligned(16))) float qs[kRows * C::kQ];
-    __shared__ float ps[kTilesPerChunk][8][64];
-    __shared__ float tmx[kTilesPerChunk][kRows], trs[kTilesPerChunk][kRows];
-    __shared__ int32_t slots[kChunk];
-    __shared__ uint32_t waves[NW];
+    using C = PagedCfg<DK, T, R>;
+    constexpr int KG = C::KG, KP = C::KP, KB = C::KB, VL = C::VL, VB = C::VB;
+    __shared__ __attribute__((aligned(16))) PagedLds<DK, R> s;
+    __shared__ uint32_t waves[C::NW];
     extern __shared__ uint32_t off[];
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int lane = tid & 63;
 
     chunk_offsets(p, off, waves);
     if (blockIdx.x == 0)
@@ -214,8 +260,7 @@ __global__ __launch_bounds__(64 * NW) void paged_kv_kernel(PagedParams p)
         const int b = find_range(off, p.requests, ci);
         bool unused = false;
         const RequestKeys rk = request_keys(p, b, &unused);
-        const int c0 = rk.first / kChunk;
-        const int cbase = (c0 + (int)(ci - off[b])) * kChunk;
+        const int cbase = (rk.first / kChunk + (int)(ci - off[b])) * kChunk;
         const bool only = off[b + 1] - off[b] == 1; // the request's only chunk
         // chunk-relative keys [lo, hi] are attended
         const int lo = max(rk.first - cbase, 0), hi = min(rk.len - 1 - cbase, kChunk - 1);
@@ -230,176 +275,241 @@ __global__ __launch_bounds__(64 * NW) void paged_kv_kernel(PagedParams p)
                 atomicOr(p.err, kErrPages);
                 page = 0;
             }
-            slots[i] = page * (int32_t)p.page_tokens + (int32_t)(t % p.page_tokens);
+            s.slots[i] = page * (int32_t)p.page_tokens + (int32_t)(t % p.page_tokens);
         }
         // the unit's query rows, scaled; zero past the group and the head dim
-        const int h0 = kh * p.group + unit * kRows;
-        const int nrows = min(p.group - unit * kRows, kRows);
-        for (int i = tid; i < kRows * (DK / 4); i += C::kThreads) {
+        const int h0 = kh * p.group + unit * C::kRowsUnit;
+        const int nrows = min(p.group - unit * C::kRowsUnit, C::kRowsUnit);
+        for (int i = tid; i < R * DK; i += C::kThreads) {
             const int r = i / (DK / 4), d = 4 * (i % (DK / 4));
             const bool in = r < nrows && (FULL || d < p.dim);
-            const f4 x = ldg4(p.q + rk.row * p.q_stride + (in ? (int64_t)(h0 + r) * p.dim + d : 0));
-            *(f4 *)(qs + r * C::kQ + d) = in ? x * p.q_scale : f4{0.f, 0.f, 0.f, 0.f};
+            f4 x = ldg4(p.q + rk.row * p.q_stride + (in ? (int64_t)(h0 + r) * p.dim + d : 0));
+            x = in ? x * p.q_scale : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = (d + e) % 32; // 8 g + jj
+                s.q[r / 4][(d & ~31) + 4 * (k % 8) + k / 8][r % 4] = x[e];
+            }
         }
         __syncthreads();
 
         const T *kp = static_cast<const T *>(p.k) + (int64_t)kh * p.dim;
         const T *vp = static_cast<const T *>(p.v) + (int64_t)kh * p.dim;
-        const bool rin = col < nrows;
 
-        float s[TPW][2][4];
+        // scores: lane = key
+        f4 acc[KG][R];
         bool bad = false;
 #pragma unroll
-        for (int tt = 0; tt < TPW; ++tt) {
-            const int t = w * TPW + tt;
-            const bool any = kTile * t <= hi && kTile * t + kTile - 1 >= lo;
-            float tm = kNegInf;
-            if (any) {
+        for (int kg = 0; kg < KG; ++kg) {
+            const int k0 = 64 * (w * KG + kg);
+            if (k0 > hi || k0 + 63 < lo)
+                continue;
+            const T *row = kp + (int64_t)s.slots[k0 + lane] * p.row_stride;
+            uint32_t kb[KB][32];
+            auto load = [&](int i, uint32_t *to) {
 #pragma unroll
-                for (int blk = 0; blk < 2; ++blk) {
-                    const T *row = kp + (int64_t)slots[kTile * t + 16 * blk + col] * p.row_stride;
-                    Piece8<T> kb[NU];
+                for (int e = 0; e < 8; ++e) {
+                    const int d = C::kLine * i + e * (16 / (int)sizeof(T));
+                    const bool in = FULL || d < p.dim;
+                    const u4 x = *(gu4_cptr)(row + (in ? d : 0)); // (not streamed, see above)
 #pragma unroll
-                    for (int u = 0; u < NU; ++u) {
-                        const int d = 32 * u + 8 * g;
-                        kb[u].load(row + (FULL || d < p.dim ? d : 0));
-                    }
-                    f4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int u = 0; u < NU; ++u) {
-                        const int d = 32 * u + 8 * g;
-                        const f4 qa = *(const f4 *)(qs + col * C::kQ + d);
-                        const f4 qb = *(const f4 *)(qs + col * C::kQ + d + 4);
-#pragma unroll
-                        for (int jj = 0; jj < 8; ++jj) {
-                            const float k = kb[u][jj];
-                            acc = mfma(FULL || d < p.dim ? k : 0.f, jj < 4 ? qa[jj] : qb[jj - 4],
-                                       acc);
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float x = acc[r];
-                        s[tt][blk][r] =
-                            CAP ? soft_cap(x, p.softcap, p.inv_softcap) : x;
-                        const int key = kTile * t + 16 * blk + 4 * g + r;
-                        const bool ok = key >= lo && key <= hi;
-                        bad |= ok && rin && !is_finite(s[tt][blk][r]);
-                        tm = ok ? fmaxf(tm, s[tt][blk][r]) : tm;
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        to[4 * e + j] = in ? x[j] : 0u;
                 }
-                tm = max_xor16(tm);
-                tm = max_xor32(tm);
-            }
-            if (g == 0)
-                tmx[t][col] = tm;
-        }
-        __syncthreads(); // every tile's maximum
-        float tmr[kTilesPerChunk];
+            };
 #pragma unroll
-        for (int t = 0; t < kTilesPerChunk; ++t)
-            tmr[t] = tmx[t][col];
-        {
-            float m = kNegInf;
+            for (int i = 0; i < KB; ++i)
+                load(i, kb[i]);
 #pragma unroll
-            for (int t = 0; t < kTilesPerChunk; ++t) {
-                m = fmaxf(m, tmr[t]);
-                if (t / TPW != w)
-                    continue;
-                if (!(kTile * t <= hi && kTile * t + kTile - 1 >= lo))
-                    continue;
-                bool ok[2][4];
+            for (int r = 0; r < R; ++r)
+                acc[kg][r] = f4{0.f, 0.f, 0.f, 0.f};
+            each<KP>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                uint32_t *words = kb[i % KB];
 #pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
+                for (int m = 0; m < C::kLine / 16; ++m) {
+                    float a[R];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int key = kTile * t + 16 * blk + 4 * g + r;
-                        ok[blk][r] = key >= lo && key <= hi;
-                    }
-                float pr[2][4];
-                const float rs = tile_probs(s[t % TPW], ok, safe_max(m), pr);
+                    for (int r = 0; r < R; ++r)
+                        a[r] = s.q[r][C::kLine * i + 16 * m + lane / 4][lane % 4];
+                    each<16>([&](auto nc) {
+                        constexpr int n = decltype(nc)::value;
+                        const float k = value_of<T>(words, chain_dim(16 * m + n));
 #pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
+                        for (int r = 0; r < R; ++r)
+                            acc[kg][r] = mfma_rows4<n>(a[r], k, acc[kg][r]);
+                    });
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (i + KB < KP)
+                    load(i + KB, words);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            const int key = k0 + lane;
+            const bool ok = key >= lo && key <= hi;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        ps[t][4 * blk + r][lane] = pr[blk][r];
-                if (g == 0)
-                    trs[t][col] = rs;
+            for (int r = 0; r < R; ++r) {
+                f4 tm;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = acc[kg][r][e];
+                    x = CAP ? soft_cap(x, p.softcap, p.inv_softcap) : x;
+                    bad |= ok && 4 * r + e < nrows && !is_finite(x);
+                    x = ok ? x : kNegInf;
+                    acc[kg][r][e] = x;
+                    tm[e] = max_tile(x);
+                }
+                if ((lane & 31) == 0)
+                    s.max[key / kTile][r] = tm;
             }
         }
         if (bad)
             atomicOr(p.err, kErrScore);
-        __syncthreads(); // every tile's probabilities and row sums
+        const int t0 = lo / kTile, t1 = hi / kTile; // tiles with attended keys
+        __syncthreads(); // every tile's maximum
 
-        // the l chain and the P.V chains of the wave's output blocks; block x:
-        // A operand V[key][d0 + VW col + x], so O[x][i] is dim
-        // d0 + VW (4g + i) + x of row col
-        const int d0 = C::VD * w;
-        const int vd = d0 + VW * col;
-        const bool vin = FULL || vd < p.dim;
-        float m = kNegInf, l = 0.f;
-        f4 O[VW];
+        // probabilities against the running maximum at the lane's tile
 #pragma unroll
-        for (int x = 0; x < VW; ++x)
-            O[x] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < kTilesPerChunk; ++t) {
-            if (!(kTile * t <= hi && kTile * t + kTile - 1 >= lo))
+        for (int kg = 0; kg < KG; ++kg) {
+            const int k0 = 64 * (w * KG + kg);
+            if (k0 > hi || k0 + 63 < lo)
                 continue;
-            PieceN<T, VW> vr[8];
+            const int key = k0 + lane, t = key / kTile;
+            const bool ok = key >= lo && key <= hi;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int key = kTile * t + 16 * (e >> 2) + 4 * g + (e & 3);
-                vr[e].load(vp + (int64_t)slots[key] * p.row_stride + (vin ? vd : 0));
+            for (int r = 0; r < R; ++r) {
+                f4 before, m; // running maxima before and at the tile
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    before[e] = kNegInf;
+                for (int i = t0; i < k0 / kTile; ++i) {
+                    const f4 x = s.max[i][r];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        before[e] = fmaxf(before[e], x[e]);
+                }
+                const f4 first = s.max[k0 / kTile][r], mine = s.max[t][r];
+                f4 pr, sum, alpha;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (t > k0 / kTile && t0 <= k0 / kTile)
+                        before[e] = fmaxf(before[e], first[e]);
+                    m[e] = fmaxf(before[e], mine[e]);
+                    const float ms = safe_max(m[e]);
+                    pr[e] = ok ? fexp(acc[kg][r][e] - ms) : 0.f;
+                    alpha[e] = fexp(before[e] - ms);
+                    sum[e] = sum_tile(pr[e]);
+                }
+                const int k = key % kTile;
+                *(f4 *)s.p[r][t][(k & 16) + 4 * (k & 3) + (k >> 2 & 3)] = pr;
+                if ((lane & 31) == 0) {
+                    s.alpha[t][r] = alpha;
+                    s.sum[t][r] = sum;
+                }
             }
-            const float mn = fmaxf(m, tmr[t]);
-            const float ms = safe_max(mn);
-            const float alpha = fexp(m - ms);
-            l = __builtin_fmaf(l, alpha, trs[t][col]);
-            m = mn;
+        }
+        __syncthreads(); // every tile's probabilities, row sums and factors
+
+        if (w >= C::PVW)
+            continue;
+        // the l chain and the P.V chains of the lane's VL output dims
+        const int vd = (64 * w + lane) * VL;
+        const T *vlane = vp + (FULL || vd < p.dim ? vd : 0);
+        f4 l[R], O[R][VL];
 #pragma unroll
-            for (int x = 0; x < VW; ++x)
-                O[x] = O[x] * alpha;
+        for (int r = 0; r < R; ++r) {
+            l[r] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float pe = ps[t][e][lane];
+            for (int x = 0; x < VL; ++x)
+                O[r][x] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        Values<T, VL> vb[VB][kTile];
+        auto load_v = [&](int t, Values<T, VL> *to) {
+            const int slots = s.slots[kTile * t + (lane & 31)];
 #pragma unroll
-                for (int x = 0; x < VW; ++x)
-                    O[x] = mfma(vr[e][x], pe, O[x]);
+            for (int n = 0; n < kTile; ++n) {
+                const int slot = __builtin_amdgcn_readlane(slots, chain_key(n));
+                to[n].load(vlane + (int64_t)slot * p.row_stride);
+            }
+        };
+        auto attend = [&](int t, const Values<T, VL> *v) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const f4 alpha = s.alpha[t][r], sum = s.sum[t][r];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    l[r][e] = __builtin_fmaf(l[r][e], alpha[e], sum[e]);
+#pragma unroll
+                for (int x = 0; x < VL; ++x)
+                    O[r][x] = O[r][x] * alpha;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float a[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    a[r] = s.p[r][t][16 * half + lane / 4][lane % 4];
+                each<16>([&](auto nc) {
+                    constexpr int n = decltype(nc)::value;
+#pragma unroll
+                    for (int x = 0; x < VL; ++x)
+#pragma unroll
+                        for (int r = 0; r < R; ++r)
+                            O[r][x] = mfma_rows4<n>(
+                                a[r], value_of<T>(v[16 * half + n].w, x), O[r][x]);
+                });
+            }
+        };
+        // VB tiles in flight; tiles past the last repeat it (not attended)
+#pragma unroll
+        for (int i = 0; i < VB; ++i)
+            load_v(min(t0 + i, t1), vb[i]);
+        for (int t = t0; t <= t1; t += VB) {
+#pragma unroll
+            for (int i = 0; i < VB; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (t + i <= t1)
+                    attend(t + i, vb[i]);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(min(t + i + VB, t1), vb[i]);
             }
         }
 
-        if (!rin)
+        if (!FULL && vd >= p.dim)
             continue;
-        // lane (col, g): the 4 VW dims from d0 + 4 VW g of row col
-        const int dg = d0 + 4 * VW * g;
-        const int h = h0 + col;
-        const int64_t part = (int64_t)ci * p.qheads + h;
-        float *dst = only ? p.out + rk.row * p.o_stride + (int64_t)h * p.dim + dg
-                          : p.ws_o + part * p.dim + dg;
+        f4 mlast[R];
         bool nonfinite = false;
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-            if (!FULL && dg + 4 * k >= p.dim)
-                continue;
-            f4 v;
+        for (int r = 0; r < R; ++r) {
+            mlast[r] = s.max[t0][r];
+            for (int i = t0 + 1; i <= t1; ++i) {
+                const f4 x = s.max[i][r];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mlast[r][e] = fmaxf(mlast[r][e], x[e]);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int n = 4 * k + e;
-                v[e] = O[n % VW][n / VW];
-                if (only) {
-                    v[e] = v[e] / l;
-                    nonfinite |= !is_finite(v[e]);
+                if (4 * r + e >= nrows)
+                    continue;
+                const int h = h0 + 4 * r + e;
+                const int64_t part = (int64_t)ci * p.qheads + h;
+                float *dst = only ? p.out + rk.row * p.o_stride + (int64_t)h * p.dim + vd
+                                  : p.ws_o + part * p.dim + vd;
+#pragma unroll
+                for (int x = 0; x < VL; ++x) {
+                    const float v = only ? O[r][x][e] / l[r][e] : O[r][x][e];
+                    nonfinite |= only && !is_finite(v);
+                    stg(dst + x, v);
+                }
+                if (!only && w == 0 && lane == 0) {
+                    stg(p.ws_ml + 2 * part, mlast[r][e]);
+                    stg(p.ws_ml + 2 * part + 1, l[r][e]);
                 }
             }
-            stg4(dst + 4 * k, v);
         }
         if (nonfinite)
             atomicOr(p.err, kErrOutput);
-        if (!only && w == 0 && g == 0) {
-            stg(p.ws_ml + 2 * part, m);
-            stg(p.ws_ml + 2 * part + 1, l);
-        }
     }
 }
 
@@ -476,34 +586,44 @@ __global__ __launch_bounds__(kPagedLanes * kPagedSpans) void paged_combine_kerne
 
 constexpr int kPagedGroupsPerCu = 4;
 
-template <int DK, typename T, bool FULL, bool CAP>
-static hipError_t launch_paged(const PagedParams &p, int64_t items, hipStream_t stream)
+template <int DK, typename T, bool FULL, bool CAP, int R>
+static hipError_t launch_paged(PagedParams p, int64_t chunks, hipStream_t stream)
 {
-    constexpr int NW = DK == 64 ? 4 : 4;
+    using C = PagedCfg<DK, T, R>;
+    p.units = (p.group + C::kRowsUnit - 1) / C::kRowsUnit;
+    const int64_t items = chunks * p.kvheads * p.units;
     const int cus = std::max(device_cus(), 1);
     const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(items, kPagedGroupsPerCu * cus));
     const size_t lds = ((size_t)p.requests + 1) * sizeof(uint32_t);
-    paged_kv_kernel<DK, T, FULL, CAP, NW><<<(unsigned)grid, 64 * NW, lds, stream>>>(p);
+    paged_kv_kernel<DK, T, FULL, CAP, R><<<(unsigned)grid, C::kThreads, lds, stream>>>(p);
     return hipGetLastError();
 }
 
-template <int DK, typename T> static hipError_t launch_paged(const PagedParams &p, int64_t items,
+template <int DK, typename T, bool FULL, bool CAP>
+static hipError_t launch_paged(const PagedParams &p, int64_t chunks, hipStream_t stream)
+{
+    return p.group <= 4   ? launch_paged<DK, T, FULL, CAP, 1>(p, chunks, stream)
+           : p.group <= 8 ? launch_paged<DK, T, FULL, CAP, 2>(p, chunks, stream)
+                          : launch_paged<DK, T, FULL, CAP, 4>(p, chunks, stream);
+}
+
+template <int DK, typename T> static hipError_t launch_paged(const PagedParams &p, int64_t chunks,
                                                              hipStream_t stream)
 {
     if (p.softcap > 0.f)
-        return p.dim == DK ? launch_paged<DK, T, true, true>(p, items, stream)
-                           : launch_paged<DK, T, false, true>(p, items, stream);
-    return p.dim == DK ? launch_paged<DK, T, true, false>(p, items, stream)
-                       : launch_paged<DK, T, false, false>(p, items, stream);
+        return p.dim == DK ? launch_paged<DK, T, true, true>(p, chunks, stream)
+                           : launch_paged<DK, T, false, true>(p, chunks, stream);
+    return p.dim == DK ? launch_paged<DK, T, true, false>(p, chunks, stream)
+                       : launch_paged<DK, T, false, false>(p, chunks, stream);
 }
 
 template <typename T>
-static hipError_t launch_paged(const PagedParams &p, int64_t items, hipStream_t stream)
+static hipError_t launch_paged(const PagedParams &p, int64_t chunks, hipStream_t stream)
 {
-    return p.dim <= 64    ? launch_paged<64, T>(p, items, stream)
-           : p.dim <= 128 ? launch_paged<128, T>(p, items, stream)
-           : p.dim <= 256 ? launch_paged<256, T>(p, items, stream)
-                          : launch_paged<512, T>(p, items, stream);
+    return p.dim <= 64    ? launch_paged<64, T>(p, chunks, stream)
+           : p.dim <= 128 ? launch_paged<128, T>(p, chunks, stream)
+           : p.dim <= 256 ? launch_paged<256, T>(p, chunks, stream)
+                          : launch_paged<512, T>(p, chunks, stream);
 }
 
 // Chunks that one request may have.
@@ -604,14 +724,14 @@ int pcl_paged_attention(pcl_context *ctx, const pcl_paged_desc *desc)
     p.qheads = (int)d.qheads;
     p.kvheads = (int)s.kvheads;
     p.group = (int)group;
-    p.units = (int)((group + pcl::kRows - 1) / pcl::kRows);
+    p.units = 1;
     p.dim = (int)s.dim;
     p.q_scale = d.q_scale;
     p.softcap = d.softcap;
     p.inv_softcap = d.softcap > 0.0f ? 1.0f / d.softcap : 0.0f;
-    const int64_t items = d.requests * each * s.kvheads * p.units;
-    hipError_t e = s.type == PCL_CACHE_F32 ? pcl::launch_paged<float>(p, items, ctx->stream)
-                                           : pcl::launch_paged<__bf16>(p, items, ctx->stream);
+    const int64_t chunks = d.requests * each;
+    hipError_t e = s.type == PCL_CACHE_F32 ? pcl::launch_paged<float>(p, chunks, ctx->stream)
+                                           : pcl::launch_paged<__bf16>(p, chunks, ctx->stream);
     if (e == hipSuccess && each > 1) {
         const dim3 grid((unsigned)d.requests, (unsigned)d.qheads,
                         (unsigned)((s.dim + 4 * pcl::kPagedLanes - 1) / (4 * pcl::kPagedLanes)));
