@@ -513,19 +513,22 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
     }
 }
 
-// The ordered merge of a request's chunk partials for one query head and a
-// slab of 4 LANES dims: groups of LANES lanes merge a span of 16 chunks each,
-// ascending from (-inf, 0, 0), and leave it in LDS, then the first group folds
-// the spans in ascending order. Requests of one chunk are written already.
-constexpr int kPagedLanes = 8;
-constexpr int kPagedSpans = 32; // spans per round
+// The ordered merge of a request's chunk partials. LANES lanes hold four dims
+// each of one query head; SPANS such groups merge a span of 16 chunks each,
+// ascending from (-inf, 0, 0), in batches of BATCH loads, and the first group
+// folds the spans in ascending order. Requests of one chunk are written already.
+constexpr int kCombineMost = 256; // threads of a workgroup, at most
 
-__global__ __launch_bounds__(kPagedLanes * kPagedSpans) void paged_combine_kernel(PagedParams p)
+struct CombineShape {
+    int lanes, spans, heads; // powers of two; heads: query heads of a workgroup
+};
+
+template <int BATCH>
+__global__ __launch_bounds__(kCombineMost) void paged_combine_kernel(PagedParams p, CombineShape c)
 {
-    constexpr int L = kPagedLanes;
-    __shared__ f4 so[kPagedSpans][L];
-    __shared__ float sm[kPagedSpans], sl[kPagedSpans];
-    const int b = blockIdx.x, h = blockIdx.y;
+    __shared__ f4 so[kCombineMost];
+    __shared__ float sm[kCombineMost], sl[kCombineMost];
+    const int b = blockIdx.x;
     const uint32_t base = p.ws_off[b];
     const int nch = (int)(p.ws_off[b + 1] - base);
     if (nch <= 1)
@@ -534,43 +537,52 @@ __global__ __launch_bounds__(kPagedLanes * kPagedSpans) void paged_combine_kerne
     const RequestKeys rk = request_keys(p, b, &unused);
     const int c0 = rk.first / kChunk, c1 = c0 + nch; // the request's chunks
     const int s0 = c0 / kSpanChunks, s1 = (c1 - 1) / kSpanChunks + 1;
-    const int gi = threadIdx.x / L, q = threadIdx.x % L;
-    const int d = 4 * L * blockIdx.z + 4 * q;
-    const bool din = d < p.dim;
+    const int tid = threadIdx.x;
+    const int q = tid % c.lanes, gi = tid / c.lanes % c.spans;
+    const int h = blockIdx.y * c.heads + tid / (c.lanes * c.spans);
+    const int d = 4 * (c.lanes * blockIdx.z + q);
+    const bool in = h < p.qheads && d < p.dim;
+    const int64_t row = in ? h : 0;
+    const int at = in ? d : 0;
     Merged4 t = {kNegInf, 0.f, f4{0.f, 0.f, 0.f, 0.f}};
-    for (int r0 = s0; r0 < s1; r0 += kPagedSpans) {
-        const int n = min(s1 - r0, kPagedSpans);
-        if (gi < n) {
-            const int a = max((r0 + gi) * kSpanChunks, c0), e = min((r0 + gi + 1) * kSpanChunks, c1);
-            f2 ml[kSpanChunks];
-            f4 ov[kSpanChunks];
+    for (int r0 = s0; r0 < s1; r0 += c.spans) {
+        Merged4 s = {kNegInf, 0.f, f4{0.f, 0.f, 0.f, 0.f}};
+        if (r0 + gi < s1) {
+            const int e = min((r0 + gi + 1) * kSpanChunks, c1);
+            for (int a = max((r0 + gi) * kSpanChunks, c0); a < e; a += BATCH) {
+                f2 ml[BATCH];
+                f4 ov[BATCH];
 #pragma unroll
-            for (int i = 0; i < kSpanChunks; ++i) {
-                const int64_t part =
-                    (int64_t)(base + (uint32_t)((a + i < e ? a + i : a) - c0)) * p.qheads + h;
-                ml[i] = ldg2(p.ws_ml + 2 * part);
-                ov[i] = ldg4(p.ws_o + part * p.dim + (din ? d : 0));
-            }
-            Merged4 s = {kNegInf, 0.f, f4{0.f, 0.f, 0.f, 0.f}};
+                for (int i = 0; i < BATCH; ++i) {
+                    const int64_t part =
+                        (int64_t)(base + (uint32_t)(min(a + i, e - 1) - c0)) * p.qheads + row;
+                    ml[i] = ldg2(p.ws_ml + 2 * part);
+                    ov[i] = ldg4(p.ws_o + part * p.dim + at);
+                }
 #pragma unroll
-            for (int i = 0; i < kSpanChunks; ++i) {
-                const bool in = a + i < e;
-                merge_into4(s, in ? ml[i].x : kNegInf, in ? ml[i].y : 0.f,
-                            in ? ov[i] : f4{0.f, 0.f, 0.f, 0.f});
-            }
-            so[gi][q] = s.acc;
-            if (q == 0) {
-                sm[gi] = s.M;
-                sl[gi] = s.L;
+                for (int i = 0; i < BATCH; ++i) {
+                    // chunks past the span merge as empty parts (no-ops)
+                    const bool here = a + i < e;
+                    merge_into4(s, here ? ml[i].x : kNegInf, here ? ml[i].y : 0.f,
+                                here ? ov[i] : f4{0.f, 0.f, 0.f, 0.f});
+                }
             }
         }
+        if (c.spans == 1) {
+            merge_into4(t, s.M, s.L, s.acc);
+            continue;
+        }
+        so[tid] = s.acc;
+        sm[tid] = s.M;
+        sl[tid] = s.L;
         __syncthreads();
         if (gi == 0)
-            for (int i = 0; i < n; ++i)
-                merge_into4(t, sm[i], sl[i], so[i][q]);
+            for (int i = 0; i < min(s1 - r0, c.spans); ++i)
+                merge_into4(t, sm[tid + i * c.lanes], sl[tid + i * c.lanes],
+                            so[tid + i * c.lanes]);
         __syncthreads();
     }
-    if (gi != 0 || !din)
+    if (gi != 0 || !in)
         return;
     f4 v;
     bool nonfinite = false;
@@ -582,6 +594,35 @@ __global__ __launch_bounds__(kPagedLanes * kPagedSpans) void paged_combine_kerne
     stg4(p.out + rk.row * p.o_stride + (int64_t)h * p.dim + d, v);
     if (nonfinite)
         atomicOr(p.err, kErrOutput);
+}
+
+// Groups of the combine: as many spans at once as some four thousand waves
+// allow (one long request: 32, each a round trip or two; 64 requests of 16
+// heads of 256 dims: 4), the fewer the wider.
+static hipError_t launch_paged_combine(const PagedParams &p, int64_t chunks, hipStream_t stream)
+{
+    auto pow2_to = [](int64_t n, int most) { // the least power of two >= n, at most `most`
+        int x = 1;
+        while (x < n && x < most)
+            x *= 2;
+        return x;
+    };
+    const int quads = p.dim / 4;
+    const int64_t lanes = (int64_t)p.requests * p.qheads * quads;
+    CombineShape c;
+    c.spans = pow2_to(chunks / kSpanChunks + 1, 32);
+    while (c.spans > 1 && c.spans * lanes > 4096 * 64)
+        c.spans /= 2;
+    c.lanes = std::min(pow2_to(quads, 64), kCombineMost / c.spans);
+    c.heads = std::max(1, 64 / (c.spans * c.lanes));
+    const dim3 grid((unsigned)p.requests, (unsigned)((p.qheads + c.heads - 1) / c.heads),
+                    (unsigned)((quads + c.lanes - 1) / c.lanes));
+    const int threads = c.lanes * c.spans * c.heads;
+    if (c.spans >= 16)
+        paged_combine_kernel<16><<<grid, threads, 0, stream>>>(p, c);
+    else
+        paged_combine_kernel<8><<<grid, threads, 0, stream>>>(p, c);
+    return hipGetLastError();
 }
 
 constexpr int kPagedGroupsPerCu = 4;
@@ -732,12 +773,8 @@ int pcl_paged_attention(pcl_context *ctx, const pcl_paged_desc *desc)
     const int64_t chunks = d.requests * each;
     hipError_t e = s.type == PCL_CACHE_F32 ? pcl::launch_paged<float>(p, chunks, ctx->stream)
                                            : pcl::launch_paged<__bf16>(p, chunks, ctx->stream);
-    if (e == hipSuccess && each > 1) {
-        const dim3 grid((unsigned)d.requests, (unsigned)d.qheads,
-                        (unsigned)((s.dim + 4 * pcl::kPagedLanes - 1) / (4 * pcl::kPagedLanes)));
-        pcl::paged_combine_kernel<<<grid, pcl::kPagedLanes * pcl::kPagedSpans, 0, ctx->stream>>>(p);
-        e = hipGetLastError();
-    }
+    if (e == hipSuccess && each > 1)
+        e = pcl::launch_paged_combine(p, each, ctx->stream);
     if (e != hipSuccess) {
         std::fprintf(stderr, "pcl_paged_attention: launch: %s\n", hipGetErrorString(e));
         return PCL_NON_FINITE_VALUE;
