@@ -15,8 +15,11 @@ OBJ_DIR = os.path.join(HERE, "_build")
 SOURCES = ["csrc/split_kv.hip", "csrc/pipe_kv.hip", "csrc/spread_kv.hip",
            "csrc/tiled.hip", "csrc/tiled_wide.hip", "csrc/fan_kv.hip",
            "csrc/api.hip", "csrc/kv_cache.hip", "csrc/head_transform.hip",
-           "csrc/output_block.hip", "csrc/page_tables.hip", "csrc/paged_kv.hip"]
+           "csrc/output_block.hip", "csrc/page_tables.hip", "csrc/paged_attention.hip",
+           "csrc/paged_kv_d64.hip", "csrc/paged_kv_d128.hip", "csrc/paged_kv_d256.hip",
+           "csrc/paged_kv_d512.hip"]
 HEADERS = ["csrc/attention_device.hpp", "csrc/context.hpp", "csrc/launch.hpp", "csrc/paged.hpp",
+           "csrc/paged_params.hpp", "csrc/paged_kv.hpp",
            os.path.join(ROOT, "include", "pcl_attention.h")]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
