@@ -341,37 +341,50 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
     uint32_t *const ring = dyn + (size_t)w * NB * 2048;
     int at = 0;
     const uint32_t row_bytes = (uint32_t)(p.row_stride * sizeof(T));
-    auto copy = [&](const char *from, int e) {
-        __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(ring + at * 2048 + e * 256),
-                                         16, 0, kStreamed);
+    // Where a unit's eight copies read: worked out before the wait for the unit
+    // in their buffer, whose slots' LDS round trips it hides.
+    struct Sources {
+        const char *from[8];
     };
     // K unit i of an item: row 8 e + lane / 8 of the group, the line's 16-byte
     // pieces in the order piece ^ (row & 7), so that a lane's reads of its own
     // row fall in other banks than its neighbours'
-    auto issue_k = [&](const int32_t *slots, int kh, int i) {
+    auto sources_k = [&](const int32_t *slots, int kh, int i) {
         const int line = i % KP;
         const int d = C::kLine * line + (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
         const char *base = static_cast<const char *>(p.k) +
                            ((int64_t)kh * p.dim + (FULL || d < p.dim ? d : 0)) * sizeof(T);
         const int32_t *mine = slots + 64 * (w * KG + i / KP) + lane / 8;
+        Sources c;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            copy(base + (uint64_t)(uint32_t)mine[8 * e] * row_bytes, e);
+            c.from[e] = base + (uint64_t)(uint32_t)mine[8 * e] * row_bytes;
+        return c;
     };
     // V unit i of the tiles from t0 to t1 (past them the last tile again): its
     // keys in the order of the P.V chain
-    auto issue_v = [&](const int32_t *slots, int kh, int t0, int t1, int i) {
+    auto sources_v = [&](const int32_t *slots, int kh, int t0, int t1, int i) {
         const int d = 64 * VL * w + lane % C::kLanesV * (16 / (int)sizeof(T));
         const char *base = static_cast<const char *>(p.v) +
                            ((int64_t)kh * p.dim + (FULL || d < p.dim ? d : 0)) * sizeof(T);
+        Sources c;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int n = C::kKeysV * i + (e * 64 + lane) / C::kLanesV; // chain step from tile t0 on
             const int t = min(t0 + n / kTile, t1), k = n % kTile;
-            copy(base + (uint64_t)(uint32_t)slots[kTile * t + (k & 16) + 4 * (k & 3) + (k >> 2 & 3)] *
-                            row_bytes,
-                 e);
+            c.from[e] =
+                base +
+                (uint64_t)(uint32_t)slots[kTile * t + (k & 16) + 4 * (k & 3) + (k >> 2 & 3)] *
+                    row_bytes;
         }
+        return c;
+    };
+    auto issue = [&](const Sources &c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            __builtin_amdgcn_global_load_lds((global_ptr)c.from[e],
+                                             (lds_ptr)(ring + at * 2048 + e * 256), 16, 0,
+                                             kStreamed);
     };
     // the consumed unit's contents are there; then, read, its buffer is free
     auto wait_unit = [&]() {
@@ -389,7 +402,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NB; ++i, at = at + 1 == NB ? 0 : at + 1)
-        issue_k(s.slots[0], x.kh, i);
+        issue(sources_k(s.slots[0], x.kh, i));
 
     int buf = 0;
     for (uint32_t item = blockIdx.x;; buf ^= 1) {
@@ -414,6 +427,11 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
                 for (int r = 0; r < R; ++r)
                     acc[kg][r] = f4{0.f, 0.f, 0.f, 0.f};
             }
+            Sources c;
+            if constexpr (i + NB < UK)
+                c = sources_k(s.slots[buf], x.kh, i + NB);
+            else
+                c = sources_v(s.slots[buf], x.kh, t0, t1, i + NB - UK);
             wait_unit();
             uint32_t kw[32];
 #pragma unroll
@@ -426,10 +444,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
                                         : 0u;
             }
             free_unit();
-            if constexpr (i + NB < UK)
-                issue_k(s.slots[buf], x.kh, i + NB);
-            else
-                issue_v(s.slots[buf], x.kh, t0, t1, i + NB - UK);
+            issue(c);
             at = at + 1 == NB ? 0 : at + 1;
             if (k0 <= x.hi && k0 + 63 >= x.lo) {
 #pragma unroll
@@ -563,6 +578,9 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
         const int units = ((t1 - t0 + 1) * kTile + C::kKeysV - 1) / C::kKeysV;
         const int rounds = max(units, NB);
         for (int i = 0; i < rounds; ++i) {
+            const Sources c = i + NB < rounds
+                                  ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
+                                  : sources_k(s.slots[buf ^ 1], y.kh, i + NB - rounds);
             wait_unit();
             uint32_t vw[C::kKeysV][WV];
 #pragma unroll
@@ -579,10 +597,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
                 }
             }
             free_unit();
-            if (i + NB < rounds)
-                issue_v(s.slots[buf], x.kh, t0, t1, i + NB);
-            else
-                issue_k(s.slots[buf ^ 1], y.kh, i + NB - rounds);
+            issue(c);
             at = at + 1 == NB ? 0 : at + 1;
             if (i < units) {
 #pragma unroll

@@ -686,6 +686,45 @@ def test_attention_has_the_contiguous_bits(pcl, torch, ctx, dtype, heads, window
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(4, 4, 64), (16, 2, 64), (12, 1, 64), (8, 4, 128), (5, 1, 128),
+                                   (16, 8, 256), (14, 2, 256), (4, 2, 512), (16, 2, 512),
+                                   (16, 1, 512), (2, 1, 496)],
+                         ids=lambda h: "x".join(map(str, h)))
+def test_launches_of_few_items(pcl, torch, ctx, dtype, heads):
+    # every item with a CU to itself: the kernels with two buffers a wave
+    for lengths in ([1], [100], [257, 40], [64, 2, 700]):
+        cache = Cache(pcl, torch, heads, lengths, 16, dtype, sum(lengths))
+        q = torch.randn((len(lengths), heads[0] * heads[2]), device="cuda:0")
+        out = cache.attend(ctx, q, max_length=max(lengths))
+        loose = cache.attend(ctx, q)
+        assert ctx.sync() == 0
+        for b, n in enumerate(lengths):
+            want = cache.contiguous(ctx, q[b:b + 1], b)
+            assert np.array_equal(bits(out[b] + 0.0), bits(want + 0.0)), (lengths, b)
+            assert np.array_equal(bits(loose[b]), bits(out[b]))
+            exact = cache.plain(q[b], b)
+            assert float((out[b].double() - exact).abs().max()) <= tolerance(n, heads[2])
+        assert ctx.sync() == 0
+
+
+@pytest.mark.gpu
+def test_uniform_batches_of_whole_chunks(pcl, torch, ctx):
+    # more items than workgroups: each takes several, full chunks throughout
+    for heads, dtype in (((16, 8, 256), "bf16"), ((16, 2, 512), "f32"), ((4, 4, 64), "bf16")):
+        cache = Cache(pcl, torch, heads, [2048] * 24, 64, dtype, 77)
+        q = torch.randn((24, heads[0] * heads[2]), device="cuda:0")
+        first = cache.attend(ctx, q)
+        again = cache.attend(ctx, q)
+        assert ctx.sync() == 0
+        assert np.array_equal(bits(first), bits(again))
+        for b in (0, 11, 23):
+            want = cache.contiguous(ctx, q[b:b + 1], b)
+            assert np.array_equal(bits(first[b] + 0.0), bits(want + 0.0))
+        assert ctx.sync() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads", [(16, 8, 256), (16, 2, 512)], ids=["d256", "d512"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_long_requests(pcl, torch, ctx, heads, dtype):
@@ -1065,6 +1104,42 @@ def test_a_batch_through_its_life(pcl, torch, heads, window, dtype, captured):
     server.transform.close()
     ctx.close()
     plain.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dtype", [((12, 1, 128), "bf16"), ((8, 1, 256), "f32"),
+                                         ((9, 3, 112), "bf16")], ids=str)
+def test_a_first_call_inside_a_capture(pcl, torch, heads, dtype):
+    # nothing of a kernel's setup needs a call before the capture
+    stream = torch.cuda.Stream()
+    cache = Cache(pcl, torch, heads, [300, 5, 900], 16, dtype, 9)
+    qheads, _, dim = heads
+    q = torch.randn((3, qheads * dim), device="cuda:0")
+    out = torch.full_like(q, 9.5)
+    torch.cuda.synchronize()
+    ctx = pcl.Context(0, stream.cuda_stream)
+    d = ctx.paged_desc(
+        pools=cache.pools.desc, q=q.data_ptr(), q_stride=qheads * dim, q_rows=3, qheads=qheads,
+        table=cache.table.data_ptr(), table_stride=cache.stride,
+        lengths=cache.dlengths.data_ptr(), requests=3, max_length=900, q_scale=scale_of(dim),
+        out=out.data_ptr(), o_stride=qheads * dim)
+    ctx.reserve(ctx.paged_workspace_bytes(d))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ctx.paged_attention(d)
+    for i in range(4):
+        q.normal_()
+        out.fill_(9.5)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for b in range(3):
+            want = cache.contiguous(ctx, q[b:b + 1], b)
+            assert np.array_equal(bits(out[b] + 0.0), bits(want + 0.0))
+        assert ctx.sync() == 0
+    graph.reset()
+    ctx.close()
 
 
 @pytest.mark.gpu
