@@ -27,14 +27,11 @@ __global__ __launch_bounds__(kCombineMost) void paged_combine_kernel(PagedParams
 {
     __shared__ f4 so[kCombineMost];
     __shared__ float sm[kCombineMost], sl[kCombineMost];
-    const int b = blockIdx.x;
-    const uint32_t base = p.ws_off[b];
-    const int nch = (int)(p.ws_off[b + 1] - base);
-    if (nch <= 1)
+    const int4 req = p.ws_req[blockIdx.x]; // (one load; all that a request's lanes need)
+    if (req.y <= 1)
         return;
-    bool unused = false;
-    const RequestKeys rk = request_keys(p, b, &unused);
-    const int c0 = rk.first / kChunk, c1 = c0 + nch; // the request's chunks
+    const uint32_t base = (uint32_t)req.x;
+    const int c0 = req.z, c1 = c0 + req.y; // the request's chunks
     const int s0 = c0 / kSpanChunks, s1 = (c1 - 1) / kSpanChunks + 1;
     const int tid = threadIdx.x;
     const int q = tid % c.lanes, gi = tid / c.lanes % c.spans;
@@ -90,7 +87,7 @@ __global__ __launch_bounds__(kCombineMost) void paged_combine_kernel(PagedParams
         v[j] = t.acc[j] / t.L;
         nonfinite |= !is_finite(v[j]);
     }
-    stg4(p.out + rk.row * p.o_stride + (int64_t)h * p.dim + d, v);
+    stg4(p.out + req.w * p.o_stride + (int64_t)h * p.dim + d, v);
     if (nonfinite)
         atomicOr(p.err, kErrOutput);
 }
@@ -158,15 +155,15 @@ static int check_paged(const pcl_paged_desc &d)
     return PCL_OK;
 }
 
-// Workspace bytes: the chunk partials of every request at its longest (none
-// where no request can have two chunks), then the chunk offsets.
+// Workspace bytes: four words of every request, then their chunk partials at the
+// requests' longest (none where no request can have two chunks).
 static size_t paged_bytes(const pcl_paged_desc &d)
 {
     if (d.requests == 0)
         return 0;
     const int64_t each = most_chunks(d);
     const size_t parts = each > 1 ? (size_t)(d.requests * each) * d.qheads : 0;
-    return parts * (d.pools.dim + 2) * sizeof(float) + (d.requests + 1) * sizeof(uint32_t);
+    return d.requests * sizeof(int4) + parts * (d.pools.dim + 2) * sizeof(float);
 }
 
 } // namespace pcl
@@ -209,9 +206,9 @@ int pcl_paged_attention(pcl_context *ctx, const pcl_paged_desc *desc)
     p.out = d.out;
     p.o_stride = d.o_stride;
     const int64_t parts = each > 1 ? d.requests * each * d.qheads : 0;
-    p.ws_o = body;
-    p.ws_ml = body + parts * s.dim;
-    p.ws_off = reinterpret_cast<uint32_t *>(body + parts * (s.dim + 2));
+    p.ws_req = reinterpret_cast<int4 *>(body);
+    p.ws_o = body + 4 * d.requests;
+    p.ws_ml = p.ws_o + parts * s.dim;
     p.err = ctx->err;
     p.requests = (int)d.requests;
     p.q_rows = (int)d.q_rows;

@@ -275,8 +275,9 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kerne
 
     fill_request_words(p, req, waves);
     if (blockIdx.x == 0)
-        for (int i = tid; i <= p.requests; i += C::kThreads)
-            p.ws_off[i] = req.off[i];
+        for (int i = tid; i < p.requests; i += C::kThreads)
+            p.ws_req[i] = int4{(int)req.off[i], (int)(req.off[i + 1] - req.off[i]),
+                               first_key(p, req.len[i]) / kChunk, req.row[i]};
     const uint32_t items = __builtin_amdgcn_readfirstlane(req.off[p.requests]) *
                            (uint32_t)(p.kvheads * p.units);
     if (blockIdx.x >= items)

@@ -18,7 +18,8 @@ struct PagedParams {
     float *out;
     int64_t o_stride;
     float *ws_o, *ws_ml; // [chunk][qheads][dim], [chunk][qheads][2]
-    uint32_t *ws_off;    // [requests + 1] chunks before a request
+    int4 *ws_req;        // [requests] for the combine: chunks before it, its chunks,
+                         // its first chunk, its row
     int *err;
     int requests, q_rows, max_length, window, pages;
     uint32_t page_tokens;
