@@ -931,6 +931,16 @@ int launch_plan(pcl_context *ctx, const pcl_attention_desc &desc, Plan *plan)
 
 } // namespace
 
+int pcl::open_timed_span(pcl_context *ctx, int role)
+{
+    return open_span(ctx, role);
+}
+
+void pcl::close_timed_span(pcl_context *ctx, int span)
+{
+    close_span(ctx, span);
+}
+
 bool pcl::stream_capturing(hipStream_t stream)
 {
     return capturing(stream);

@@ -70,6 +70,11 @@ int kv_cache_reserve(pcl_kv_cache *c, int64_t n);
 // Records the step in *pending and counts its n rows (written at row len).
 void kv_cache_advance_rows(pcl_kv_cache *c, int64_t n, pcl_kv_pending *pending);
 
+// A timed span of `role` on the context's stream, opened and closed around its
+// launches (nothing while timing is off).
+int open_timed_span(pcl_context *ctx, int role);
+void close_timed_span(pcl_context *ctx, int span);
+
 // True while `stream` is being captured into a graph.
 bool stream_capturing(hipStream_t stream);
 

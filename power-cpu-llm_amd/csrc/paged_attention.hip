@@ -94,7 +94,10 @@ __global__ __launch_bounds__(kCombineMost) void paged_combine_kernel(PagedParams
 
 // Groups of the combine: as many spans at once as some four thousand waves
 // allow (one long request: 32, each a round trip or two; 64 requests of 16
-// heads of 256 dims: 4), the fewer the wider.
+// heads of 256 dims: 4), the fewer the wider. In groups of 8 lanes and 32 spans
+// throughout, 256 requests of up to 2048 keys took 48 us here (5.6 now), 64 of up to
+// 8192 keys 27 us (5.6). Batches of 16 loads from 4 spans on were 1 to 3 us slower
+// (146 registers against 114), 2048 or 8192 waves within 1 us.
 static hipError_t launch_paged_combine(const PagedParams &p, int64_t chunks, hipStream_t stream)
 {
     auto pow2_to = [](int64_t n, int most) { // the least power of two >= n, at most `most`
@@ -226,12 +229,17 @@ int pcl_paged_attention(pcl_context *ctx, const pcl_paged_desc *desc)
     p.inv_softcap = d.softcap > 0.0f ? 1.0f / d.softcap : 0.0f;
     const int64_t chunks = d.requests * each;
     const bool bf16 = s.type == PCL_CACHE_BF16;
+    int span = pcl::open_timed_span(ctx, 0);
     hipError_t e = p.dim <= 64    ? pcl::launch_paged_kv<64>(p, bf16, chunks, ctx->stream)
                    : p.dim <= 128 ? pcl::launch_paged_kv<128>(p, bf16, chunks, ctx->stream)
                    : p.dim <= 256 ? pcl::launch_paged_kv<256>(p, bf16, chunks, ctx->stream)
                                   : pcl::launch_paged_kv<512>(p, bf16, chunks, ctx->stream);
-    if (e == hipSuccess && each > 1)
+    pcl::close_timed_span(ctx, span);
+    if (e == hipSuccess && each > 1) {
+        span = pcl::open_timed_span(ctx, 1);
         e = pcl::launch_paged_combine(p, each, ctx->stream);
+        pcl::close_timed_span(ctx, span);
+    }
     if (e != hipSuccess) {
         std::fprintf(stderr, "pcl_paged_attention: launch: %s\n", hipGetErrorString(e));
         return PCL_NON_FINITE_VALUE;

@@ -19,13 +19,16 @@
 // KV head do not pay for sixteen. A request of one chunk is written at once; the
 // others leave chunk partials in the workspace for paged_combine_kernel.
 //
-// Bound by HBM where the lengths add up to some hundred MB: 64 requests of up to
-// 8192 keys, 16 x 8 x 256 heads in bf16, 0.86 GB, 155 us (5.5 TB/s), 148 of them
-// here and 7 in the combine; 16 of up to 32768, 16 x 2 x 512, f32, 1.71 GB, 305
-// us (5.6 TB/s); 256 of up to 2048, 32 x 8 x 128, bf16, 0.45 GB, 101 us (4.4
-// TB/s: most items are partial chunks). Below that by the chain of an item: the
+// Bound by HBM where the lengths add up to some hundred MB (MI355X, cold inputs;
+// a call with its combine, the figures in brackets without): 64 requests of up
+// to 8192 keys, 16 x 8 x 256 heads in bf16, 0.86 GB, 150 us (143: 6.0 TB/s); 16 of
+// up to 32768, 16 x 2 x 512, f32, 1.71 GB, 300 us (289: 5.9 TB/s); 32 with a
+// 1024-key window, 16 x 8 x 256, f32, 0.54 GB, 96 us (91: 5.9 TB/s); one of 131072,
+// 16 x 2 x 512, bf16, 0.54 GB, 109 us (98: 5.5 TB/s, two rounds of items); 256 of
+// up to 2048, 32 x 8 x 128, bf16, 0.45 GB, 101 us (95: 4.7 TB/s, most items are
+// partial chunks of 128 KiB at most). Below that by the chain of an item: the
 // lengths, the table, K, two meetings of the waves, V (one request of 100 keys:
-// 12 us).
+// 11.3 us).
 //
 // How it came there (the first case): canonical 16 x 16 x 4 MFMAs fed from
 // registers 291 us; 4 x 4 x 1 ones, a lane loading its own key's row, 345 us with
@@ -260,8 +263,12 @@ __device__ __forceinline__ PagedItem find_item(const PagedParams &p, const Reque
 // FULL: the head dim equals the padded head dim DK. Every wave keeps memory
 // busy through an item: the next item's pages and query are requested ahead of
 // the scores, the first V before the softmax, the next item's K with the last V.
+//
+// Three waves a SIMD (168 registers, no spill) up to eight query rows: 1 % faster
+// than the two or three that the compiler left room for.
 template <int DK, typename T, bool FULL, int R, int NB>
-__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_kv_kernel(PagedParams p)
+__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
+                             (FULL && R <= 2 && NB == 1 ? 3 : 1)) void paged_kv_kernel(PagedParams p)
 {
     using C = PagedCfg<DK, T, R>;
     constexpr int KG = C::KG, KP = C::KP, UK = C::UK, VL = C::VL, NQ = C::NQ;

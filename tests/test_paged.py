@@ -300,6 +300,29 @@ def test_workspace_holds_every_chunk_of_every_request(pcl):
     assert nbytes(max_length=256, requests=0) == 0
 
 
+@pytest.mark.parametrize("source,kernel", [
+    # 16/8/256 heads in f32 and bf16 pages: many items, and few
+    ("paged_kv_d256.hip", "_ZN3pcl15paged_kv_kernelILi256EfLb1ELi1ELi1EEEvNS_11PagedParamsE"),
+    ("paged_kv_d256.hip", "_ZN3pcl15paged_kv_kernelILi256EDF16bLb1ELi1ELi1EEEvNS_11PagedParamsE"),
+    ("paged_kv_d256.hip", "_ZN3pcl15paged_kv_kernelILi256EfLb1ELi1ELi2EEEvNS_11PagedParamsE"),
+    ("paged_kv_d256.hip", "_ZN3pcl15paged_kv_kernelILi256EfLb1ELi2ELi1EEEvNS_11PagedParamsE"),
+    ("paged_attention.hip",
+     "_ZN3pcl20paged_combine_kernelILi8EEEvNS_11PagedParamsENS_12CombineShapeE"),
+    ("head_transform.hip",
+     "_ZN3pcl22paged_transform_kernelILi256ELi16EDF16bEEvNS_15TransformParamsE"),
+])
+def test_paged_kernels_do_not_spill_registers(source, kernel):
+    # the chunk kernel is held to three waves a SIMD: a spill would cost every
+    # unit of K and V
+    import os
+    from test_boundary import _resource_remarks
+    if not os.path.exists("/opt/rocm/bin/hipcc"):
+        pytest.skip("hipcc absent")
+    spills = _resource_remarks(source)
+    assert kernel in spills, sorted(spills)
+    assert spills[kernel] == 0
+
+
 # ---- on the device ----------------------------------------------------------
 
 @pytest.fixture(scope="module")
@@ -904,6 +927,24 @@ def test_many_requests(pcl, torch, ctx):
             continue
         want = cache.contiguous(ctx, q[b:b + 1], b)
         assert np.array_equal(bits(out[b] + 0.0), bits(want + 0.0)), b
+
+
+@pytest.mark.gpu
+def test_timing_counts_the_launches(pcl, torch):
+    own = pcl.Context(0)
+    cache = Cache(pcl, torch, (4, 2, 64), [700, 40], 16, "f32", 22)
+    q = torch.randn((2, 256), device="cuda:0")
+    cache.attend(own, q)
+    own.set_timing(True)
+    cache.attend(own, q)
+    cache.attend(own, q, rows=[-1, 1], max_length=40)  # (one chunk at most: no combine)
+    assert own.sync() == 0  # (the longer request has no row)
+    ms, launches = own.timing()
+    assert launches == (2, 1) and ms[0] > 0 and ms[1] > 0
+    own.set_timing(False)
+    cache.attend(own, q)
+    assert own.timing()[1] == (0, 0)
+    own.close()
 
 
 @pytest.mark.gpu
