@@ -365,7 +365,7 @@ int ensure_workspace(pcl_context *ctx, size_t bytes)
     if (ctx->ws) {
         (void)hipStreamSynchronize(ctx->stream);
         if (ctx->ws_captured)
-            ctx->ws_retired.push_back(ctx->ws);
+            pcl::retire(ctx->ws_retired, ctx->ws);
         else
             (void)hipFree(ctx->ws);
         ctx->ws = nullptr;

@@ -70,6 +70,17 @@ int kv_cache_reserve(pcl_kv_cache *c, int64_t n);
 // Records the step in *pending and counts its n rows (written at row len).
 void kv_cache_advance_rows(pcl_kv_cache *c, int64_t n, pcl_kv_pending *pending);
 
+// Keeps a device allocation that a captured graph holds until its owner goes;
+// with no memory for the record it is never freed (no exception leaves the
+// library).
+template <typename T> void retire(std::vector<T *> &kept, T *old)
+{
+    try {
+        kept.push_back(old);
+    } catch (...) {
+    }
+}
+
 // A timed span of `role` on the context's stream, opened and closed around its
 // launches (nothing while timing is off).
 int open_timed_span(pcl_context *ctx, int role);

@@ -345,7 +345,7 @@ int ensure_table(pcl_head_transform *t, int64_t end)
         return PCL_RESOURCE_LIMIT;
     }
     if (t->tab && t->captured)
-        t->retired.push_back(t->tab);
+        pcl::retire(t->retired, t->tab);
     else if (t->tab)
         (void)hipFree(t->tab);
     t->tab = tab;

@@ -264,11 +264,11 @@ __device__ __forceinline__ PagedItem find_item(const PagedParams &p, const Reque
 // busy through an item: the next item's pages and query are requested ahead of
 // the scores, the first V before the softmax, the next item's K with the last V.
 //
-// Three waves a SIMD (168 registers, no spill) up to eight query rows: 1 % faster
-// than the two or three that the compiler left room for.
+// Three waves a SIMD (168 registers, no spill) for four query rows: 1 % faster
+// than the two or three that the compiler left room for; eight rows would spill.
 template <int DK, typename T, bool FULL, int R, int NB>
 __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
-                             (FULL && R <= 2 && NB == 1 ? 3 : 1)) void paged_kv_kernel(PagedParams p)
+                             (FULL && R == 1 && NB == 1 ? 3 : 1)) void paged_kv_kernel(PagedParams p)
 {
     using C = PagedCfg<DK, T, R>;
     constexpr int KG = C::KG, KP = C::KP, UK = C::UK, VL = C::VL, NQ = C::NQ;
@@ -349,24 +349,32 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
     uint32_t *const ring = dyn + (size_t)w * NB * 2048;
     int at = 0;
     const uint32_t row_bytes = (uint32_t)(p.row_stride * sizeof(T));
-    // Where a unit's eight copies read: worked out before the wait for the unit
-    // in their buffer, whose slots' LDS round trips it hides.
+    // Where a unit's eight copies read.
     struct Sources {
         const char *from[8];
     };
-    // K unit i of an item: row 8 e + lane / 8 of the group, the line's 16-byte
-    // pieces in the order piece ^ (row & 7), so that a lane's reads of its own
-    // row fall in other banks than its neighbours'
-    auto sources_k = [&](const int32_t *slots, int kh, int i) {
-        const int line = i % KP;
-        const int d = C::kLine * line + (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
-        const char *base = static_cast<const char *>(p.k) +
-                           ((int64_t)kh * p.dim + (FULL || d < p.dim ? d : 0)) * sizeof(T);
-        const int32_t *mine = slots + 64 * (w * KG + i / KP) + lane / 8;
+    // Key group kg's K rows 8 e + lane / 8, each at the lane's 16-byte piece of the
+    // line's: the pieces of row r lie in the order piece ^ (r & 7), so that a
+    // lane's reads of its own row fall in other banks than its neighbours'.
+    const int piece = (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
+    auto rows_k = [&](const int32_t *slots, int kh, int kg) {
+        const char *base =
+            static_cast<const char *>(p.k) + ((int64_t)kh * p.dim + piece) * sizeof(T);
+        const int32_t *mine = slots + 64 * (w * KG + kg) + lane / 8;
         Sources c;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             c.from[e] = base + (uint64_t)(uint32_t)mine[8 * e] * row_bytes;
+        return c;
+    };
+    // line `line` of those rows (a piece past the head dim: the row's first one)
+    auto line_k = [&](const Sources &rows, int line) {
+        const int d = C::kLine * line;
+        const int64_t step = (FULL || d + piece < p.dim ? d : -piece) * (int64_t)sizeof(T);
+        Sources c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            c.from[e] = rows.from[e] + step;
         return c;
     };
     // V unit i of the tiles from t0 to t1 (past them the last tile again): its
@@ -410,7 +418,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NB; ++i, at = at + 1 == NB ? 0 : at + 1)
-        issue(sources_k(s.slots[0], x.kh, i));
+        issue(line_k(rows_k(s.slots[0], x.kh, i / KP), i % KP));
 
     int buf = 0;
     for (uint32_t item = blockIdx.x;; buf ^= 1) {
@@ -427,19 +435,26 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         // scores: lane = key
         f4 acc[KG][R];
         bool bad = false;
+        // The copies behind a consumed unit go out once it is read, from sources
+        // worked out during the unit before; the query is read ahead of the wait
+        // (16 requests of up to 8192 keys, 32 query heads and one KV head of 128
+        // dims, bf16: 50 -> 42 us; one request of 300 keys, 16 x 2 x 512: 32 -> 31).
+        Sources rows = rows_k(s.slots[buf], x.kh, NB / KP % KG);
+        Sources c = NB < UK ? line_k(rows, NB % KP) : sources_v(s.slots[buf], x.kh, t0, t1, 0);
         each<UK>([&](auto ic) {
-            constexpr int i = decltype(ic)::value, kg = i / KP;
+            constexpr int i = decltype(ic)::value, kg = i / KP, M = C::kLine / 16;
             const int k0 = 64 * (w * KG + kg);
             if (i % KP == 0) {
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                     acc[kg][r] = f4{0.f, 0.f, 0.f, 0.f};
             }
-            Sources c;
-            if constexpr (i + NB < UK)
-                c = sources_k(s.slots[buf], x.kh, i + NB);
-            else
-                c = sources_v(s.slots[buf], x.kh, t0, t1, i + NB - UK);
+            float a[M][R];
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    a[m][r] = s.q[r][C::kLine * (i % KP) + 16 * m + lane / 4][lane % 4];
             wait_unit();
             uint32_t kw[32];
 #pragma unroll
@@ -454,21 +469,27 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             free_unit();
             issue(c);
             at = at + 1 == NB ? 0 : at + 1;
+            constexpr int n1 = i + 1 + NB; // the unit that the next consumed one makes room for
+            if constexpr (i + 1 < UK) {
+                if constexpr (n1 < UK) {
+                    if constexpr (n1 % KP == 0)
+                        rows = rows_k(s.slots[buf], x.kh, n1 / KP);
+                    c = line_k(rows, n1 % KP);
+                } else {
+                    c = sources_v(s.slots[buf], x.kh, t0, t1, n1 - UK);
+                }
+            }
             if (k0 <= x.hi && k0 + 63 >= x.lo) {
-#pragma unroll
-                for (int m = 0; m < C::kLine / 16; ++m) {
-                    float a[R];
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        a[r] = s.q[r][C::kLine * (i % KP) + 16 * m + lane / 4][lane % 4];
+                each<M>([&](auto mc) {
+                    constexpr int m = decltype(mc)::value;
                     each<16>([&](auto nc) {
                         constexpr int n = decltype(nc)::value;
                         const float k = value_of<T>(kw, chain_dim(16 * m + n));
 #pragma unroll
                         for (int r = 0; r < R; ++r)
-                            acc[kg][r] = mfma_rows4<n>(a[r], k, acc[kg][r]);
+                            acc[kg][r] = mfma_rows4<n>(a[m][r], k, acc[kg][r]);
                     });
-                }
+                });
             }
         });
 
@@ -555,7 +576,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
                 O[r][v] = f4{0.f, 0.f, 0.f, 0.f};
         }
         // 16 keys from chain step n0 of tile t; word(n): the words of step n
-        auto attend = [&](int t, int half, auto word) {
+        auto attend = [&](int t, int half, const float (&a)[R], auto word) {
             if (half == 0) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -568,10 +589,6 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
                         O[r][j] = O[r][j] * alpha;
                 }
             }
-            float a[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                a[r] = s.p[r][t][16 * half + lane / 4][lane % 4];
             each<16>([&](auto nc) {
                 constexpr int n = decltype(nc)::value;
                 const uint32_t *v = word(n);
@@ -585,10 +602,22 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         constexpr int WV = (VL * (int)sizeof(T) + 3) / 4; // words of a lane's values
         const int units = ((t1 - t0 + 1) * kTile + C::kKeysV - 1) / C::kKeysV;
         const int rounds = max(units, NB);
+        // the unit that V unit i makes room for
+        auto behind_v = [&](int i) {
+            const int n = i + NB - rounds; // the next item's first units follow this one's
+            return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
+                         : line_k(rows_k(s.slots[buf ^ 1], y.kh, n / KP), n % KP);
+        };
+        c = behind_v(0);
         for (int i = 0; i < rounds; ++i) {
-            const Sources c = i + NB < rounds
-                                  ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
-                                  : sources_k(s.slots[buf ^ 1], y.kh, i + NB - rounds);
+            float a[C::kKeysV / 16][R];
+#pragma unroll
+            for (int h = 0; h < C::kKeysV / 16; ++h) {
+                const int n = C::kKeysV * i + 16 * h, t = min(t0 + n / kTile, t1);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    a[h][r] = s.p[r][t][n % kTile + lane / 4][lane % 4];
+            }
             wait_unit();
             uint32_t vw[C::kKeysV][WV];
 #pragma unroll
@@ -607,6 +636,8 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             free_unit();
             issue(c);
             at = at + 1 == NB ? 0 : at + 1;
+            if (i + 1 < rounds)
+                c = behind_v(i + 1);
             if (i < units) {
 #pragma unroll
                 for (int h = 0; h < C::kKeysV / 16; ++h) {
@@ -614,7 +645,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
                     if (C::kKeysV > kTile && t > t1)
                         continue;
                     const int half = C::kKeysV < kTile ? i % 2 : h % 2;
-                    attend(t, half, [&](int k) { return vw[16 * h + k]; });
+                    attend(t, half, a[h], [&](int k) { return vw[16 * h + k]; });
                 }
             }
         }

@@ -966,6 +966,32 @@ def test_another_stream(pcl, torch):
     own.close()
 
 
+@pytest.mark.gpu
+def test_two_contexts_at_once(pcl, torch):
+    # each has its stream, workspace and error flag; the pages are shared
+    heads = (16, 8, 256)
+    cache = Cache(pcl, torch, heads, [3000] * 12, 16, "bf16", 23)
+    q = [torch.randn((12, 16 * 256), device="cuda:0") for _ in range(2)]
+    out = [torch.zeros_like(x) for x in q]
+    own = [pcl.Context(0) for _ in q]
+    descs = [c.paged_desc(
+        pools=cache.pools.desc, q=x.data_ptr(), q_stride=16 * 256, q_rows=12, qheads=16,
+        table=cache.table.data_ptr(), table_stride=cache.stride,
+        lengths=cache.dlengths.data_ptr(), requests=12, max_length=3000, q_scale=scale_of(256),
+        out=o.data_ptr(), o_stride=16 * 256) for c, x, o in zip(own, q, out)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, d in zip(own, descs):
+            c.paged_attention(d)
+    assert [c.sync() for c in own] == [0, 0]
+    for c, x, o in zip(own, q, out):
+        for b in (0, 5, 11):
+            want = cache.contiguous(c, x[b:b + 1], b)
+            assert c.sync() == 0
+            assert np.array_equal(bits(o[b] + 0.0), bits(want + 0.0))
+        c.close()
+
+
 # ---- a run of them together -------------------------------------------------
 
 class Server:
