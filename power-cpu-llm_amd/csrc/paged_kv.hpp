@@ -118,7 +118,8 @@ template <int BLOCK> __device__ __forceinline__ f4 mfma_rows4(float a, float b, 
 }
 
 // Head dim of the n-th step of the canonical score chain (u, jj, g), and the
-// key of a tile at the n-th step of the canonical P.V chain (b, r, g).
+// key of a tile at the n-th step of the canonical P.V chain (b, r, g); the
+// latter is its own inverse.
 __host__ __device__ constexpr int chain_dim(int n)
 {
     return 32 * (n / 32) + 8 * (n % 4) + n % 32 / 4;
@@ -126,7 +127,7 @@ __host__ __device__ constexpr int chain_dim(int n)
 
 __host__ __device__ constexpr int chain_key(int n)
 {
-    return 16 * (n / 16) + 4 * (n % 4) + n % 16 / 4;
+    return (n & 16) + 4 * (n & 3) + (n >> 2 & 3);
 }
 
 template <int CTRL> __device__ __forceinline__ float dpp(float x)
@@ -405,10 +406,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         for (int e = 0; e < 8; ++e) {
             const int n = C::kKeysV * i + (e * 64 + lane) / C::kLanesV; // chain step from tile t0 on
             const int t = min(t0 + n / kTile, t1), k = n % kTile;
-            c.from[e] =
-                base +
-                (uint64_t)(uint32_t)slots[kTile * t + (k & 16) + 4 * (k & 3) + (k >> 2 & 3)] *
-                    row_bytes;
+            c.from[e] = base + (uint64_t)(uint32_t)slots[kTile * t + chain_key(k)] * row_bytes;
         }
         return c;
     };
@@ -569,8 +567,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
                     alpha[e] = fexp(before[e] - ms);
                     sum[e] = sum_tile(pr[e]);
                 }
-                const int k = key % kTile;
-                *(f4 *)s.p[r][t][(k & 16) + 4 * (k & 3) + (k >> 2 & 3)] = pr;
+                *(f4 *)s.p[r][t][chain_key(key % kTile)] = pr;
                 if ((lane & 31) == 0) {
                     s.alpha[t][r] = alpha;
                     s.sum[t][r] = sum;
@@ -592,7 +589,8 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             for (int v = 0; v < VL; ++v)
                 O[r][v] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        // 16 keys from chain step n0 of tile t; word(n): the words of step n
+        // 16 chain steps of tile t, its first or second half; a: their
+        // probabilities, word(n): the words of step n
         auto attend = [&](int t, int half, const float (&a)[R], auto word) {
             if (half == 0) {
 #pragma unroll
