@@ -28,6 +28,7 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
+    "-pthread",
     "-shared",
     # No contraction: every multiply-add the kernels mean to fuse is written
     # as an explicit fma, so all kernels share one operation sequence.

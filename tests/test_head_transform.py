@@ -298,6 +298,52 @@ def test_device_transform_matches_the_oracle(pcl, torch, ctx, oracle, case):
 
 
 @pytest.mark.gpu
+def test_rotation_table_built_at_once_and_grown_in_steps(pcl, torch, ctx, oracle):
+    # 5001 rows at once are shared out to eight threads; the other table grows
+    # over 256, 512 and 1024 rows: every row has the same bits, and those at the
+    # seams are the oracle's
+    dim, n = 32, 5001
+    g = np.random.default_rng(41)
+    rows = g.standard_normal((n, dim)).astype(np.float32)
+    ones = np.ones(dim, np.float32)
+    x = dev(torch, rows)
+    outs = []
+    for steps in ((), (100, 300, 700)):
+        t = pcl.HeadTransform(ctx, 1, 1, dim, ones, ones, 1e-6, 10000.0)
+        out = torch.full((n, dim), float("nan"), device="cuda:0")
+        for p in steps:
+            t.query(x.data_ptr(), 1, p, out.data_ptr())
+        t.query(x.data_ptr(), n, 0, out.data_ptr())
+        assert ctx.sync() == 0
+        outs.append(out.cpu().numpy())
+        t.close()
+    assert np.array_equal(bits(outs[0]), bits(outs[1]))
+    each = -(-n // 8)
+    for p in sorted({q + d for q in range(0, n, each) for d in (-1, 0) if q + d >= 0} | {n - 1}):
+        want, _, _ = oracle_tokens(oracle, rows[p:p + 1], rows[p:p + 1], None, 1, 1, 1, dim, p, ones,
+                                   ones, 1e-6, 10000.0, None)
+        assert_rotated_close(outs[0][p], want, dim)
+
+
+@pytest.mark.gpu
+def test_non_finite_angles_of_a_long_table_are_refused(pcl, torch, ctx):
+    # frequencies of 1e36: angles are finite up to position 340, and the rows
+    # past it are some threads' and not others'
+    ones = np.ones(32, np.float32)
+    t = pcl.HeadTransform(ctx, 1, 1, 32, ones, ones, 1e-6, 1.0 + 2.0 ** -20,
+                          factors=np.full(16, 1e-36, np.float32))
+    x = torch.ones(32, device="cuda:0")
+    out = torch.zeros(32, device="cuda:0")
+    t.query(x.data_ptr(), 1, 100, out.data_ptr())
+    with pytest.raises(pcl.AttentionError) as e:
+        t.query(x.data_ptr(), 1, 5000, out.data_ptr())
+    assert e.value.kind == "NonFiniteValue"
+    t.query(x.data_ptr(), 1, 100, out.data_ptr())  # the shorter table is still there
+    assert ctx.sync() == 0
+    t.close()
+
+
+@pytest.mark.gpu
 def test_transform_rejects_bad_geometry_parameters_and_inputs(pcl, torch, ctx):
     ones = np.ones(64, np.float32)
     with pytest.raises(pcl.AttentionError) as e:
