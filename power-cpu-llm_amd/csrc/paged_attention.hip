@@ -124,11 +124,13 @@ static hipError_t launch_paged_combine(const PagedParams &p, int64_t chunks, hip
     return hipGetLastError();
 }
 
-// Chunks that one request may have.
+// Chunks that one request may have. (A window is any positive int64_t: it is
+// held to the longest request before anything is added to it.)
 static int64_t most_chunks(const pcl_paged_desc &d)
 {
     const int64_t all = (d.max_length + kChunk - 1) / kChunk;
-    return d.window ? std::min(all, (d.window + kChunk - 2) / kChunk + 1) : all;
+    const int64_t window = std::min(d.window, d.max_length);
+    return window ? std::min(all, (window + kChunk - 2) / kChunk + 1) : all;
 }
 
 static int check_paged(const pcl_paged_desc &d)

@@ -300,6 +300,25 @@ def test_workspace_holds_every_chunk_of_every_request(pcl):
     assert nbytes(max_length=256, requests=0) == 0
 
 
+@pytest.mark.parametrize("window", [16384, 1 << 31, (1 << 63) - 255, (1 << 63) - 254,
+                                    (1 << 63) - 1])
+def test_a_window_past_the_longest_request_is_no_window(pcl, window):
+    # the whole range of the argument: the workspace is that of all keys, and so
+    # is the bound of the items
+    lib = pcl.load()
+
+    def nbytes(window, **kw):
+        kw = dict(dict(table_stride=64, max_length=16384), **kw)
+        return lib.pcl_paged_workspace_bytes(ctypes.byref(paged_of(
+            pcl, pools_of(pcl, page_tokens=256, pages=64), window=window, **kw)))
+
+    for n in (1, 256, 257, 1000, 16384):
+        assert nbytes(window, max_length=n) == nbytes(0, max_length=n) > 0
+    if window > 1 << 30:
+        many = dict(requests=2048, q_rows=2048, max_length=1 << 30, table_stride=1 << 30)
+        assert nbytes(window, **many) == nbytes(0, **many) == 0
+
+
 @pytest.mark.parametrize("source,kernel", [
     # 16/8/256 heads in f32 and bf16 pages: many items, and few
     ("paged_kv_d256.hip", "_ZN3pcl15paged_kv_kernelILi256EfLb1ELi1ELi1EEEvNS_11PagedParamsE"),
@@ -768,6 +787,24 @@ def test_long_requests(pcl, torch, ctx, heads, dtype):
         want = cache.contiguous(ctx, q[b:b + 1], b, 6000)
         assert np.array_equal(bits(windowed[b] + 0.0), bits(want + 0.0)), n
     assert ctx.sync() == 0
+
+
+@pytest.mark.gpu
+def test_a_window_without_a_limit(pcl, torch):
+    # windows up to the last int64_t attend every key, through a workspace of
+    # that launch alone
+    heads = (4, 2, 64)
+    cache = Cache(pcl, torch, heads, [700, 40, 3000], 16, "f32", 41)
+    q = torch.randn((3, 256), device="cuda:0")
+    for window in (3000, 1 << 40, (1 << 63) - 1):
+        torch.cuda.synchronize()
+        own = pcl.Context(0)
+        out = cache.attend(own, q, window=window)
+        for b in range(3):
+            want = cache.contiguous(own, q[b:b + 1], b)
+            assert np.array_equal(bits(out[b] + 0.0), bits(want + 0.0))
+        assert own.sync() == 0
+        own.close()
 
 
 @pytest.mark.gpu
