@@ -189,7 +189,8 @@ void *pcl_context_stream(pcl_context *ctx);
  * allowed score or output) are recorded in the context's device error flag.
  * Grows the context's workspace when needed (a device allocation);
  * pcl_context_reserve avoids that inside timed regions and before a graph
- * capture. On a stream that is capturing a graph, AUTO does not take the
+ * capture. A workspace that a captured launch holds is kept until the context
+ * is destroyed. On a stream that is capturing a graph, AUTO does not take the
  * spread decode (its workgroups accept a published word by the launch's
  * epoch, which every replay would repeat) but the pipelined kernel, with the
  * same bits; an explicit PCL_KERNEL_SPREAD_KV is refused there with
@@ -391,8 +392,10 @@ void pcl_head_transform_destroy(pcl_head_transform *transform);
  * sin and cos of each f32 angle, rounded once to f32: within an f32 ulp of
  * the reference's libm::sincosf, src/libm.rs:350, and equal to it for all
  * but about 0.1 % of angles) for positions up to the largest seen so far and
- * kept on the device; PCL_NON_FINITE_VALUE for a non-finite angle,
- * PCL_RESOURCE_LIMIT beyond 2^24 positions. A rotated Q or K value y_j
+ * kept on the device until the transform is destroyed, outgrown tables too (a
+ * captured launch may hold one); PCL_NON_FINITE_VALUE for a non-finite angle,
+ * PCL_RESOURCE_LIMIT beyond 2^24 positions, and inside a graph capture for a
+ * position past the table, which is not built there. A rotated Q or K value y_j
  * (pair j, j + dim/2) is therefore within 2^-20 * (|y_j| + |y_{j+dim/2}|)
  * of the reference's, and almost always equal to it; V rows are bit for
  * bit. */

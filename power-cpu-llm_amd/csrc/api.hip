@@ -358,6 +358,18 @@ int zero_tag_region(pcl_context *ctx, void *ws, size_t bytes, uint32_t *gen)
     return PCL_OK;
 }
 
+// True while `stream` is being captured into a graph (an error of the query
+// itself counts as not capturing and is cleared).
+bool capturing(hipStream_t stream)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &st) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return st != hipStreamCaptureStatusNone;
+}
+
 int ensure_workspace(pcl_context *ctx, size_t bytes)
 {
     if (bytes <= ctx->ws_bytes)
@@ -370,6 +382,7 @@ int ensure_workspace(pcl_context *ctx, size_t bytes)
             (void)hipFree(ctx->ws);
         ctx->ws = nullptr;
         ctx->ws_bytes = 0;
+        ctx->ws_captured = false;
     }
     hipError_t e = hipMalloc(&ctx->ws, bytes);
     if (e != hipSuccess) {
@@ -381,6 +394,16 @@ int ensure_workspace(pcl_context *ctx, size_t bytes)
     // a new buffer's score-word region starts at zero, an epoch no launch
     // takes
     return zero_tag_region(ctx, ctx->ws, bytes, &ctx->ws_tag_gen);
+}
+
+// ensure_workspace for a launch on ctx's stream that is given the workspace's
+// address: in a capture the graph holds it.
+int launch_workspace(pcl_context *ctx, size_t bytes)
+{
+    const int rc = ensure_workspace(ctx, bytes);
+    if (rc == PCL_OK && !ctx->ws_captured)
+        ctx->ws_captured = capturing(ctx->stream);
+    return rc;
 }
 
 hipEvent_t take_event(pcl_context *ctx)
@@ -509,7 +532,10 @@ int run_plan(pcl_context *ctx, Plan &plan)
     if (plan.empty)
         return PCL_OK;
     if (plan.ws_floats) {
-        const int rc = ensure_workspace(ctx, plan.ws_floats * sizeof(float));
+        // (a spread plan is not being captured: launch_plan)
+        const size_t bytes = plan.ws_floats * sizeof(float);
+        const int rc = plan.kernel == PCL_KERNEL_SPREAD_KV ? ensure_workspace(ctx, bytes)
+                                                           : launch_workspace(ctx, bytes);
         if (rc != PCL_OK)
             return rc;
     }
@@ -891,18 +917,6 @@ int pcl_debug_tiled_rows(const pcl_attention_desc *desc, int cus)
 
 namespace {
 
-// True while `stream` is being captured into a graph (an error of the query
-// itself counts as not capturing and is cleared).
-bool capturing(hipStream_t stream)
-{
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &st) != hipSuccess) {
-        (void)hipGetLastError();
-        return false;
-    }
-    return st != hipStreamCaptureStatusNone;
-}
-
 // The plan of a device-resident launch on ctx's stream. A launch being
 // captured into a graph never takes the spread decode: its workgroups accept
 // a published word by the launch's epoch, a kernel argument that every
@@ -954,12 +968,9 @@ size_t pcl::workspace_bytes_for(size_t body)
 int pcl::workspace_body(pcl_context *ctx, size_t bytes, float **body)
 {
     const size_t all = workspace_bytes_for(bytes);
-    if (capturing(ctx->stream)) {
-        if (all > ctx->ws_bytes)
-            return PCL_RESOURCE_LIMIT;
-        ctx->ws_captured = true;
-    }
-    const int rc = ensure_workspace(ctx, all);
+    if (all > ctx->ws_bytes && capturing(ctx->stream))
+        return PCL_RESOURCE_LIMIT;
+    const int rc = launch_workspace(ctx, all);
     if (rc == PCL_OK)
         *body = static_cast<float *>(ctx->ws) + kTagFloats;
     return rc;

@@ -28,9 +28,9 @@ struct pcl_context {
     // epoch generation for which the workspace's published-word region was
     // last zeroed
     uint32_t ws_tag_gen = 0;
-    // a captured paged attention holds the workspace's address: workspaces
-    // outgrown after such a capture are kept until the context is destroyed
-    bool ws_captured = false;
+    // a captured launch holds the workspace's address: one that is outgrown
+    // after such a capture is kept until the context is destroyed
+    bool ws_captured = false; // of `ws`
     std::vector<void *> ws_retired;
     int *err = nullptr;
     // this device's scratch of pcl_attention_launch_noalloc (never freed)

@@ -261,9 +261,9 @@ struct pcl_head_transform {
     float *scales = nullptr;    // device [2][dim]: query, key
     float *tab = nullptr;       // device (sin, cos) pairs [rows][dim/2][2]
     int64_t tab_rows = 0;
-    // a captured graph holds the table's address: a table that grows after
-    // such a capture is kept until the transform is destroyed
-    bool captured = false;
+    // a captured launch may hold the table's address, so one that is outgrown
+    // is kept until the transform is destroyed (tables double up to the last
+    // position there is: all of these together are smaller than two of `tab`)
     std::vector<float *> retired;
 };
 
@@ -340,11 +340,14 @@ bool rope_rows(const pcl_head_transform *t, int64_t from, int64_t to, float *out
     return finite.load(std::memory_order_relaxed);
 }
 
-// Table rows for positions [0, end): grown by doubling, built on the host.
+// Table rows for positions [0, end): grown by doubling, built on the host (and
+// so not in a capture).
 int ensure_table(pcl_head_transform *t, int64_t end)
 {
     if (end <= t->tab_rows)
         return PCL_OK;
+    if (pcl::stream_capturing(t->ctx->stream))
+        return PCL_RESOURCE_LIMIT;
     const int64_t half = t->dim / 2;
     const int64_t rows = std::min<int64_t>(
         kMaxPositions, std::max<int64_t>(end, std::max<int64_t>(2 * t->tab_rows, 256)));
@@ -372,10 +375,8 @@ int ensure_table(pcl_head_transform *t, int64_t end)
             (void)hipFree(tab);
         return PCL_RESOURCE_LIMIT;
     }
-    if (t->tab && t->captured)
+    if (t->tab)
         pcl::retire(t->retired, t->tab);
-    else if (t->tab)
-        (void)hipFree(t->tab);
     t->tab = tab;
     t->tab_rows = rows;
     return PCL_OK;
@@ -527,11 +528,6 @@ int pcl_paged_append_transformed(pcl_head_transform *t, const pcl_page_pools *po
         ((uintptr_t)raw_q | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)q_out) % 16)
         return PCL_INVALID_SHAPE;
     (void)hipSetDevice(t->ctx->device);
-    if (pcl::stream_capturing(t->ctx->stream)) {
-        if (position_limit > t->tab_rows) // the table cannot be built in a capture
-            return PCL_RESOURCE_LIMIT;
-        t->captured = true;
-    }
     const int rc = ensure_table(t, position_limit);
     if (rc != PCL_OK)
         return rc;

@@ -172,3 +172,148 @@ def test_output_block_replays_give_the_eager_bits(pcl, torch, n):
     finally:
         ctx.close()
         plain.close()
+
+
+def nan_blocks(torch, nbytes, count=24):
+    """Fresh device memory full of NaNs, where a freed block of `nbytes` would
+    be handed out again."""
+    blocks = [torch.full((max(nbytes // 4, 1),), float("nan"), device="cuda:0")
+              for _ in range(count)]
+    torch.cuda.synchronize()
+    return blocks
+
+
+@pytest.mark.parametrize("grow", ["reserve", "launch", "paged"])
+def test_a_captured_launch_keeps_its_workspace(pcl, torch, grow):
+    # the graph holds the workspace's address: a later call that needs a larger
+    # one leaves the old one to the graph
+    stream = torch.cuda.Stream()
+    ctx = pcl.Context(0, stream.cuda_stream)
+    try:
+        step = Step(torch, ctx, 16, 8, 256, 8192, kernel=pcl.KERNEL_PIPE_KV)
+        step.fill(torch, 0x6C0)
+        held = ctx.workspace_bytes(step.desc)
+        ctx.reserve(held)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ctx.launch(step.desc)
+        if grow == "reserve":
+            ctx.reserve(4 * held)
+        elif grow == "launch":
+            big = Step(torch, ctx, 16, 8, 256, 40000, kernel=pcl.KERNEL_PIPE_KV)
+            big.fill(torch, 0x6C1)
+            torch.cuda.synchronize()
+            ctx.launch(big.desc)
+        else:
+            k = torch.zeros((64, 256, 8, 256), device="cuda:0")
+            pools = pcl.page_pools(k=k.data_ptr(), v=k.data_ptr(), type=pcl.CACHE_F32, pages=64,
+                                   page_tokens=256, kvheads=8, dim=256)
+            table = torch.arange(64, device="cuda:0", dtype=torch.int32).repeat(4, 1)
+            lengths = torch.full((4,), 64 * 256, device="cuda:0", dtype=torch.int32)
+            q = torch.zeros((4, 16 * 256), device="cuda:0")
+            torch.cuda.synchronize()
+            ctx.paged_attention(ctx.paged_desc(
+                pools=pools, q=q.data_ptr(), q_stride=16 * 256, q_rows=4, qheads=16,
+                table=table.data_ptr(), table_stride=64, lengths=lengths.data_ptr(), requests=4,
+                max_length=64 * 256, out=q.data_ptr(), o_stride=16 * 256))
+        assert ctx.sync() == 0
+        blocks = nan_blocks(torch, held)
+        for rep in range(4):
+            step.fill(torch, 0x6C2 + rep)
+            step.out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = step.out.cpu().numpy()
+            assert ctx.sync() == 0
+            want = eager(torch, pcl, step, kernel=pcl.KERNEL_PIPE_KV)
+            assert np.array_equal(bits(got), bits(want)), rep
+            # nobody else's memory was written
+            assert all(bool(torch.isnan(b).all()) for b in blocks), rep
+        graph.reset()
+    finally:
+        ctx.close()
+
+
+@pytest.mark.parametrize("call", ["prepare", "query", "append", "attend_token"])
+def test_a_captured_transform_keeps_its_rotation_table(pcl, torch, call):
+    # the same of the table of a transform, which grows with the positions; a
+    # table that is too short is refused inside a capture, which goes on
+    qheads, kvh, dim, at = 16, 8, 256, 40
+    stream = torch.cuda.Stream()
+    ctx = pcl.Context(0, stream.cuda_stream)
+    plain = pcl.Context(0, torch.cuda.current_stream().cuda_stream)
+    rng = np.random.default_rng(7)
+    scales = [1.0 + 0.1 * rng.standard_normal(dim) for _ in range(2)]
+    # prepared queries, keys and values, and the attended output
+    shapes = [(1, h, dim) for h in (qheads, kvh, kvh, qheads)]
+    made = []
+
+    def side(c):
+        """A transform, a cache of `at` tokens and the outputs on context c."""
+        t = pcl.HeadTransform(c, qheads, kvh, dim, *scales, 1e-6, 10000.0)
+        cache = pcl.LayerCache(c, kvh, dim, 1 << 20, None, 1 << 30)
+        cache.reserve_rows(1024)
+        rows = torch.full((at, kvh, dim), 0.5, device="cuda:0")
+        torch.cuda.synchronize()
+        cache.append(rows.data_ptr(), rows.data_ptr(), at)
+        cache.commit()
+        assert c.sync() == 0
+        out = [torch.full(s, float("nan"), device="cuda:0") for s in shapes]
+        made.extend((cache, t))
+        return t, cache, out
+
+    def run(t, cache, out):
+        ptr = [x.data_ptr() for x in raw + out]
+        if call == "prepare":
+            t.prepare(*ptr[:3], 1, at, *ptr[3:6])
+        elif call == "query":
+            t.query(ptr[0], 1, at, ptr[3])
+        elif call == "append":
+            cache.append_transformed(t, *ptr[:3], 1, ptr[3])
+        else:
+            cache.attend_token(t, *ptr[:3], ptr[3], ptr[6], q_scale=0.0625)
+
+    try:
+        raw = [torch.randn(s, device="cuda:0") for s in shapes[:3]]
+        t, cache, out = side(ctx)
+        ctx.reserve(1 << 24)
+        t.query(raw[0].data_ptr(), 1, 0, out[0].data_ptr())  # builds the first rows
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out[3].mul_(1.0)
+            with pytest.raises(pcl.AttentionError) as e:
+                t.query(raw[0].data_ptr(), 1, 4000, out[0].data_ptr())
+            assert e.value.kind == "ResourceLimit"
+            run(t, cache, out)
+        # a far position: a longer table
+        t.query(raw[0].data_ptr(), 1, 5000, out[0].data_ptr())
+        assert ctx.sync() == 0
+        blocks = nan_blocks(torch, 256 * dim * 4)
+        for rep in range(4):
+            for x in raw:
+                x.normal_()
+            for x in out:
+                x.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert ctx.sync() == 0
+            t2, cache2, want = side(plain)
+            run(t2, cache2, want)
+            assert plain.sync() == 0
+            for got, x in zip(out, want):
+                assert np.array_equal(bits(got.cpu().numpy()), bits(x.cpu().numpy())), rep
+            if call in ("append", "attend_token"):
+                # the appended row (the replay writes it where the capture did)
+                for got, x in zip(cache.read(at, 1), cache2.read(at, 1)):
+                    assert np.array_equal(bits(got), bits(x)), rep
+            assert all(bool(torch.isnan(b).all()) for b in blocks), rep
+        graph.reset()
+    finally:
+        for x in made:
+            x.close()
+        ctx.close()
+        plain.close()
