@@ -140,14 +140,14 @@ __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
 template <bool KEEP> __global__ __launch_bounds__(kPageThreads) void page_return_kernel(PageParams p)
 {
     extern __shared__ uint32_t offsets[]; // returned pages before a request [requests + 1]
-    __shared__ uint32_t waves[kPageThreads / 64];
+    __shared__ uint64_t waves[kPageThreads / 64];
     const int tid = threadIdx.x;
     if (KEEP && p.counters[kCountState] != 1)
         return; // no step stands
     const int per = (p.requests + kPageThreads - 1) / kPageThreads;
     const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
     const int64_t free_count = (int64_t)p.counters[kCountFree] - (KEEP ? p.counters[kCountTaken] : 0);
-    uint32_t sum = 0;
+    uint64_t sum = 0; // (lengths that are wrong may add up past 2^32)
     bool bad = false;
     // tokens request i holds before the call (with the step's) and after it
     auto tokens = [&](int i, uint32_t *now, uint32_t *after) {
@@ -172,16 +172,17 @@ template <bool KEEP> __global__ __launch_bounds__(kPageThreads) void page_return
         offsets[i] = n;
         sum += n;
     }
-    uint32_t total;
-    uint32_t at = block_offsets(sum, waves, &total);
+    uint64_t all;
+    uint64_t at = block_offsets(sum, waves, &all);
     for (int i = i0; i < i1; ++i) {
         const uint32_t n = offsets[i];
-        offsets[i] = at;
+        offsets[i] = (uint32_t)at;
         at += n;
     }
+    const uint32_t total = (uint32_t)all;
     if (tid == 0)
         offsets[p.requests] = total;
-    bad |= free_count < 0 || free_count + total > p.pages;
+    bad |= free_count < 0 || free_count + (int64_t)all > p.pages;
     if (__syncthreads_or(bad)) {
         if (tid == 0)
             atomicOr(p.err, kErrPages);

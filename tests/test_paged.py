@@ -444,6 +444,20 @@ def test_damaged_tables_are_reported(pcl, torch, ctx):
     assert np.array_equal(batch.state()["lengths"], good["lengths"])
 
 
+@pytest.mark.gpu
+def test_released_pages_past_32_bits_are_refused(pcl, torch, ctx):
+    # lengths that add up to 2^32 pages, of pools of 2^21
+    n = 1 << 21
+    batch = DeviceBatch(pcl, torch, 2048, n, 1, n, 64)
+    ctx.page_reset(batch.desc)
+    batch.a["lengths"].fill_(n)
+    ctx.page_release(batch.desc, batch.put([1] * 2048))
+    assert ctx.sync() == BAD_PAGES
+    assert bool((batch.a["lengths"] == n).all()) and int(batch.a["counters"][0]) == n
+    del batch
+    torch.cuda.empty_cache()
+
+
 def dtype_of(torch, name):
     return torch.float32 if name == "f32" else torch.bfloat16
 
