@@ -537,16 +537,20 @@ int pcl_page_reset(pcl_context *ctx, const pcl_page_batch *batch);
  * fit (negative or too many tokens for the table or step_rows, too few free
  * pages, a length outside the table) is refused as a whole: bit 5 of the error
  * flag, no rows, slots all -1, counters[3] = 0. A page number outside the pools
- * in the table or the free list leaves that row's slot -1, with the error. */
+ * in the table or the free list leaves that row's slot -1 (and -1 as the new
+ * page's entry), with the error, and the step does not stand (counters[3] = 0,
+ * so a commit finds none). */
 int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *new_tokens);
 /* The standing step's tokens count as held: all of them, or the first kept[b]
  * of each request (device, [requests]; speculative tokens that were refused);
  * pages that hold only tokens not kept go back to the free list. Without a
  * standing step nothing happens; a count outside 0..new tokens, like step data
- * out of range, is bit 5 of the error flag and changes nothing. */
+ * out of range or a page outside the pools among those given back, is bit 5 of
+ * the error flag and changes nothing. */
 int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *kept);
 /* Requests with finished[b] != 0 (device, [requests]) give all their pages back
- * and hold no tokens; a standing step is dropped. */
+ * and hold no tokens; a standing step is dropped. With a length out of range or
+ * a page outside the pools among those given back nothing changes (bit 5). */
 int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *finished);
 
 /* K and V rows [n][kvheads][dim] (f32, device, 16-byte aligned) into the slots

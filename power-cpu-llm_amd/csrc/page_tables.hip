@@ -45,22 +45,35 @@ __device__ __forceinline__ uint32_t held_tokens(const PageParams &p, const int32
     return n >= 0 && (uint32_t)n <= p.max_tokens ? (uint32_t)n : ~0u;
 }
 
-// One thread per row of the step; every workgroup forms the sums over all
-// requests by itself (they are a few loads a thread), the first one also
-// writes the words of each request. A decode step is a chain of latencies:
-// the lengths' load, the two scans in one 64-bit sum, the search, the page's
-// load: 3.4 us for 64 requests (an empty launch takes 3.5 us back to back), 5.1 us
-// for 512 requests and 7163 rows, 4.9 us for 96 prompts of 136277 rows.
+// Four words at any word's address.
+typedef int32_t int4w __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ bool in_pools(const PageParams &p, int32_t page)
+{
+    return page >= 0 && page < p.pages;
+}
+
+// The first workgroup writes the words of each request and the counters, the
+// others have one thread per row of the step; every workgroup forms the sums over
+// all requests by itself (they are a few loads a thread). The rows look at their
+// own pages, the first workgroup at every page under a new token: with one outside
+// the pools the step does not stand (a look at 64000 pages beside 1024000 rows:
+// 17.6 us instead of 17.1). A decode step is a chain of latencies: the lengths'
+// load, the two scans in one 64-bit sum, the search, the page's load. Launches of
+// a replayed graph, one behind the other: 3.4 us for 64 requests, 4.9 us for 96
+// prompts of 134989 rows in all.
 __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
 {
     extern __shared__ uint32_t offsets[]; // rows [requests + 1], pages [requests]
     __shared__ uint64_t waves[kPageThreads / 64];
     uint32_t *row_off = offsets, *page_off = offsets + p.requests + 1;
     const int tid = threadIdx.x;
+    const bool books = blockIdx.x == 0;
     const int per = (p.requests + kPageThreads - 1) / kPageThreads;
     const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
     const int free_count = p.counters[kCountFree];
     uint64_t sum = 0; // rows in the low half, pages in the high half
+    uint32_t held_page = 0; // (a negative number is the largest)
     bool bad = false;
     for (int i = i0; i < i1; ++i) {
         const uint32_t len = held_tokens(p, p.lengths, i);
@@ -74,6 +87,10 @@ __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
         row_off[i] = rows;
         page_off[i] = need;
         sum += (uint64_t)need << 32 | rows;
+        // the step goes on in a held page (its number is looked at behind the sums)
+        if (books && rows && len % p.page_tokens)
+            held_page = max(held_page,
+                            (uint32_t)p.table[i * p.table_stride + len / p.page_tokens]);
     }
     uint64_t total;
     uint64_t at = block_offsets(sum, waves, &total);
@@ -86,25 +103,45 @@ __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
     const uint32_t rows = (uint32_t)total, taken = (uint32_t)(total >> 32);
     if (tid == 0)
         row_off[p.requests] = rows;
-    bad |= free_count < 0 || free_count > p.pages || (int64_t)taken > free_count ||
-           rows > (uint32_t)p.step_rows;
+    const bool had = free_count >= 0 && free_count <= p.pages && (int64_t)taken <= free_count;
+    bad |= !had || rows > (uint32_t)p.step_rows;
+    bool damaged = held_page >= (uint32_t)p.pages;
+    // (the first words ahead of the barrier: a decode step takes no more)
+    if (books && had && (uint32_t)tid < taken)
+        damaged |= !in_pools(p, p.free_pages[free_count - 1 - tid]);
     const bool ok = !__syncthreads_or(bad);
 
-    if (blockIdx.x == 0) {
+    if (books) {
         for (int i = tid; i < p.requests; i += kPageThreads) {
             const uint32_t n = ok ? row_off[i + 1] - row_off[i] : 0;
             p.step_lengths[i] = (int32_t)((uint32_t)p.lengths[i] + n);
             p.newest[i] = n ? (int32_t)(row_off[i] + n - 1) : -1;
         }
+        // the other words, four to a load (past the last four those again)
+        constexpr uint32_t kAhead = 4, kRound = 4 * kAhead * kPageThreads;
+        for (uint32_t u0 = 0; ok && u0 + kPageThreads < taken; u0 += kRound) {
+            int4w words[kAhead];
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; ++j)
+                words[j] = *(const int4w *)(p.free_pages + free_count - taken +
+                                            min(u0 + 4 * (j * kPageThreads + tid), taken - 4));
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    damaged |= !in_pools(p, words[j][e]);
+        }
+        damaged = __syncthreads_or(damaged);
         if (tid == 0) {
             p.counters[kCountRows] = ok ? (int32_t)rows : 0;
             p.counters[kCountTaken] = ok ? (int32_t)taken : 0;
-            p.counters[kCountState] = ok;
-            if (!ok)
+            p.counters[kCountState] = ok && !damaged;
+            if (!ok || damaged)
                 atomicOr(p.err, kErrPages);
         }
+        return;
     }
-    const uint32_t t = blockIdx.x * kPageThreads + tid;
+    const uint32_t t = (blockIdx.x - 1) * kPageThreads + tid;
     if (t >= (uint32_t)p.step_rows)
         return;
     int32_t slot = -1, position = -1, request = -1;
@@ -118,15 +155,14 @@ __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
             column < held
                 ? *entry
                 : p.free_pages[free_count - 1 - (int)(page_off[request] + column - held)];
+        const bool in = in_pools(p, page); // else the table or free list is damaged
         position = (int32_t)pos;
-        if (page < 0 || page >= p.pages) {
-            atomicOr(p.err, kErrPages); // the caller's table or free list is damaged
-        } else {
+        // a new page's first token is its first row (a number outside the pools
+        // leaves no earlier request's page in its place)
+        if (column >= held && pos % p.page_tokens == 0)
+            *entry = in ? page : -1;
+        if (in)
             slot = page * (int32_t)p.page_tokens + (int32_t)(pos % p.page_tokens);
-            // a new page's first token is its first row
-            if (column >= held && pos % p.page_tokens == 0)
-                *entry = page;
-        }
     }
     p.slots[t] = slot;
     p.positions[t] = position;
@@ -136,7 +172,8 @@ __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
 // The pages behind the kept ones of every request go back on the free list,
 // in the order of the requests and of their pages: one workgroup. KEEP: the
 // step's commit (`in`: the tokens kept of each request's new ones, null for
-// all); otherwise the release of the requests whose flag is set.
+// all); otherwise the release of the requests whose flag is set. With a page
+// outside the pools among them nothing changes.
 template <bool KEEP> __global__ __launch_bounds__(kPageThreads) void page_return_kernel(PageParams p)
 {
     extern __shared__ uint32_t offsets[]; // returned pages before a request [requests + 1]
@@ -183,17 +220,27 @@ template <bool KEEP> __global__ __launch_bounds__(kPageThreads) void page_return
     if (tid == 0)
         offsets[p.requests] = total;
     bad |= free_count < 0 || free_count + (int64_t)all > p.pages;
-    if (__syncthreads_or(bad)) {
-        if (tid == 0)
+    auto refused = [&]() { // nothing changes
+        const bool any = __syncthreads_or(bad);
+        if (any && tid == 0)
             atomicOr(p.err, kErrPages);
-        return; // nothing changes
-    }
-    for (uint32_t u = tid; u < total; u += kPageThreads) {
-        const int i = find_range(offsets, p.requests, u);
-        uint32_t now, after;
-        tokens(i, &now, &after);
-        p.free_pages[free_count + u] =
-            p.table[i * p.table_stride + pages_of(after, p.page_tokens) + (u - offsets[i])];
+        return any;
+    };
+    if (refused())
+        return;
+    if (total) {
+        auto page_at = [&](uint32_t u) { // returned page u
+            const int i = find_range(offsets, p.requests, u);
+            uint32_t now, after;
+            tokens(i, &now, &after);
+            return p.table[i * p.table_stride + pages_of(after, p.page_tokens) + (u - offsets[i])];
+        };
+        for (uint32_t u = tid; u < total; u += kPageThreads)
+            bad |= !in_pools(p, page_at(u));
+        if (refused())
+            return;
+        for (uint32_t u = tid; u < total; u += kPageThreads)
+            p.free_pages[free_count + u] = page_at(u);
     }
     __syncthreads(); // the lengths are read above
     for (int i = i0; i < i1; ++i) {
@@ -358,7 +405,7 @@ int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *
     if (!new_tokens || (uintptr_t)new_tokens % 4)
         return PCL_INVALID_SHAPE;
     p.in = new_tokens;
-    const int groups = (p.step_rows + pcl::kPageThreads - 1) / pcl::kPageThreads;
+    const int groups = 1 + (p.step_rows + pcl::kPageThreads - 1) / pcl::kPageThreads;
     const size_t lds = (2 * (size_t)p.requests + 1) * sizeof(uint32_t);
     pcl::page_step_kernel<<<groups, pcl::kPageThreads, lds, ctx->stream>>>(p);
     return launched("step");

@@ -445,6 +445,92 @@ def test_damaged_tables_are_reported(pcl, torch, ctx):
 
 
 @pytest.mark.gpu
+def test_a_step_over_damaged_pages_is_not_committed(pcl, torch, ctx):
+    # request 0 held pages 0 and 1, gave them back, and request 1 owns them now:
+    # request 0's table still names them
+    batch = DeviceBatch(pcl, torch, 2, 4, 8, 6, 20)
+    model = PageModel(2, 4, 8, 6, 20)
+    call = device_call(ctx, batch)
+    ctx.page_reset(batch.desc)
+    for name, words in (("step", [9, 0]), ("commit", None), ("release", [1, 0]), ("step", [0, 9]),
+                        ("commit", None)):
+        getattr(model, name)(*([] if words is None else [words]))
+        error, state = call(name, words)
+        assert error == 0
+        model.check(state)
+    assert model.table == [[0, 1, -1, -1], [1, 0, -1, -1]] and model.lengths == [0, 9]
+    good = {n: x.clone() for n, x in batch.a.items()}
+    top = len(model.free) - 1
+
+    def held():
+        return [batch.a[n].cpu().numpy().copy() for n in ("lengths", "counters", "free_pages")]
+
+    # a number outside the pools on the free list: no page of another request
+    # stands in its place, the step does not stand, so that nothing of it is
+    # committed, and the next step does not find the pages held
+    for bad in (6, -1, 99, 1 << 30, -(1 << 31)):
+        batch.a["free_pages"][top] = bad
+        error, state = call("step", [5, 0])
+        assert error == BAD_PAGES and (state["slots"] == -1).all()
+        assert state["counters"][3] == 0
+        assert state["table"].tolist() == [-1, 1, -1, -1, 1, 0, -1, -1]
+        before = held()
+        for kept in (None, [5, 0], [2, 0], [0, 0]):
+            error, _ = call("commit", kept)
+            assert error == 0
+            assert all(np.array_equal(x, y) for x, y in zip(before, held()))
+        batch.a["free_pages"][top] = good["free_pages"][top]
+        error, state = call("step", [5, 1])
+        assert error == 0 and state["slots"][:6].tolist() == [8 * 2 + i for i in range(5)] + [1]
+        for n, x in good.items():
+            batch.a[n].copy_(x)
+    # one in a held entry: the partly filled page that the step goes on in, a page
+    # that a release gives back
+    batch.a["table"][4 + 1] = 6
+    error, _ = call("step", [1, 1])
+    assert error == BAD_PAGES
+    before = held()
+    assert before[1][3] == 0 and call("commit", None)[0] == 0
+    assert all(np.array_equal(x, y) for x, y in zip(before, held()))
+    # (a step that does not touch the page is committed)
+    assert call("step", [1, 0])[0] == 0 and call("commit", None)[0] == 0
+    before = held()
+    assert call("release", [1, 1])[0] == BAD_PAGES
+    assert all(np.array_equal(x, y) for x, y in zip(before, held()))
+    assert call("release", [1, 0])[0] == 0
+    assert batch.a["lengths"].tolist() == [0, 9]
+    # or one behind the step among the pages that a commit gives back
+    for n, x in good.items():
+        batch.a[n].copy_(x)
+    assert call("step", [17, 3])[0] == 0
+    batch.a["table"][2] = 6
+    before = held()
+    assert call("commit", [1, 3])[0] == BAD_PAGES
+    assert all(np.array_equal(x, y) for x, y in zip(before, held()))
+
+
+@pytest.mark.gpu
+def test_damage_anywhere_in_a_long_step_is_found(pcl, torch, ctx):
+    # more pages than the threads look at in one round, one of them outside the
+    # pools
+    batch = DeviceBatch(pcl, torch, 3, 6000, 1, 12000, 11000)
+    ctx.page_reset(batch.desc)
+    good = batch.a["free_pages"].clone()
+    for u in (0, 255, 4095, 4096, 8191, 10500, 10999):
+        batch.a["free_pages"][12000 - 1 - u] = 12000
+        ctx.page_step(batch.desc, batch.put([5000, 1000, 5000]))
+        assert ctx.sync() == BAD_PAGES
+        state = batch.state()
+        assert state["counters"].tolist() == [12000, 11000, 11000, 0]
+        assert np.flatnonzero(state["slots"] == -1).tolist() == [u]
+        assert np.count_nonzero(state["table"] == -1) == 3 * 6000 - 11000 + 1
+        batch.a["free_pages"].copy_(good)
+    batch.a["free_pages"][12000 - 1 - 11000] = 12000  # (the next page is not taken)
+    ctx.page_step(batch.desc, batch.put([5000, 1000, 5000]))
+    assert ctx.sync() == 0 and batch.state()["counters"][3] == 1
+
+
+@pytest.mark.gpu
 def test_released_pages_past_32_bits_are_refused(pcl, torch, ctx):
     # lengths that add up to 2^32 pages, of pools of 2^21
     n = 1 << 21
