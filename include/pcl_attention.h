@@ -549,8 +549,11 @@ int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *
  * the error flag and changes nothing. */
 int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *kept);
 /* Requests with finished[b] != 0 (device, [requests]) give all their pages back
- * and hold no tokens; a standing step is dropped. With a length out of range or
- * a page outside the pools among those given back nothing changes (bit 5). */
+ * and hold no tokens; a standing step is dropped. With a length out of range, or
+ * a page among those given back that lies outside the pools, that another
+ * request's table holds too or that occurs twice, nothing changes (bit 5): the
+ * bookkeeping counts no shares of a page, so a caller whose block tables share
+ * pages gives such requests' pages back itself, in the state's words. */
 int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *finished);
 
 /* K and V rows [n][kvheads][dim] (f32, device, 16-byte aligned) into the slots
@@ -585,7 +588,8 @@ int pcl_paged_append_transformed(pcl_head_transform *transform, const pcl_page_p
  * max_length bounds the lengths (it sizes the workspace); a longer request or a
  * row at or past q_rows is left out with bit 5 of the error flag, and a page
  * outside the pools is read as page 0, with bit 5. Rows must differ from each
- * other. Several requests may share pages. */
+ * other. Several requests may share pages; one that still appends must hold the
+ * page that it appends to alone, and pcl_page_release refuses shared pages. */
 typedef struct pcl_paged_desc {
     pcl_page_pools pools;
     const float *q;

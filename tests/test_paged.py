@@ -510,6 +510,107 @@ def test_a_step_over_damaged_pages_is_not_committed(pcl, torch, ctx):
 
 
 @pytest.mark.gpu
+def test_shared_pages_are_not_released(pcl, torch, ctx):
+    # block tables may share pages; one that another request holds, or that two
+    # requests give back at once, must not come to be free: the release is refused
+    shape = (4, 6, 8, 24, 100)
+    batch = DeviceBatch(pcl, torch, *shape)
+    model = PageModel(*shape)
+    call = device_call(ctx, batch)
+    ctx.page_reset(batch.desc)
+    model.step([20, 30, 9, 5])
+    assert call("step", [20, 30, 9, 5])[0] == 0
+    model.commit()
+    assert call("commit", None)[0] == 0
+    model.step([1, 1, 1, 1])
+    assert call("step", [1, 1, 1, 1])[0] == 0  # it stands
+    good = {n: x.clone() for n, x in batch.a.items()}
+
+    def back():
+        for n, x in good.items():
+            batch.a[n].copy_(x)
+
+    def refused(finished):
+        before = batch.state()
+        error, after = call("release", finished)
+        assert error == BAD_PAGES
+        for n in STATE:
+            assert np.array_equal(before[n], after[n]), n
+
+    # request 1 begins with the pages of request 0
+    batch.a["table"][6:8] = batch.a["table"][:2]
+    for finished in ([1, 0, 0, 0], [0, 1, 0, 0], [1, 1, 0, 0], [1, 1, 1, 1], [0, 1, 0, 7]):
+        refused(finished)
+    # the others are released as ever, and nobody at all
+    assert call("release", [0, 0, 0, 0])[0] == 0
+    error, state = call("release", [0, 0, 1, 1])
+    assert error == 0 and state["lengths"].tolist() == [20, 30, 0, 0]
+    assert state["free_pages"][:int(state["counters"][0])].tolist() == model.free + [7, 8, 9]
+    refused([1, 0, 0, 0])
+    # each with its own pages again
+    batch.a["table"].copy_(good["table"])
+    error, state = call("release", [1, 0, 0, 0])
+    assert error == 0
+    assert state["free_pages"][:int(state["counters"][0])].tolist() == \
+        model.free + [7, 8, 9, 0, 1, 2]
+    # a page twice in one table
+    back()
+    batch.a["table"][1] = batch.a["table"][0]
+    refused([1, 0, 0, 0])
+    # the only page that is shared is the last one of either
+    back()
+    batch.a["table"][6 + 3] = batch.a["table"][2]
+    refused([0, 1, 0, 0])
+    # words behind the list may hold anything, words of it may not
+    for word in (-1, -(1 << 31), (1 << 31) - 1, 5):
+        back()
+        batch.a["free_pages"][len(model.free):] = word
+        error, state = call("release", [0, 0, 1, 0])
+        assert error == 0
+        assert state["free_pages"][:int(state["counters"][0])].tolist() == model.free + [7, 8]
+        if word < 0:
+            back()
+            batch.a["free_pages"][3] = word
+            refused([0, 0, 1, 0])
+
+
+@pytest.mark.gpu
+def test_one_shared_page_among_many_is_found(pcl, torch, ctx):
+    # more words, returned and kept pages than the workgroup's threads take at once
+    shape = (40, 700, 1, 20000, 16000)
+    batch = DeviceBatch(pcl, torch, *shape)
+    model = PageModel(*shape)
+    call = device_call(ctx, batch)
+    ctx.page_reset(batch.desc)
+    counts = [100 + 15 * (b % 41) for b in range(40)]
+    assert model.step(counts) and call("step", counts)[0] == 0
+    assert model.commit() and call("commit", None)[0] == 0
+    finished = [b % 2 for b in range(40)]
+    good = batch.a["table"].clone()
+    for b, column in ((0, 0), (38, counts[38] - 1), (20, 133)):
+        for c, other in ((1, 0), (39, counts[39] - 1), (21, 250)):
+            batch.a["table"][700 * b + column] = batch.a["table"][700 * c + other]
+            error, state = call("release", finished)
+            assert error == BAD_PAGES
+            assert state["lengths"].tolist() == counts
+            assert state["free_pages"][:len(model.free)].tolist() == model.free
+            batch.a["table"].copy_(good)
+    model.release(finished)
+    error, state = call("release", finished)
+    assert error == 0
+    model.void()  # (what the step wrote stands)
+    for name in ("lengths", "free_pages", "counters"):
+        want = {"lengths": model.lengths, "free_pages": model.free,
+                "counters": [len(model.free)]}[name]
+        assert state[name][:len(want)].tolist() == want
+    rest = [1 - f for f in finished]
+    model.release(rest)
+    error, state = call("release", rest)
+    assert error == 0 and len(model.free) == 20000
+    assert state["free_pages"].tolist() == model.free
+
+
+@pytest.mark.gpu
 def test_damage_anywhere_in_a_long_step_is_found(pcl, torch, ctx):
     # more pages than the threads look at in one round, one of them outside the
     # pools
