@@ -1021,6 +1021,81 @@ def test_softcap(pcl, torch, ctx, softcap):
     assert ctx.sync() == 0
 
 
+def exact_and_bound(cache, q, b, window=0, softcap=0.0):
+    """The attention of request b in 64 bits, and a bound of the kernels' error for
+    each value, from the request's own numbers. With u = 2^-24, half an f32 step:
+
+    a score is a chain of dim fmas from zero, off by at most 1.01 dim u sum|q_d k_d|
+    (1.01 for the higher powers of u; the scaled query is the kernels' own); a cap
+    passes that on at most as it is and adds 20 u of its value (exp off by 13 u at
+    worst where 1 - exp(-2 |t|) cancels, and the roundings of t, the sums, the
+    reciprocal and the product).
+    exp(x) is exp2 of x log2(e), x a difference: 3 |x| u of the argument and 2 u of
+    the instruction. A term is multiplied by the exp of its own tile and by the
+    factors of the tiles, chunks and spans behind it, whose arguments are the steps
+    of one running maximum: together at most R = max s - s_t, with 2 u each.
+    A term passes through at most 256 fmas and 8 factors of its chunk and one fma
+    per chunk of its span and per span, two more where a part enters a merge.
+    The numerator's terms are thus off by e (relative), the denominator's by no
+    more, and their quotient by 2.02 e of the sum of |w v|, and 4 u of itself."""
+    torch = cache.torch
+    qheads, kvheads, dim = cache.heads
+    n = cache.lengths[b]
+    lo = max(0, n - window) if window else 0
+    k, v = cache.k[b][lo:].double(), cache.v[b][lo:].double()
+    x = (q[:qheads * dim] * np.float32(scale_of(dim))).double().view(kvheads, -1, dim)
+    kt = k.permute(1, 2, 0).contiguous()
+    s, size = torch.matmul(x, kt), torch.matmul(x.abs(), kt.abs())
+    capped = softcap * torch.tanh(s / softcap) if softcap else s
+    w = torch.softmax(capped, -1)
+    vt = v.permute(1, 0, 2).contiguous()
+    exact = torch.matmul(w, vt)
+    spans = n // (16 * 256) + 1
+    e = 1.01 * dim * size.amax(-1, keepdim=True) + \
+        (20 * capped.abs().amax(-1, keepdim=True) if softcap else 0) + \
+        3 * (capped.amax(-1, keepdim=True) - capped.amin(-1, keepdim=True)) + \
+        2 * (1 + 8 + 17 + spans + 1) + 256 + 8 + 16 + spans + 2
+    u = 2.0 ** -24
+    bound = 2.02 * e * u * torch.matmul(w, vt.abs()) + 4 * u * exact.abs()
+    return exact.reshape(-1), bound.reshape(-1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(16, 8, 256), (16, 2, 512), (32, 8, 128), (4, 4, 64)],
+                         ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 6000])
+def test_long_requests_in_64_bits(pcl, torch, ctx, heads, dtype, window):
+    # a bound well below the outputs, which shrink with the number of keys
+    lengths = [20000, 3, 70001, 257]
+    cache = Cache(pcl, torch, heads, lengths, 64, dtype, 13)
+    q = torch.randn((4, heads[0] * heads[2]), device="cuda:0")
+    out = cache.attend(ctx, q, window=window)
+    assert ctx.sync() == 0
+    for b, n in enumerate(lengths):
+        exact, bound = exact_and_bound(cache, q[b], b, window)
+        assert float(bound.max()) < 0.5 * float(exact.abs().mean()), n
+        assert bool(((out[b].double() - exact).abs() <= bound).all()), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("softcap", [0.75, 3.0, 50.0])
+def test_softcap_in_64_bits(pcl, torch, ctx, dtype, softcap):
+    # scores far past the cap, around it and far below it
+    for heads in ((16, 8, 256), (32, 8, 128), (10, 2, 80)):
+        cache = Cache(pcl, torch, heads, [1, 300, 700, 5000], 16, dtype, 3)
+        q = 6 * torch.randn((4, heads[0] * heads[2]), device="cuda:0")
+        out = cache.attend(ctx, q, softcap=softcap)
+        assert ctx.sync() == 0
+        for b in range(4):
+            exact, bound = exact_and_bound(cache, q[b], b, softcap=softcap)
+            # and the cap shows
+            other = exact_and_bound(cache, q[b], b)[0] if b else -exact
+            assert float(bound.max()) < 0.5 * float((exact - other).abs().mean())
+            assert bool(((out[b].double() - exact).abs() <= bound).all()), (heads, b)
+
+
 @pytest.mark.gpu
 def test_rows_strides_and_requests_left_out(pcl, torch, ctx):
     # requests without a row or keys, rows in another order, padded strides:
