@@ -57,11 +57,11 @@ __device__ __forceinline__ bool in_pools(const PageParams &p, int32_t page)
 // others have one thread per row of the step; every workgroup forms the sums over
 // all requests by itself (they are a few loads a thread). The rows look at their
 // own pages, the first workgroup at every page under a new token: with one outside
-// the pools the step does not stand (a look at 64000 pages beside 1024000 rows:
-// 17.6 us instead of 17.1). A decode step is a chain of latencies: the lengths'
-// load, the two scans in one 64-bit sum, the search, the page's load. Launches of
-// a replayed graph, one behind the other: 3.4 us for 64 requests, 4.9 us for 96
-// prompts of 134989 rows in all.
+// the pools the step does not stand (the look at 64000 pages beside 1024000 rows
+// costs 0.5 us of 17). A decode step is a chain of latencies: the lengths' load,
+// the two scans in one 64-bit sum, the search, the page's load. Profiled durations:
+// 3.9 us for 64 requests, 5.5 us for 512 requests and 7163 rows, 5.0 us for 96
+// prompts of 136277 rows; a call takes 7.7 us, the host's time.
 __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
 {
     extern __shared__ uint32_t offsets[]; // rows [requests + 1], pages [requests]
@@ -226,9 +226,9 @@ __device__ __forceinline__ bool pages_can_return(const PageParams &p, int free_c
 // in the order of the requests and of their pages: one workgroup. KEEP: the
 // step's commit (`in`: the tokens kept of each request's new ones, null for
 // all); otherwise the release of the requests whose flag is set. Where a page
-// cannot go back nothing changes. In a replayed graph: 3.1 us for the commit of 64
-// requests; a release of nobody 4.0 us, of one of 96 prompts (90 pages of 8485)
-// 18 us, of all of them 31 us, of 256 requests of 250 pages 0.19 ms: three looks
+// cannot go back nothing changes. Profiled durations: 3.7 us for the commit of 64
+// requests; a release of nobody 4.2 us, of one of 96 prompts (90 pages of 8484)
+// 19 us, of all of them 30 us, of 256 requests of 250 pages 0.19 ms: three looks
 // at every page that goes back, one at every page that stays, some 1024 at a time.
 template <bool KEEP> constexpr int kReturnThreads = KEEP ? kPageThreads : 1024;
 

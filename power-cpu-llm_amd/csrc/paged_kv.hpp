@@ -111,7 +111,8 @@ template <int N, int I = 0, typename F> __device__ __forceinline__ void each(F &
 // b, the four rows' a are those of lanes 4 BLOCK .. 4 BLOCK + 3. The f32 MFMAs
 // are chains of fmas over their k slots (checked bit for bit on MI355X), so 4 of
 // these in the order of the slots equal one v_mfma_f32_16x16x4f32 of the
-// canonical chains, at an eighth of its matrix time for four rows.
+// canonical chains, at a quarter of its matrix time: the same rate, and no rows
+// of the sixteen left unused by four.
 template <int BLOCK> __device__ __forceinline__ f4 mfma_rows4(float a, float b, f4 acc)
 {
     return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, acc, 4, BLOCK, 0);
