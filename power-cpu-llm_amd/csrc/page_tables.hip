@@ -229,7 +229,8 @@ __device__ __forceinline__ bool pages_can_return(const PageParams &p, int free_c
 // cannot go back nothing changes. Profiled durations: 3.7 us for the commit of 64
 // requests; a release of nobody 4.2 us, of one of 96 prompts (90 pages of 8484)
 // 19 us, of all of them 30 us, of 256 requests of 250 pages 0.19 ms: three looks
-// at every page that goes back, one at every page that stays, some 1024 at a time.
+// at every page that goes back, one at every page that stays and one at every word
+// of the list, 1024 at a time.
 template <bool KEEP> constexpr int kReturnThreads = KEEP ? kPageThreads : 1024;
 
 template <bool KEEP>
@@ -291,7 +292,8 @@ __global__ __launch_bounds__(kReturnThreads<KEEP>) void page_return_kernel(PageP
     if (!KEEP && all)
         add_up(stay_off, stay_sum, &stay_all);
     const uint32_t total = (uint32_t)all;
-    bad |= free_count < 0 || free_count + (int64_t)all > p.pages || stay_all > UINT32_MAX;
+    // (more than 2^31 pages stay only where tables share them)
+    bad |= free_count < 0 || free_count + (int64_t)all > p.pages || stay_all > INT32_MAX;
     auto refused = [&]() {
         const bool any = __syncthreads_or(bad);
         if (any && tid == 0)

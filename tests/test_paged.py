@@ -641,6 +641,11 @@ def test_released_pages_past_32_bits_are_refused(pcl, torch, ctx):
     ctx.page_release(batch.desc, batch.put([1] * 2048))
     assert ctx.sync() == BAD_PAGES
     assert bool((batch.a["lengths"] == n).all()) and int(batch.a["counters"][0]) == n
+    # or that many stay
+    batch.a["counters"][0] = 0
+    ctx.page_release(batch.desc, batch.put([1] + [0] * 2047))
+    assert ctx.sync() == BAD_PAGES
+    assert bool((batch.a["lengths"] == n).all()) and int(batch.a["counters"][0]) == 0
     del batch
     torch.cuda.empty_cache()
 
