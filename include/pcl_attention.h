@@ -23,7 +23,8 @@
  *   5. the head transform that prepares Q, K and V rows for 3 and 4;
  *   6. the attention output block (projection, post-norm, residual);
  *   7. batches of requests over a paged cache: page bookkeeping, appends and
- *      single-token attention.
+ *      single-token attention;
+ *   8. drafted tokens, parts of prompts and shared pages over a paged cache.
  */
 #ifndef PCL_ATTENTION_H
 #define PCL_ATTENTION_H
@@ -518,7 +519,8 @@ typedef struct pcl_page_batch {
     int32_t *table;       /* [requests][table_stride] pages of each request */
     int32_t *free_pages;  /* [pages] a stack: the last free entry is taken first */
     int32_t *counters;    /* [4] free pages; of the step: its rows, the pages it
-                             takes, 1 while it stands uncommitted */
+                             takes, 1 while it stands uncommitted (2: a fork,
+                             section 8) */
     /* what a step writes: */
     int32_t *step_lengths; /* [requests] tokens held with the step's */
     int32_t *newest;       /* [requests] row of the newest token, -1 for none */
@@ -551,9 +553,8 @@ int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t
 /* Requests with finished[b] != 0 (device, [requests]) give all their pages back
  * and hold no tokens; a standing step is dropped. With a length out of range, or
  * a page among those given back that lies outside the pools, that another
- * request's table holds too or that occurs twice, nothing changes (bit 5): the
- * bookkeeping counts no shares of a page, so a caller whose block tables share
- * pages gives such requests' pages back itself, in the state's words. */
+ * request's table holds too or that occurs twice, nothing changes (bit 5): where
+ * block tables share pages, pcl_page_release_shared gives them back. */
 int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *finished);
 
 /* K and V rows [n][kvheads][dim] (f32, device, 16-byte aligned) into the slots
@@ -589,7 +590,8 @@ int pcl_paged_append_transformed(pcl_head_transform *transform, const pcl_page_p
  * row at or past q_rows is left out with bit 5 of the error flag, and a page
  * outside the pools is read as page 0, with bit 5. Rows must differ from each
  * other. Several requests may share pages; one that still appends must hold the
- * page that it appends to alone, and pcl_page_release refuses shared pages. */
+ * page that it appends to alone, and pcl_page_release refuses shared pages
+ * (pcl_page_release_shared gives them back). */
 typedef struct pcl_paged_desc {
     pcl_page_pools pools;
     const float *q;
@@ -616,6 +618,162 @@ typedef struct pcl_paged_desc {
 int pcl_paged_attention(pcl_context *ctx, const pcl_paged_desc *desc);
 /* Workspace bytes a descriptor needs (0 when it is refused). */
 size_t pcl_paged_workspace_bytes(const pcl_paged_desc *desc);
+
+/* ---- 8. drafted tokens and shared pages ---------------------------------------
+ *
+ * A round of drafted tokens is a step of section 7 in which a request's new tokens
+ * form a tree: each follows another of them, or the held tokens, and attends the
+ * held tokens and its own branch.
+ *
+ *   pcl_page_step                          the drafted tokens' rows
+ *   pcl_page_tree_masks                    their positions and branches
+ *   per layer:
+ *     pcl_paged_append[_transformed]       at the tree's positions
+ *     pcl_paged_tree_attention             every new token
+ *   pcl_page_accept                        the branch that was verified: which rows
+ *                                          move to follow the held tokens
+ *   pcl_page_commit                        with the branches' lengths as kept
+ *   pcl_paged_copy                         the rows, in every layer at once
+ *
+ * Without a tree the new tokens are a chain, each behind the one before it: drafted
+ * tokens of one continuation, or a prompt's part behind what the pages hold, with
+ * no masks and nothing to move.
+ *
+ * Requests that begin as copies of others (several answers to a prompt, beams)
+ * share their whole pages:
+ *
+ *   pcl_page_fork                          their tables; a page of its own for a
+ *                                          fork's last, partly filled one
+ *   pcl_page_commit                        the forks hold their sources' tokens
+ *   pcl_paged_copy                         those last pages' rows, in every layer
+ *   pcl_page_release_shared                of requests that ended, the pages that
+ *                                          nobody else holds
+ *
+ * State, streams, captures, workspaces and the error flag are those of section 7. */
+
+/* The trees of a standing step, device memory: rows as the step lays them out. */
+typedef struct pcl_page_tree {
+    const int32_t *parents; /* [step_rows] index among its request's new tokens of
+                               the token that each follows, below its own; -1: the
+                               held tokens */
+    int64_t words;          /* 64-bit words of a mask, 1 to 8: trees of up to 64 *
+                               words tokens */
+    /* what the call writes: */
+    int32_t *positions; /* [step_rows] tokens held + tokens before it on its branch,
+                           -1 behind the last row */
+    uint64_t *masks;    /* [step_rows][words] bit j: new token j of its request is
+                           on its branch (itself too); 0 behind the last row */
+} pcl_page_tree;
+
+/* Positions and branches of the standing step's new tokens (without one: of none).
+ * A parent that is not below its token counts as -1, and of a request with more
+ * than 64 * words new tokens each sees the held tokens alone, in the chain's
+ * positions, both with bit 5 of the error flag. */
+int pcl_page_tree_masks(pcl_context *ctx, const pcl_page_batch *batch, const pcl_page_tree *tree);
+
+/* Rows that verified branches move: paths (device, [requests][depth]) holds of each
+ * request the counts[b] (device, [requests]; at most depth) new tokens that are
+ * kept, their indexes ascending. from and to ([requests][depth]) receive the slots
+ * of the k-th one's row and of the row that it moves to, the k-th behind the held
+ * tokens, -1 where nothing moves. Call it before the commit (with kept = counts),
+ * and pcl_paged_copy with lists = requests, entries = depth and no row counts before
+ * the next step. Indexes that do not ascend within the new tokens, or counts out of
+ * range, are bit 5 of the error flag: that request's lists are -1, the others' may
+ * be, and the step does not stand any more, so that a commit finds none. Without a
+ * standing step all lists are -1. depth * requests below 2^31. */
+int pcl_page_accept(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *paths,
+                    const int32_t *counts, int64_t depth, int32_t *from, int32_t *to);
+
+/* Opens a fork: a step without rows in which every request b with sources[b] >= 0
+ * (device, [requests]) begins as a copy of request sources[b]. It must hold no
+ * tokens, and its source must not be a fork of the same call. Its table gets the
+ * source's whole pages, and a page from the free list (in request order) where the
+ * source's last one is partly filled; from, to and rows (device, [requests]) receive
+ * that page's first slot, the new one's, and the rows to copy (pcl_paged_copy with
+ * lists = requests, entries = 1; -1, -1 and 0 where there are none). As a step's, its
+ * held state changes with pcl_page_commit, whose `kept` must be NULL for a fork (or
+ * it is refused with bit 5), and one that is not committed is replaced by the next
+ * fork or step. A fork that does not fit (a request that holds tokens, a source that
+ * is none, too few free pages, a length outside the table) is refused as a whole,
+ * with bit 5; one whose last pages lie outside the pools does not stand, with bit 5.
+ * Forks may be forked once they are committed. */
+int pcl_page_fork(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *sources,
+                  int32_t *from, int32_t *to, int32_t *rows);
+
+/* pcl_page_release where block tables share pages: requests with finished[b] != 0
+ * hold no tokens any more, and those of their pages that no other request holds go
+ * back, each once, the highest number first (so that the lowest is taken next). A
+ * standing step or fork is dropped. With a length out of range, a page among the
+ * finished requests' that lies outside the pools, or one of them on the free list
+ * already, nothing changes (bit 5). Uses the context's workspace (inside a capture
+ * it is not grown: pcl_context_reserve the bytes before). */
+int pcl_page_release_shared(pcl_context *ctx, const pcl_page_batch *batch,
+                            const int32_t *finished);
+/* Workspace bytes of that call (0 for a batch that is refused). */
+size_t pcl_page_release_workspace_bytes(const pcl_page_batch *batch);
+
+/* Copies rows of pages, K and V, from slot to slot in the pools of `layers` layers
+ * (a host array; the same pages and page_tokens in all, heads and types may differ).
+ * from and to (device, [lists][entries]) name slots; an entry with a negative one is
+ * left out, one past the pools too, with bit 5 of the error flag. rows NULL: one row
+ * an entry, the entries of a list in order; none reads a row that an earlier one of
+ * its list writes (it may write one that an earlier one reads). rows (device,
+ * [lists], only with entries = 1): an entry copies that many consecutive slots (none
+ * for 0 or less), and the two ranges do not overlap. Lists do not touch the rows
+ * that another one writes. */
+int pcl_paged_copy(pcl_context *ctx, const pcl_page_pools *pools, int64_t layers,
+                   const int32_t *from, const int32_t *to, const int32_t *rows, int64_t lists,
+                   int64_t entries);
+
+/* Attention of every new token of a step over its request's pages. Request b, with
+ * n = step_lengths[b] - lengths[b] new tokens, has them in rows newest[b] - n + 1 to
+ * newest[b] (a step's arrays as they are); their query heads are at q + row *
+ * q_stride, their outputs go to out + row * o_stride. New token i is at position
+ * lengths[b] + i and attends keys [0, lengths[b] + i]; with masks it is at
+ * positions[row] and attends the held keys [0, lengths[b]) and each new token j with
+ * bit j of masks[row] (any bits; pcl_page_tree_masks makes a tree's). With a window a
+ * token attends only keys whose position is less than `window` before its own (the
+ * new tokens' by positions; at least lengths[b] each). Requests without new tokens
+ * or with a negative newest are left out, and a token that attends no key too: their
+ * output rows stay as they were. Queries are scaled and scores capped as in
+ * pcl_attention_desc. A token's output has the bits that pcl_attention_launch gives
+ * for the request's keys and values in one segment (the chain: causal, first_key 0,
+ * first_query lengths[b]; masks: with the same mask as bytes), whatever else is in
+ * the batch; only a zero's sign may differ. Keys that no token attends may hold
+ * anything. A key that one token attends and another one does not may make the
+ * latter a NaN where its value is not finite; the former sets the error flag then.
+ * max_length bounds step_lengths, max_new the new tokens of a request (they size the
+ * workspace with q_rows). A request past them or whose rows do not lie in q_rows,
+ * or with more new tokens than its masks have bits, is left out with bit 5 of the
+ * error flag; a page outside the pools is read as page 0, with bit 5. Rows of
+ * different requests must differ. */
+typedef struct pcl_paged_tree_desc {
+    pcl_page_pools pools;
+    const float *q;
+    int64_t q_stride, q_rows; /* q_rows: rows that q, out, masks and positions hold */
+    int64_t qheads;           /* at most 4096 */
+    const int32_t *table;     /* [requests][table_stride] */
+    int64_t table_stride;
+    const int32_t *lengths;      /* [requests] tokens held */
+    const int32_t *step_lengths; /* [requests] with the new ones */
+    const int32_t *newest;       /* [requests] row of the newest token, -1 for none */
+    const uint64_t *masks;       /* [q_rows][mask_words] or NULL */
+    int64_t mask_words;          /* 1 to 8; 0 without masks */
+    const int32_t *positions;    /* [q_rows] with masks (may be NULL without a window) */
+    int64_t requests;            /* at most 2048 */
+    int64_t max_length;          /* at most table_stride * page_tokens */
+    int64_t max_new;             /* below 2^20 */
+    int64_t window;              /* 0 = all keys */
+    float q_scale;
+    float softcap; /* 0 = off */
+    float *out;
+    int64_t o_stride;
+} pcl_paged_tree_desc;
+
+/* Launch asynchronously; results and errors as pcl_paged_attention. */
+int pcl_paged_tree_attention(pcl_context *ctx, const pcl_paged_tree_desc *desc);
+/* Workspace bytes a descriptor needs (0 when it is refused). */
+size_t pcl_paged_tree_workspace_bytes(const pcl_paged_tree_desc *desc);
 
 /* Library identification (for loaders). */
 const char *pcl_version(void);

@@ -23,6 +23,10 @@ error behaviour:
       batches of requests over a paged cache: Context.page_reset / page_step /
       page_commit / page_release, Context.paged_append,
       HeadTransform.append_paged and Context.paged_attention.
+  PclPageTree, PclPagedTreeDesc
+      drafted tokens, parts of prompts and shared pages over a paged cache:
+      Context.page_tree / page_accept / page_fork / page_release_shared,
+      Context.paged_copy and Context.paged_tree_attention.
 
 There is no CPU fallback: without the built library every entry raises.
 """
@@ -102,6 +106,14 @@ EXPORTS = (
     "pcl_paged_append_transformed",
     "pcl_paged_attention",
     "pcl_paged_workspace_bytes",
+    "pcl_page_tree_masks",
+    "pcl_page_accept",
+    "pcl_page_fork",
+    "pcl_page_release_shared",
+    "pcl_page_release_workspace_bytes",
+    "pcl_paged_copy",
+    "pcl_paged_tree_attention",
+    "pcl_paged_tree_workspace_bytes",
     "pcl_version",
 )
 
@@ -164,6 +176,32 @@ class PclPagedDesc(ctypes.Structure):
         ("max_length", ctypes.c_int64), ("window", ctypes.c_int64), ("q_scale", ctypes.c_float),
         ("softcap", ctypes.c_float), ("out", ctypes.c_void_p), ("o_stride", ctypes.c_int64),
     ]
+
+
+class PclPageTree(ctypes.Structure):
+    """pcl_page_tree: the trees of a standing step."""
+    _fields_ = [("parents", ctypes.c_void_p), ("words", ctypes.c_int64),
+                ("positions", ctypes.c_void_p), ("masks", ctypes.c_void_p)]
+
+
+class PclPagedTreeDesc(ctypes.Structure):
+    """pcl_paged_tree_desc: one layer's attention of every new token of a step."""
+    _fields_ = [
+        ("pools", PclPagePools),
+        ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("q_rows", ctypes.c_int64),
+        ("qheads", ctypes.c_int64), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p), ("step_lengths", ctypes.c_void_p),
+        ("newest", ctypes.c_void_p), ("masks", ctypes.c_void_p), ("mask_words", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("requests", ctypes.c_int64),
+        ("max_length", ctypes.c_int64), ("max_new", ctypes.c_int64), ("window", ctypes.c_int64),
+        ("q_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("out", ctypes.c_void_p),
+        ("o_stride", ctypes.c_int64),
+    ]
+
+
+def page_tree(**kw):
+    """A PclPageTree with the given fields."""
+    return PclPageTree(**kw)
 
 
 def page_pools(**kw):
@@ -285,7 +323,15 @@ def load():
             ("pcl_paged_append_transformed", ctypes.c_int,
              [vp, pools, vp, vp, i64, vp, vp, vp, i64, vp]),
             ("pcl_paged_attention", ctypes.c_int, [vp, ctypes.POINTER(PclPagedDesc)]),
-            ("pcl_paged_workspace_bytes", sz, [ctypes.POINTER(PclPagedDesc)])):
+            ("pcl_paged_workspace_bytes", sz, [ctypes.POINTER(PclPagedDesc)]),
+            ("pcl_page_tree_masks", ctypes.c_int, [vp, batch, ctypes.POINTER(PclPageTree)]),
+            ("pcl_page_accept", ctypes.c_int, [vp, batch, vp, vp, i64, vp, vp]),
+            ("pcl_page_fork", ctypes.c_int, [vp, batch, vp, vp, vp, vp]),
+            ("pcl_page_release_shared", ctypes.c_int, [vp, batch, vp]),
+            ("pcl_page_release_workspace_bytes", sz, [batch]),
+            ("pcl_paged_copy", ctypes.c_int, [vp, pools, i64, vp, vp, vp, i64, i64]),
+            ("pcl_paged_tree_attention", ctypes.c_int, [vp, ctypes.POINTER(PclPagedTreeDesc)]),
+            ("pcl_paged_tree_workspace_bytes", sz, [ctypes.POINTER(PclPagedTreeDesc)])):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
@@ -565,6 +611,57 @@ class Context:
 
     def paged_workspace_bytes(self, desc):
         return self.lib.pcl_paged_workspace_bytes(ctypes.byref(desc))
+
+    def page_tree(self, batch, tree):
+        """Positions and branches of the standing step's trees (a PclPageTree)."""
+        self._check(self.lib.pcl_page_tree_masks(self.handle, ctypes.byref(batch),
+                                                 ctypes.byref(tree)))
+
+    def page_accept(self, batch, paths_ptr, counts_ptr, depth, from_ptr, to_ptr):
+        """Which rows the verified branches move (slots, [requests][depth])."""
+        self._check(self.lib.pcl_page_accept(
+            self.handle, ctypes.byref(batch), ctypes.c_void_p(paths_ptr),
+            ctypes.c_void_p(counts_ptr), int(depth), ctypes.c_void_p(from_ptr),
+            ctypes.c_void_p(to_ptr)))
+
+    def page_fork(self, batch, sources_ptr, from_ptr, to_ptr, rows_ptr):
+        """Opens a fork: request b begins as a copy of sources[b] (negative: not);
+        the rows to copy go to from / to / rows ([requests])."""
+        self._check(self.lib.pcl_page_fork(
+            self.handle, ctypes.byref(batch), ctypes.c_void_p(sources_ptr),
+            ctypes.c_void_p(from_ptr), ctypes.c_void_p(to_ptr), ctypes.c_void_p(rows_ptr)))
+
+    def page_release_shared(self, batch, finished_ptr):
+        """Requests with a nonzero flag give back the pages that nobody else
+        holds."""
+        self._check(self.lib.pcl_page_release_shared(self.handle, ctypes.byref(batch),
+                                                     ctypes.c_void_p(finished_ptr)))
+
+    def page_release_workspace_bytes(self, batch):
+        return self.lib.pcl_page_release_workspace_bytes(ctypes.byref(batch))
+
+    def paged_copy(self, pools, from_ptr, to_ptr, lists, entries=1, rows_ptr=None):
+        """Rows from slot to slot in the pages of several layers (a sequence of
+        PclPagePools): lists of entries in order, or, with rows, runs."""
+        array = (PclPagePools * len(pools))(*pools)
+        self._check(self.lib.pcl_paged_copy(
+            self.handle, array, len(pools), ctypes.c_void_p(from_ptr), ctypes.c_void_p(to_ptr),
+            ctypes.c_void_p(rows_ptr), int(lists), int(entries)))
+
+    @staticmethod
+    def paged_tree_desc(**kw):
+        d = PclPagedTreeDesc()
+        d.q_scale = 1.0
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def paged_tree_attention(self, desc):
+        """Every new token of a step over its request's pages."""
+        self._check(self.lib.pcl_paged_tree_attention(self.handle, ctypes.byref(desc)))
+
+    def paged_tree_workspace_bytes(self, desc):
+        return self.lib.pcl_paged_tree_workspace_bytes(ctypes.byref(desc))
 
     def sync(self):
         """Wait; returns the device error flag (cleared)."""

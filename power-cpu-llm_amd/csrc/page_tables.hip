@@ -16,6 +16,7 @@
 // lie behind the held ones, the free list stands until the commit), so its
 // workgroups need no order among them and a repeated step repeats its result.
 #include "context.hpp"
+#include "page_batch.hpp"
 #include "paged.hpp"
 
 #include <algorithm>
@@ -23,35 +24,8 @@
 
 namespace pcl {
 
-constexpr int kPageThreads = 256;
-
-enum { kCountFree, kCountRows, kCountTaken, kCountState, kCounters };
-
-struct PageParams {
-    int32_t *lengths, *table, *free_pages, *counters, *step_lengths, *newest;
-    int32_t *slots, *positions, *row_request;
-    const int32_t *in; // new tokens, kept tokens or finished flags per request
-    int64_t table_stride;
-    int requests, pages, step_rows;
-    uint32_t page_tokens, max_tokens; // tokens a request may hold
-    int *err;
-};
-
-// Tokens request i holds, or ~0 when its length is outside the table.
-__device__ __forceinline__ uint32_t held_tokens(const PageParams &p, const int32_t *lengths,
-                                                int i)
-{
-    const int32_t n = lengths[i];
-    return n >= 0 && (uint32_t)n <= p.max_tokens ? (uint32_t)n : ~0u;
-}
-
 // Four words at any word's address.
 typedef int32_t int4w __attribute__((ext_vector_type(4), aligned(4)));
-
-__device__ __forceinline__ bool in_pools(const PageParams &p, int32_t page)
-{
-    return page >= 0 && page < p.pages;
-}
 
 // The first workgroup writes the words of each request and the counters, the
 // others have one thread per row of the step; every workgroup forms the sums over
@@ -135,7 +109,7 @@ __global__ __launch_bounds__(kPageThreads) void page_step_kernel(PageParams p)
         if (tid == 0) {
             p.counters[kCountRows] = ok ? (int32_t)rows : 0;
             p.counters[kCountTaken] = ok ? (int32_t)taken : 0;
-            p.counters[kCountState] = ok && !damaged;
+            p.counters[kCountState] = ok && !damaged ? kStepStands : kStepNone;
             if (!ok || damaged)
                 atomicOr(p.err, kErrPages);
         }
@@ -243,13 +217,15 @@ __global__ __launch_bounds__(kReturnThreads<KEEP>) void page_return_kernel(PageP
     __shared__ uint64_t waves[kThreads / 64];
     uint32_t *stay_off = offsets + p.requests + 1;
     const int tid = threadIdx.x;
-    if (KEEP && p.counters[kCountState] != 1)
+    const int state = KEEP ? p.counters[kCountState] : kStepNone;
+    if (KEEP && state != kStepStands && state != kForkStands)
         return; // no step stands
     const int per = (p.requests + kThreads - 1) / kThreads;
     const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
     const int64_t free_count = (int64_t)p.counters[kCountFree] - (KEEP ? p.counters[kCountTaken] : 0);
     uint64_t sum = 0, stay_sum = 0; // (lengths that are wrong may add up past 2^32)
-    bool bad = false;
+    // (a fork's pages are its source's too: none goes back)
+    bool bad = KEEP && state == kForkStands && p.in;
     // tokens request i holds before the call (with the step's) and after it
     auto tokens = [&](int i, uint32_t *now, uint32_t *after) {
         const uint32_t len = held_tokens(p, p.lengths, i);
@@ -333,7 +309,7 @@ __global__ __launch_bounds__(kReturnThreads<KEEP>) void page_return_kernel(PageP
     }
     if (tid == 0) {
         p.counters[kCountFree] = (int32_t)(free_count + total);
-        p.counters[kCountState] = 0;
+        p.counters[kCountState] = kStepNone;
     }
 }
 
@@ -412,13 +388,7 @@ bool valid_pools(const pcl_page_pools &s)
            ((uintptr_t)s.k | (uintptr_t)s.v) % 16 == 0;
 }
 
-} // namespace pcl
-
-namespace {
-
-using pcl::PageParams;
-
-int launched(const char *what)
+int page_launched(const char *what)
 {
     const hipError_t e = hipGetLastError();
     if (e == hipSuccess)
@@ -427,19 +397,25 @@ int launched(const char *what)
     return PCL_NON_FINITE_VALUE;
 }
 
-int page_params(pcl_context *ctx, const pcl_page_batch *b, PageParams *p)
+int check_batch(const pcl_page_batch &b)
 {
-    if (!ctx || !b || b->requests <= 0 || b->requests > pcl::kMaxRequests || b->table_stride <= 0 ||
-        b->table_stride > pcl::kMaxSlots || b->page_tokens <= 0 ||
-        b->page_tokens > pcl::kMaxPageTokens || b->pages <= 0 ||
-        b->pages > pcl::kMaxSlots / b->page_tokens || b->step_rows <= 0 ||
-        b->step_rows > pcl::kMaxStepRows)
+    if (b.requests <= 0 || b.requests > kMaxRequests || b.table_stride <= 0 ||
+        b.table_stride > kMaxSlots || b.page_tokens <= 0 || b.page_tokens > kMaxPageTokens ||
+        b.pages <= 0 || b.pages > kMaxSlots / b.page_tokens || b.step_rows <= 0 ||
+        b.step_rows > kMaxStepRows)
         return PCL_INVALID_SHAPE;
-    const void *words[] = {b->lengths,      b->table,  b->free_pages, b->counters,   b->step_lengths,
-                           b->newest,       b->slots,  b->positions,  b->row_request};
+    const void *words[] = {b.lengths, b.table, b.free_pages, b.counters,   b.step_lengths,
+                           b.newest,  b.slots, b.positions,  b.row_request};
     for (const void *w : words)
         if (!w || (uintptr_t)w % 4)
             return PCL_INVALID_SHAPE;
+    return PCL_OK;
+}
+
+int page_params(pcl_context *ctx, const pcl_page_batch *b, PageParams *p)
+{
+    if (!ctx || !b || check_batch(*b) != PCL_OK)
+        return PCL_INVALID_SHAPE;
     p->lengths = b->lengths;
     p->table = b->table;
     p->free_pages = b->free_pages;
@@ -456,13 +432,17 @@ int page_params(pcl_context *ctx, const pcl_page_batch *b, PageParams *p)
     p->step_rows = (int)b->step_rows;
     p->page_tokens = (uint32_t)b->page_tokens;
     p->max_tokens =
-        (uint32_t)std::min<int64_t>(b->table_stride * b->page_tokens, pcl::kMaxSlots);
+        (uint32_t)std::min<int64_t>(b->table_stride * b->page_tokens, kMaxSlots);
     p->err = ctx->err;
     (void)hipSetDevice(ctx->device);
     return PCL_OK;
 }
 
-} // namespace
+} // namespace pcl
+
+using pcl::PageParams;
+using pcl::page_launched;
+using pcl::page_params;
 
 extern "C" {
 
@@ -476,7 +456,7 @@ int pcl_page_reset(pcl_context *ctx, const pcl_page_batch *batch)
         {batch->requests * batch->table_stride, batch->pages, batch->step_rows});
     const int64_t groups = std::min<int64_t>((words + 255) / 256, 1024);
     pcl::page_reset_kernel<<<(unsigned)groups, pcl::kPageThreads, 0, ctx->stream>>>(p);
-    return launched("reset");
+    return page_launched("reset");
 }
 
 int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *new_tokens)
@@ -491,7 +471,7 @@ int pcl_page_step(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *
     const int groups = 1 + (p.step_rows + pcl::kPageThreads - 1) / pcl::kPageThreads;
     const size_t lds = (2 * (size_t)p.requests + 1) * sizeof(uint32_t);
     pcl::page_step_kernel<<<groups, pcl::kPageThreads, lds, ctx->stream>>>(p);
-    return launched("step");
+    return page_launched("step");
 }
 
 int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *kept)
@@ -505,7 +485,7 @@ int pcl_page_commit(pcl_context *ctx, const pcl_page_batch *batch, const int32_t
     p.in = kept;
     const size_t lds = ((size_t)p.requests + 1) * sizeof(uint32_t);
     pcl::page_return_kernel<true><<<1, pcl::kReturnThreads<true>, lds, ctx->stream>>>(p);
-    return launched("commit");
+    return page_launched("commit");
 }
 
 int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *finished)
@@ -519,7 +499,7 @@ int pcl_page_release(pcl_context *ctx, const pcl_page_batch *batch, const int32_
     p.in = finished;
     const size_t lds = 2 * ((size_t)p.requests + 1) * sizeof(uint32_t);
     pcl::page_return_kernel<false><<<1, pcl::kReturnThreads<false>, lds, ctx->stream>>>(p);
-    return launched("release");
+    return page_launched("release");
 }
 
 int pcl_paged_append(pcl_context *ctx, const pcl_page_pools *pools, const int32_t *slots,
@@ -548,7 +528,7 @@ int pcl_paged_append(pcl_context *ctx, const pcl_page_pools *pools, const int32_
         pcl::paged_rows_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
     else
         pcl::paged_rows_kernel<__bf16><<<grid, 256, 0, ctx->stream>>>(p);
-    return launched("append");
+    return page_launched("append");
 }
 
 } // extern "C"

@@ -69,7 +69,7 @@ constexpr size_t request_words_bytes(int requests)
 
 // Fills them by the whole workgroup; ends with a barrier.
 __device__ __forceinline__ void fill_request_words(const PagedParams &p, const RequestWords &r,
-                                                   uint32_t *waves)
+                                                   uint32_t *waves, int)
 {
     const int threads = blockDim.x;
     const int per = (p.requests + threads - 1) / threads;
@@ -93,6 +93,59 @@ __device__ __forceinline__ void fill_request_words(const PagedParams &p, const R
     }
     if (threadIdx.x == 0)
         r.off[p.requests] = total;
+    if (bad && blockIdx.x == 0)
+        atomicOr(p.err, kErrPages);
+    __syncthreads();
+}
+
+// The same of a tree launch: the items before each request over the KV heads
+// (chunks times units of `unit` rows), the tokens it holds with the step's and
+// without, and the step's row of its first new token.
+struct TreeWords {
+    uint32_t *off;
+    int32_t *len, *held, *row;
+};
+
+__device__ __forceinline__ TreeWords tree_words(uint32_t *lds, int requests)
+{
+    int32_t *words = reinterpret_cast<int32_t *>(lds);
+    return {lds, words + requests + 1, words + 2 * requests + 1, words + 3 * requests + 1};
+}
+
+constexpr size_t tree_words_bytes(int requests)
+{
+    return (4 * (size_t)requests + 1) * sizeof(uint32_t);
+}
+
+__device__ __forceinline__ void fill_request_words(const TreeParams &p, const TreeWords &r,
+                                                   uint64_t *waves, int unit)
+{
+    const int threads = blockDim.x;
+    const int per = (p.requests + threads - 1) / threads;
+    const int i0 = min((int)threadIdx.x * per, p.requests), i1 = min(i0 + per, p.requests);
+    uint64_t sum = 0; // (requests that share rows may add up past 2^32)
+    bool bad = false;
+    for (int i = i0; i < i1; ++i) {
+        const TreeKeys k = tree_keys(p, i, &bad);
+        const uint32_t n = (uint32_t)(k.len - k.held);
+        const uint32_t items = tree_chunks(p, k) * ((n * (uint32_t)p.group + unit - 1) / unit);
+        r.off[i] = items;
+        r.len[i] = k.len;
+        r.held[i] = k.held;
+        r.row[i] = k.row;
+        sum += items;
+    }
+    uint64_t total;
+    uint64_t at = block_offsets(sum, waves, &total);
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t items = r.off[i];
+        r.off[i] = (uint32_t)at;
+        at += items;
+    }
+    const bool fits = total * p.kvheads <= INT32_MAX;
+    bad |= !fits;
+    if (threadIdx.x == 0)
+        r.off[p.requests] = fits ? (uint32_t)total : 0;
     if (bad && blockIdx.x == 0)
         atomicOr(p.err, kErrPages);
     __syncthreads();
@@ -235,6 +288,12 @@ template <int DK, int R> struct PagedLds {
     int32_t slots[2][kChunk];             // of this item and the next
 };
 
+// Of a tree launch also each wave's first key that a row of the item attends
+// (kChunk: none); the slots of keys that none attends are -1.
+template <int DK, int R> struct TreeLds : PagedLds<DK, R> {
+    int32_t attended[2][4];
+};
+
 // find_range for a whole wave with one x: the lanes look at 64 offsets at once,
 // two LDS round trips instead of one for each bit of n (n at most 64 x 64): 256
 // requests of up to 2048 keys 101.4 -> 100.2 us.
@@ -261,7 +320,7 @@ struct PagedItem {
 };
 
 __device__ __forceinline__ PagedItem find_item(const PagedParams &p, const RequestWords &r,
-                                               uint32_t item)
+                                               uint32_t item, int)
 {
     const uint32_t per_chunk = (uint32_t)(p.kvheads * p.units);
     PagedItem x;
@@ -279,55 +338,226 @@ __device__ __forceinline__ PagedItem find_item(const PagedParams &p, const Reque
     return x;
 }
 
+// The same of a tree launch: the rows are the (new token, query head of the KV
+// head) pairs from `first_row` on, token by token. Keys that the unit's last token
+// cannot see (a chain's) are left out; `empty`: all of the chunk's.
+struct TreeItem : PagedItem {
+    int held, n, row;     // of the request: tokens held, new ones, the first's row
+    int first_row, nrows; // of the unit
+    bool empty, only;     // only: the request's one chunk
+};
+
+__device__ __forceinline__ TreeItem find_item(const TreeParams &p, const TreeWords &r,
+                                              uint32_t item, int unit)
+{
+    TreeItem x;
+    const uint32_t ci = item / (uint32_t)p.kvheads;
+    x.kh = (int)(item % (uint32_t)p.kvheads);
+    x.b = __builtin_amdgcn_readfirstlane(find_range_wave(r.off, p.requests, ci));
+    const int len = __builtin_amdgcn_readfirstlane(r.len[x.b]);
+    x.held = __builtin_amdgcn_readfirstlane(r.held[x.b]);
+    x.row = __builtin_amdgcn_readfirstlane(r.row[x.b]);
+    x.n = len - x.held;
+    const int rows = x.n * p.group, units = (rows + unit - 1) / unit;
+    const uint32_t rest = ci - __builtin_amdgcn_readfirstlane(r.off[x.b]);
+    const int chunk = units == 1 ? (int)rest : (int)(rest / (uint32_t)units);
+    x.unit = units == 1 ? 0 : (int)(rest % (uint32_t)units);
+    x.ci = (uint32_t)chunk; // (of the request)
+    const TreeKeys k = {x.row, x.held, len};
+    const int first = first_tree_key(p, x.held);
+    x.only = tree_chunks(p, k) == 1;
+    x.cbase = (first / kChunk + chunk) * kChunk;
+    x.first_row = x.unit * unit;
+    x.nrows = min(rows - x.first_row, unit);
+    int from = first, to = len - 1;
+    if (!p.masks) {
+        from = first_tree_key(p, x.held + x.first_row / p.group);
+        to = x.held + (x.first_row + x.nrows - 1) / p.group;
+    }
+    x.lo = max(from - x.cbase, 0);
+    x.hi = min(to - x.cbase, kChunk - 1);
+    x.empty = x.hi < x.lo;
+    if (x.empty)
+        x.lo = x.hi = 0;
+    return x;
+}
+
+// What a lane requests of an item's trees: masks of two of its new tokens (lane
+// 8 i + w: word w of token i and i + 8 of the unit's), the position of one of them
+// (lane i), and of its own keys where they are new.
+template <int KG> struct TreeFetched {
+    uint64_t mask[2];
+    int position, key[KG];
+};
+
+template <int KG>
+__device__ __forceinline__ void fetch_tree(const TreeParams &p, const TreeItem &x, int k0,
+                                           TreeFetched<KG> &f)
+{
+    const int lane = threadIdx.x & 63;
+    f.mask[0] = f.mask[1] = 0;
+    f.position = 0;
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg)
+        f.key[kg] = 0;
+    if (!p.masks)
+        return;
+    const int i0 = x.first_row / p.group;
+    const int last = (x.first_row + x.nrows - 1) / p.group;
+    if (x.cbase + x.hi >= x.held && lane % 8 < p.mask_words) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = i0 + lane / 8 + 8 * h;
+            if (i <= last)
+                f.mask[h] = p.masks[(int64_t)(x.row + i) * p.mask_words + lane % 8];
+        }
+    }
+    if (!p.window)
+        return;
+    f.position = p.positions[x.row + min(i0 + lane, last)];
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) {
+        const int t = x.cbase + k0 + 64 * kg + lane - x.held;
+        if (t >= 0 && t < x.n)
+            f.key[kg] = p.positions[x.row + t];
+    }
+}
+
+// The unit's rows that attend each of the lane's keys k0 + 64 kg + lane, bit r
+// for row r.
+template <int KG>
+__device__ __forceinline__ void attending_rows(const TreeParams &p, const TreeItem &x, int k0,
+                                               const TreeFetched<KG> &f, uint32_t (&rows)[KG])
+{
+    const int lane = threadIdx.x & 63;
+    const bool held = x.cbase + x.hi < x.held; // no new token among the keys
+    const bool whole = held && (!p.window || x.cbase + x.lo >= x.held + x.n - p.window);
+    bool in[KG];
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) {
+        const int key = k0 + 64 * kg + lane;
+        in[kg] = !x.empty && key >= x.lo && key <= x.hi;
+        rows[kg] = whole && in[kg] ? (1u << x.nrows) - 1 : 0;
+    }
+    if (whole)
+        return;
+    const int i0 = x.first_row / p.group;
+    int i = 0, j = x.first_row - i0 * p.group; // token (from i0 on) and head of row r
+    bool sees[KG];
+    for (int r = 0; r < x.nrows; ++r) {
+        if (r == 0 || j == 0) {
+            const int position = p.masks ? __shfl(f.position, i) : x.held + i0 + i;
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg) {
+                const int t = x.cbase + k0 + 64 * kg + lane, n = t - x.held;
+                bool s = n < 0 || n <= i0 + i;
+                int at = t;
+                if (p.masks) {
+                    if (!held) {
+                        const int w = min(max(n, 0), 511);
+                        const uint64_t word =
+                            __shfl((unsigned long long)f.mask[i / 8], 8 * (i % 8) + w / 64);
+                        s = n < 0 || (word >> (w % 64) & 1);
+                    }
+                    at = n < 0 ? t : f.key[kg];
+                }
+                sees[kg] = s && (!p.window || position - at < p.window);
+            }
+        }
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg)
+            rows[kg] |= in[kg] && sees[kg] ? 1u << r : 0;
+        if (++j == p.group) {
+            j = 0;
+            ++i;
+        }
+    }
+}
+
 // FULL: the head dim equals the padded head dim DK. Every wave keeps memory
 // busy through an item: the next item's pages and query are requested ahead of
 // the scores, the first V before the softmax, the next item's K with the last V.
 //
-// Three waves a SIMD (168 registers, no spill) for four query rows: 1 % faster
-// than the two or three that the compiler left room for; eight rows would spill.
-template <int DK, typename T, bool FULL, int R, int NB>
-__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
-                             (FULL && R == 1 && NB == 1 ? 3 : 1)) void paged_kv_kernel(PagedParams p)
+// TREE: the rows of a unit are several new tokens' (TreeParams), each with its own
+// keys; otherwise one token's query heads.
+template <int DK, typename T, bool FULL, int R, int NB, bool TREE>
+__device__ __forceinline__ void
+paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
 {
     using C = PagedCfg<DK, T, R>;
+    using Item = std::conditional_t<TREE, TreeItem, PagedItem>;
     constexpr int KG = C::KG, KP = C::KP, UK = C::UK, VL = C::VL, NQ = C::NQ;
-    __shared__ __attribute__((aligned(16))) PagedLds<DK, R> s;
-    __shared__ uint32_t waves[C::NW];
+    __shared__ __attribute__((aligned(16))) std::conditional_t<TREE, TreeLds<DK, R>, PagedLds<DK, R>> s;
+    __shared__ std::conditional_t<TREE, uint64_t, uint32_t> waves[C::NW];
     extern __shared__ __attribute__((aligned(16))) uint32_t dyn[];
-    const RequestWords req = request_words(dyn + ring_bytes<C, NB>() / 4, p.requests);
+    uint32_t *const words = dyn + ring_bytes<C, NB>() / 4;
+    const auto req = [&] {
+        if constexpr (TREE)
+            return tree_words(words, p.requests);
+        else
+            return request_words(words, p.requests);
+    }();
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
 
-    fill_request_words(p, req, waves);
+    fill_request_words(p, req, waves, C::kRowsUnit);
     if (blockIdx.x == 0)
-        for (int i = tid; i < p.requests; i += C::kThreads)
-            p.ws_req[i] = int4{(int)req.off[i], (int)(req.off[i + 1] - req.off[i]),
-                               first_key(p, req.len[i]) / kChunk, req.row[i]};
+        for (int i = tid; i < p.requests; i += C::kThreads) {
+            if constexpr (TREE) {
+                const TreeKeys k = {req.row[i], req.held[i], req.len[i]};
+                p.ws_req[i] = int4{k.row, tree_chunks(p, k), k.held, k.len - k.held};
+            } else {
+                p.ws_req[i] = int4{(int)req.off[i], (int)(req.off[i + 1] - req.off[i]),
+                                   first_key(p, req.len[i]) / kChunk, req.row[i]};
+            }
+        }
     const uint32_t items = __builtin_amdgcn_readfirstlane(req.off[p.requests]) *
-                           (uint32_t)(p.kvheads * p.units);
+                           (uint32_t)(TREE ? p.kvheads : p.kvheads * p.units);
     if (blockIdx.x >= items)
         return;
 
     // An item's page numbers of the thread's keys and its part of the unit's
     // query rows, requested (fetch) and then left in LDS (store).
+    struct Nothing {};
     struct Fetched {
         int page[KG];
         f4 q[NQ];
+        std::conditional_t<TREE, TreeFetched<KG>, Nothing> tree;
     };
     // a key outside [lo, hi] reads the nearest one inside (its score and
     // probability are not used)
-    auto position = [&](const PagedItem &x, int kg) {
+    auto position = [&](const Item &x, int kg) {
         const int key = 64 * (w * KG + kg) + lane;
         return (uint32_t)(x.cbase + min(max(key, x.lo), x.hi));
     };
-    auto fetch = [&](const PagedItem &x, Fetched &f) {
+    auto rows_of = [&](const Item &x) {
+        if constexpr (TREE)
+            return x.nrows;
+        else
+            return min(p.group - x.unit * C::kRowsUnit, C::kRowsUnit);
+    };
+    auto fetch = [&](const Item &x, Fetched &f) {
 #pragma unroll
         for (int kg = 0; kg < KG; ++kg)
             f.page[kg] = p.table[x.b * p.table_stride + position(x, kg) / p.page_tokens];
+        const int nrows = rows_of(x);
+        if constexpr (TREE) {
+            fetch_tree(p, x, 64 * w * KG, f.tree);
+            const float *q = p.q + (int64_t)x.kh * p.group * p.dim;
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int r = (tid + C::kThreads * i) / (DK / 4);
+                const int d = 4 * ((tid + C::kThreads * i) % (DK / 4));
+                const int at = x.first_row + min(r, nrows - 1); // row of the request
+                const int token = at / p.group, head = at - token * p.group;
+                f.q[i] = ldg4(q + (x.row + token) * p.q_stride + head * p.dim +
+                              (FULL || d < p.dim ? d : 0));
+            }
+            return;
+        }
         const int row = __builtin_amdgcn_readfirstlane(req.row[x.b]);
         const int h0 = x.kh * p.group + x.unit * C::kRowsUnit;
-        const int nrows = min(p.group - x.unit * C::kRowsUnit, C::kRowsUnit);
         const float *q = p.q + row * p.q_stride + (int64_t)h0 * p.dim;
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
@@ -336,7 +566,10 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             f.q[i] = ldg4(q + (r < nrows && (FULL || d < p.dim) ? r * p.dim + d : 0));
         }
     };
-    auto store = [&](const PagedItem &x, const Fetched &f, int32_t *slots) {
+    // (TREE) the rows that attend the lane's keys, of this item and the next
+    uint32_t seen[TREE ? KG : 1], seen_next[TREE ? KG : 1];
+    auto store = [&](const Item &x, const Fetched &f, int to) {
+        int32_t *slots = s.slots[to];
 #pragma unroll
         for (int kg = 0; kg < KG; ++kg) {
             int page = f.page[kg];
@@ -347,8 +580,22 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             slots[64 * (w * KG + kg) + lane] =
                 page * (int32_t)p.page_tokens + (int32_t)(position(x, kg) % p.page_tokens);
         }
+        if constexpr (TREE) {
+            attending_rows(p, x, 64 * w * KG, f.tree, seen_next);
+            int first = kChunk;
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg) {
+                if (!seen_next[kg])
+                    slots[64 * (w * KG + kg) + lane] = -1;
+                const uint64_t some = __ballot(seen_next[kg] != 0);
+                if (first == kChunk && some)
+                    first = 64 * (w * KG + kg) + __builtin_ctzll(some);
+            }
+            if (lane == 0)
+                s.attended[to][w] = first;
+        }
         // scaled; zero past the group and the head dim
-        const int nrows = min(p.group - x.unit * C::kRowsUnit, C::kRowsUnit);
+        const int nrows = rows_of(x);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
             const int r = (tid + C::kThreads * i) / (DK / 4);
@@ -372,18 +619,37 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
     struct Sources {
         const char *from[8];
     };
+    // (TREE) The slot that stands for the keys which no row of the item attends:
+    // one that some row does, so that no value is multiplied that the rows' own
+    // results do not hold, or slot 0 (such an item's sums are not used). After the
+    // barrier behind store().
+    int spare = 0, spare_next = 0; // of this item and the next
+    auto spare_slot = [&](int at) {
+        int first = kChunk;
+        if constexpr (TREE) {
+#pragma unroll
+            for (int i = 0; i < C::NW; ++i)
+                first = min(first, s.attended[at][i]);
+            first = first == kChunk ? 0 : s.slots[at][first];
+        }
+        return first;
+    };
+    auto slot_at = [&](const int32_t *slots, int key, int other) {
+        const int32_t slot = slots[key];
+        return (uint32_t)(TREE && slot < 0 ? other : slot);
+    };
     // Key group kg's K rows 8 e + lane / 8, each at the lane's 16-byte piece of the
     // line's: the pieces of row r lie in the order piece ^ (r & 7), so that a
     // lane's reads of its own row fall in other banks than its neighbours'.
     const int piece = (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
-    auto rows_k = [&](const int32_t *slots, int kh, int kg) {
+    auto rows_k = [&](const int32_t *slots, int other, int kh, int kg) {
         const char *base =
             static_cast<const char *>(p.k) + ((int64_t)kh * p.dim + piece) * sizeof(T);
         const int32_t *mine = slots + 64 * (w * KG + kg) + lane / 8;
         Sources c;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            c.from[e] = base + (uint64_t)(uint32_t)mine[8 * e] * row_bytes;
+            c.from[e] = base + (uint64_t)slot_at(mine, 8 * e, other) * row_bytes;
         return c;
     };
     // line `line` of those rows (a piece past the head dim: the row's first one)
@@ -407,7 +673,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         for (int e = 0; e < 8; ++e) {
             const int n = C::kKeysV * i + (e * 64 + lane) / C::kLanesV; // chain step from tile t0 on
             const int t = min(t0 + n / kTile, t1), k = n % kTile;
-            c.from[e] = base + (uint64_t)(uint32_t)slots[kTile * t + chain_key(k)] * row_bytes;
+            c.from[e] = base + (uint64_t)slot_at(slots, kTile * t + chain_key(k), spare) * row_bytes;
         }
         return c;
     };
@@ -425,27 +691,32 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
     };
     auto free_unit = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
-    PagedItem x = find_item(p, req, blockIdx.x);
+    Item x = find_item(p, req, blockIdx.x, C::kRowsUnit);
     {
         Fetched f;
         fetch(x, f);
-        store(x, f, s.slots[0]);
+        store(x, f, 0);
     }
     __syncthreads();
+    spare = spare_slot(0);
 #pragma unroll
     for (int i = 0; i < NB; ++i, at = at + 1 == NB ? 0 : at + 1)
-        issue(line_k(rows_k(s.slots[0], x.kh, i / KP), i % KP));
+        issue(line_k(rows_k(s.slots[0], spare, x.kh, i / KP), i % KP));
 
     int buf = 0;
     for (uint32_t item = blockIdx.x;; buf ^= 1) {
         const uint32_t next = item + gridDim.x;
         const bool more = next < items;
         // (without a next item this one is requested again, and not used)
-        const PagedItem y = find_item(p, req, more ? next : item);
+        const Item y = find_item(p, req, more ? next : item, C::kRowsUnit);
         Fetched f;
         fetch(y, f);
-        const int h0 = x.kh * p.group + x.unit * C::kRowsUnit;
-        const int nrows = min(p.group - x.unit * C::kRowsUnit, C::kRowsUnit);
+        const int nrows = rows_of(x);
+        if constexpr (TREE) {
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg)
+                seen[kg] = seen_next[kg];
+        }
         const int t0 = x.lo / kTile, t1 = x.hi / kTile; // tiles with attended keys
 
         // scores: lane = key
@@ -455,7 +726,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         // worked out during the unit before; the query is read ahead of the wait
         // (16 requests of up to 8192 keys, 32 query heads and one KV head of 128
         // dims, bf16: 50 -> 42 us; one request of 300 keys, 16 x 2 x 512: 32 -> 31).
-        Sources rows = rows_k(s.slots[buf], x.kh, NB / KP % KG);
+        Sources rows = rows_k(s.slots[buf], spare, x.kh, NB / KP % KG);
         Sources c = NB < UK ? line_k(rows, NB % KP) : sources_v(s.slots[buf], x.kh, t0, t1, 0);
         each<UK>([&](auto ic) {
             constexpr int i = decltype(ic)::value, kg = i / KP, M = C::kLine / 16;
@@ -489,7 +760,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             if constexpr (i + 1 < UK) {
                 if constexpr (n1 < UK) {
                     if constexpr (n1 % KP == 0)
-                        rows = rows_k(s.slots[buf], x.kh, n1 / KP);
+                        rows = rows_k(s.slots[buf], spare, x.kh, n1 / KP);
                     c = line_k(rows, n1 % KP);
                 } else {
                     c = sources_v(s.slots[buf], x.kh, t0, t1, n1 - UK);
@@ -515,12 +786,13 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             if (k0 > x.hi || k0 + 63 < x.lo)
                 continue;
             const int key = k0 + lane;
-            const bool ok = key >= x.lo && key <= x.hi;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 f4 tm;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    const bool ok = TREE ? seen[TREE ? kg : 0] >> (4 * r + e) & 1
+                                         : key >= x.lo && key <= x.hi;
                     float v = acc[kg][r][e];
                     v = p.softcap > 0.f ? soft_cap(v, p.softcap, p.inv_softcap) : v;
                     bad |= ok && 4 * r + e < nrows && !is_finite(v);
@@ -543,7 +815,6 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             if (k0 > x.hi || k0 + 63 < x.lo)
                 continue;
             const int key = k0 + lane, t = key / kTile;
-            const bool ok = key >= x.lo && key <= x.hi;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 f4 before, m; // running maxima before and at the tile
@@ -564,6 +835,8 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
                         before[e] = fmaxf(before[e], first[e]);
                     m[e] = fmaxf(before[e], mine[e]);
                     const float ms = safe_max(m[e]);
+                    const bool ok = TREE ? seen[TREE ? kg : 0] >> (4 * r + e) & 1
+                                         : key >= x.lo && key <= x.hi;
                     pr[e] = ok ? fexp(acc[kg][r][e] - ms) : 0.f;
                     alpha[e] = fexp(before[e] - ms);
                     sum[e] = sum_tile(pr[e]);
@@ -578,8 +851,9 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
                     s.last[r] = m;
             }
         }
-        store(y, f, s.slots[buf ^ 1]);
+        store(y, f, buf ^ 1);
         lds_barrier(); // probabilities, row sums and factors; the next query
+        spare_next = spare_slot(buf ^ 1);
 
         // the l chain and the P.V chains of the lane's VL output dims
         f4 l[R], O[R][VL];
@@ -622,7 +896,7 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         auto behind_v = [&](int i) {
             const int n = i + NB - rounds; // the next item's first units follow this one's
             return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
-                         : line_k(rows_k(s.slots[buf ^ 1], y.kh, n / KP), n % KP);
+                         : line_k(rows_k(s.slots[buf ^ 1], spare_next, y.kh, n / KP), n % KP);
         };
         c = behind_v(0);
         for (int i = 0; i < rounds; ++i) {
@@ -667,30 +941,63 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
         }
 
         const int vd = (64 * w + lane) * VL;
-        const bool only = req.off[x.b + 1] - req.off[x.b] == 1; // the request's only chunk
+        bool only; // the request's only chunk
+        if constexpr (TREE)
+            only = x.only;
+        else
+            only = req.off[x.b + 1] - req.off[x.b] == 1;
         bool nonfinite = false;
+        // row 4 r + e of the unit: its output row, partial and head
+        auto write_row = [&](int r, int e, float *row, int64_t part) {
+            float *dst = only ? row : p.ws_o + part * p.dim + vd;
+            const bool some = !TREE || l[r][e] != 0.f; // a key that the row attends
+            if (only && !some)
+                return;
+#pragma unroll
+            for (int j = 0; j < VL; ++j) {
+                const float v = only ? O[r][j][e] / l[r][e] : some ? O[r][j][e] : 0.f;
+                nonfinite |= only && !is_finite(v);
+                stg(dst + j, v);
+            }
+            if (!only && w == 0 && lane == 0) {
+                stg(p.ws_ml + 2 * part, s.last[r][e]);
+                stg(p.ws_ml + 2 * part + 1, l[r][e]);
+            }
+        };
         if (FULL || vd < p.dim) {
+            if constexpr (TREE) {
+                if (!x.empty) {
+                    int token = x.first_row / p.group, h = x.first_row - token * p.group;
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+                    for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (4 * r + e >= nrows)
-                        continue;
-                    const int h = h0 + 4 * r + e;
-                    const int64_t part = (int64_t)x.ci * p.qheads + h;
-                    float *dst = only ? p.out + req.row[x.b] * p.o_stride + (int64_t)h * p.dim + vd
-                                      : p.ws_o + part * p.dim + vd;
-#pragma unroll
-                    for (int j = 0; j < VL; ++j) {
-                        const float v = only ? O[r][j][e] / l[r][e] : O[r][j][e];
-                        nonfinite |= only && !is_finite(v);
-                        stg(dst + j, v);
-                    }
-                    if (!only && w == 0 && lane == 0) {
-                        stg(p.ws_ml + 2 * part, s.last[r][e]);
-                        stg(p.ws_ml + 2 * part + 1, l[r][e]);
-                    }
+                        for (int e = 0; e < 4; ++e) {
+                            if (4 * r + e >= nrows)
+                                continue;
+                            const int head = x.kh * p.group + h;
+                            write_row(r, e,
+                                      p.out + (x.row + token) * p.o_stride +
+                                          (int64_t)head * p.dim + vd,
+                                      ((int64_t)(x.row + token) * p.row_chunks + x.ci) * p.qheads + head);
+                            if (++h == p.group) {
+                                h = 0;
+                                ++token;
+                            }
+                        }
                 }
+            } else {
+                const int h0 = x.kh * p.group + x.unit * C::kRowsUnit;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (4 * r + e >= nrows)
+                            continue;
+                        const int h = h0 + 4 * r + e;
+                        write_row(r, e, p.out + req.row[x.b] * p.o_stride + (int64_t)h * p.dim + vd,
+                                  (int64_t)x.ci * p.qheads + h);
+                    }
+            }
         }
         if (nonfinite)
             atomicOr(p.err, kErrOutput);
@@ -698,9 +1005,25 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
             break;
         item = next;
         x = y;
+        spare = spare_next;
     }
     // no copy may land in LDS that another workgroup owns by then
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+}
+
+// Three waves a SIMD (168 registers, no spill) for four query rows: 1 % faster
+// than the two or three that the compiler left room for; eight rows would spill.
+template <int DK, typename T, bool FULL, int R, int NB>
+__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
+                             (FULL && R == 1 && NB == 1 ? 3 : 1)) void paged_kv_kernel(PagedParams p)
+{
+    paged_kv_body<DK, T, FULL, R, NB, false>(p);
+}
+
+template <int DK, typename T, bool FULL, int R, int NB>
+__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_tree_kernel(TreeParams p)
+{
+    paged_kv_body<DK, T, FULL, R, NB, true>(p);
 }
 
 // Workgroups of a kernel that a CU holds at once, for batches of up to
@@ -708,11 +1031,16 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
 // the request words take more LDS).
 constexpr int kFewRequests = 256;
 
-template <int DK, typename T, bool FULL, int R, int NB>
+template <int DK, typename T, bool FULL, int R, int NB, bool TREE>
 static hipError_t resident_groups(int requests, int *groups)
 {
     using C = PagedCfg<DK, T, R>;
-    const auto kernel = (const void *)paged_kv_kernel<DK, T, FULL, R, NB>;
+    const void *kernel;
+    if constexpr (TREE)
+        kernel = (const void *)paged_tree_kernel<DK, T, FULL, R, NB>;
+    else
+        kernel = (const void *)paged_kv_kernel<DK, T, FULL, R, NB>;
+    constexpr auto words = TREE ? tree_words_bytes : request_words_bytes;
     static std::atomic<int> known[kMaxDevices];
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -724,19 +1052,18 @@ static hipError_t resident_groups(int requests, int *groups)
     if (*groups > 0 && requests <= kFewRequests)
         return hipSuccess;
     constexpr size_t ring = ring_bytes<C, NB>();
-    static_assert(sizeof(PagedLds<DK, R>) + 64 + ring + request_words_bytes(kMaxRequests) <=
-                      160 * 1024,
+    static_assert(sizeof(TreeLds<DK, R>) + 64 + ring + words(kMaxRequests) <= 160 * 1024,
                   "the LDS of a CU");
     if (*groups == 0) {
         // more than 64 KiB of LDS in all must be allowed once per device
         e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(ring + request_words_bytes(kMaxRequests)));
+                                (int)(ring + words(kMaxRequests)));
         if (e != hipSuccess)
             return e;
     }
     const int most = requests <= kFewRequests ? kFewRequests : requests;
     e = hipOccupancyMaxActiveBlocksPerMultiprocessor(groups, kernel, C::kThreads,
-                                                     ring + request_words_bytes(most));
+                                                     ring + words(most));
     if (e != hipSuccess)
         return e;
     *groups = std::max(*groups, 1);
@@ -745,25 +1072,33 @@ static hipError_t resident_groups(int requests, int *groups)
     return hipSuccess;
 }
 
-template <int DK, typename T, bool FULL, int R, int NB>
-static hipError_t launch_paged(const PagedParams &p, int64_t items, hipStream_t stream)
+template <int DK, typename T, bool FULL, int R, int NB, typename P>
+static hipError_t launch_paged(const P &p, int64_t items, hipStream_t stream)
 {
     using C = PagedCfg<DK, T, R>;
+    constexpr bool TREE = std::is_same_v<P, TreeParams>;
     int groups = 0;
-    const hipError_t e = resident_groups<DK, T, FULL, R, NB>(p.requests, &groups);
+    const hipError_t e = resident_groups<DK, T, FULL, R, NB, TREE>(p.requests, &groups);
     if (e != hipSuccess)
         return e;
     const int64_t grid = std::min<int64_t>(items, (int64_t)groups * std::max(device_cus(), 1));
-    paged_kv_kernel<DK, T, FULL, R, NB>
-        <<<(unsigned)grid, C::kThreads, ring_bytes<C, NB>() + request_words_bytes(p.requests),
-           stream>>>(p);
+    if constexpr (TREE)
+        paged_tree_kernel<DK, T, FULL, R, NB>
+            <<<(unsigned)grid, C::kThreads, ring_bytes<C, NB>() + tree_words_bytes(p.requests),
+               stream>>>(p);
+    else
+        paged_kv_kernel<DK, T, FULL, R, NB>
+            <<<(unsigned)grid, C::kThreads, ring_bytes<C, NB>() + request_words_bytes(p.requests),
+               stream>>>(p);
     return hipGetLastError();
 }
 
-template <int DK, typename T, bool FULL, int R>
-static hipError_t launch_paged(PagedParams p, int64_t chunks, hipStream_t stream)
+// `rows`: of a KV head that one request has at most; `chunks`: of the requests at
+// their longest.
+template <int DK, typename T, bool FULL, int R, typename P>
+static hipError_t launch_paged(P p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    p.units = (p.group + PagedCfg<DK, T, R>::kRowsUnit - 1) / PagedCfg<DK, T, R>::kRowsUnit;
+    p.units = (int)((rows + PagedCfg<DK, T, R>::kRowsUnit - 1) / PagedCfg<DK, T, R>::kRowsUnit);
     // (the items at the requests' longest)
     const int64_t items = chunks * p.kvheads * p.units;
     if constexpr (FULL && R <= 2) {
@@ -773,26 +1108,34 @@ static hipError_t launch_paged(PagedParams p, int64_t chunks, hipStream_t stream
     return launch_paged<DK, T, FULL, R, 1>(p, items, stream);
 }
 
-template <int DK, typename T, bool FULL>
-static hipError_t launch_paged(const PagedParams &p, int64_t chunks, hipStream_t stream)
+template <int DK, typename T, bool FULL, typename P>
+static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    return p.group <= 4   ? launch_paged<DK, T, FULL, 1>(p, chunks, stream)
-           : p.group <= 8 ? launch_paged<DK, T, FULL, 2>(p, chunks, stream)
-                          : launch_paged<DK, T, FULL, 4>(p, chunks, stream);
+    return rows <= 4   ? launch_paged<DK, T, FULL, 1>(p, rows, chunks, stream)
+           : rows <= 8 ? launch_paged<DK, T, FULL, 2>(p, rows, chunks, stream)
+                       : launch_paged<DK, T, FULL, 4>(p, rows, chunks, stream);
 }
 
-template <int DK, typename T>
-static hipError_t launch_paged(const PagedParams &p, int64_t chunks, hipStream_t stream)
+template <int DK, typename T, typename P>
+static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    return p.dim == DK ? launch_paged<DK, T, true>(p, chunks, stream)
-                       : launch_paged<DK, T, false>(p, chunks, stream);
+    return p.dim == DK ? launch_paged<DK, T, true>(p, rows, chunks, stream)
+                       : launch_paged<DK, T, false>(p, rows, chunks, stream);
 }
 
 template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream)
 {
-    return bf16 ? launch_paged<DK, __bf16>(p, chunks, stream)
-                : launch_paged<DK, float>(p, chunks, stream);
+    return bf16 ? launch_paged<DK, __bf16>(p, p.group, chunks, stream)
+                : launch_paged<DK, float>(p, p.group, chunks, stream);
+}
+
+template <int DK>
+hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream)
+{
+    const int64_t rows = (int64_t)p.max_new * p.group;
+    return bf16 ? launch_paged<DK, __bf16>(p, rows, chunks, stream)
+                : launch_paged<DK, float>(p, rows, chunks, stream);
 }
 
 } // namespace pcl

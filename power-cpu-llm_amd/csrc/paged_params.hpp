@@ -19,7 +19,8 @@ struct PagedParams {
     int64_t o_stride;
     float *ws_o, *ws_ml; // [chunk][qheads][dim], [chunk][qheads][2]
     int4 *ws_req;        // [requests] for the combine: chunks before it, its chunks,
-                         // its first chunk, its row
+                         // its first chunk, its row (a tree launch: its first row, its
+                         // chunks, its held tokens, its new ones)
     int *err;
     int requests, q_rows, max_length, window, pages;
     uint32_t page_tokens;
@@ -58,9 +59,56 @@ __device__ __forceinline__ int request_chunks(const RequestKeys &r)
     return r.len ? (r.len - 1) / kChunk + 1 - r.first / kChunk : 0;
 }
 
+// Of a launch over every new token of a step (lengths: with the step's tokens).
+struct TreeParams : PagedParams {
+    const int32_t *held, *newest;  // [requests] tokens before the step, row of the last one
+    const uint64_t *masks;         // [q_rows][mask_words], or null: a chain
+    const int32_t *positions;      // [q_rows], with masks and a window
+    int mask_words, max_new;
+    int row_chunks; // partials of a row: chunks that one request may have
+};
+
+// A request's keys [0, len), the tokens that it held before the step, and the
+// step's row of its first new token; none (held = len) for a request without one.
+struct TreeKeys {
+    int row, held, len;
+};
+
+// The first key that any new token attends: their positions start at the held
+// tokens' count.
+__device__ __forceinline__ int first_tree_key(const TreeParams &p, int position)
+{
+    return p.window && position >= p.window ? position - p.window + 1 : 0;
+}
+
+__device__ __forceinline__ TreeKeys tree_keys(const TreeParams &p, int i, bool *bad)
+{
+    TreeKeys r;
+    const int last = p.newest[i];
+    r.held = p.held[i];
+    r.len = p.lengths[i];
+    const int64_t n = (int64_t)r.len - r.held;
+    r.row = (int)(last - n + 1);
+    if (last < 0 || n == 0) {
+        r.held = r.len = 0;
+    } else if (r.held < 0 || n < 0 || r.len > p.max_length || n > p.max_new ||
+               last - n + 1 < 0 || last >= p.q_rows || (p.masks && n > 64 * p.mask_words)) {
+        *bad = true;
+        r.held = r.len = 0;
+    }
+    return r;
+}
+
+__device__ __forceinline__ int tree_chunks(const TreeParams &p, const TreeKeys &r)
+{
+    return r.len > r.held ? (r.len - 1) / kChunk + 1 - first_tree_key(p, r.held) / kChunk : 0;
+}
+
 // The chunk kernel of a launch of at most `chunks` chunks, at padded head dim
 // DK (64, 128, 256 or 512, a source file each).
 template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream);
+template <int DK>
+hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream);
 
 } // namespace pcl

@@ -1,0 +1,4 @@
+// The chunk kernels of the attention of a step's new tokens at padded head dim 64.
+#include "paged_kv.hpp"
+
+template hipError_t pcl::launch_paged_tree<64>(const TreeParams &, bool, int64_t, hipStream_t);
