@@ -733,7 +733,8 @@ int pcl_paged_copy(pcl_context *ctx, const pcl_page_pools *pools, int64_t layers
  * positions[row] and attends the held keys [0, lengths[b]) and each new token j with
  * bit j of masks[row] (any bits; pcl_page_tree_masks makes a tree's). With a window a
  * token attends only keys whose position is less than `window` before its own (the
- * new tokens' by positions; at least lengths[b] each). Requests without new tokens
+ * new tokens' by positions, which lie from lengths[b] to step_lengths[b] - 1).
+ * Requests without new tokens
  * or with a negative newest are left out, and a token that attends no key too: their
  * output rows stay as they were. Queries are scaled and scores capped as in
  * pcl_attention_desc. A token's output has the bits that pcl_attention_launch gives

@@ -19,9 +19,11 @@ SOURCES = ["csrc/split_kv.hip", "csrc/pipe_kv.hip", "csrc/spread_kv.hip",
            "csrc/paged_kv_d64.hip", "csrc/paged_kv_d128.hip", "csrc/paged_kv_d256.hip",
            "csrc/paged_kv_d512.hip", "csrc/page_trees.hip", "csrc/paged_tree.hip",
            "csrc/paged_tree_d64.hip", "csrc/paged_tree_d128.hip", "csrc/paged_tree_d256.hip",
-           "csrc/paged_tree_d512.hip"]
+           "csrc/paged_tree_d512.hip", "csrc/paged_rows_d64.hip", "csrc/paged_rows_d128.hip",
+           "csrc/paged_rows_d256.hip", "csrc/paged_rows_d512.hip"]
 HEADERS = ["csrc/attention_device.hpp", "csrc/context.hpp", "csrc/launch.hpp", "csrc/paged.hpp",
-           "csrc/paged_params.hpp", "csrc/paged_kv.hpp", "csrc/paged_combine.hpp",
+           "csrc/paged_params.hpp", "csrc/paged_kv.hpp", "csrc/paged_rows.hpp",
+           "csrc/paged_combine.hpp",
            "csrc/page_batch.hpp",
            os.path.join(ROOT, "include", "pcl_attention.h")]
 

@@ -23,7 +23,6 @@
 namespace pcl {
 
 constexpr int64_t kMaxTreeWords = 8;
-constexpr int kTreeThreads = 64 * (int)kMaxTreeWords; // new tokens of a tree
 
 struct TreeStepParams {
     PageParams b;

@@ -1111,9 +1111,14 @@ static hipError_t launch_paged(P p, int64_t rows, int64_t chunks, hipStream_t st
 template <int DK, typename T, bool FULL, typename P>
 static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    return rows <= 4   ? launch_paged<DK, T, FULL, 1>(p, rows, chunks, stream)
-           : rows <= 8 ? launch_paged<DK, T, FULL, 2>(p, rows, chunks, stream)
-                       : launch_paged<DK, T, FULL, 4>(p, rows, chunks, stream);
+    if (rows <= 4)
+        return launch_paged<DK, T, FULL, 1>(p, rows, chunks, stream);
+    if (rows <= 8)
+        return launch_paged<DK, T, FULL, 2>(p, rows, chunks, stream);
+    if constexpr (std::is_same_v<P, TreeParams>)
+        return launch_paged_rows<DK>(p, std::is_same_v<T, __bf16>, rows, chunks, stream);
+    else
+        return launch_paged<DK, T, FULL, 4>(p, rows, chunks, stream);
 }
 
 template <int DK, typename T, typename P>

@@ -110,5 +110,9 @@ template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream);
 template <int DK>
 hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream);
+// `rows`: query rows of a KV head that one request has at most, above eight.
+template <int DK>
+hipError_t launch_paged_rows(const TreeParams &p, bool bf16, int64_t rows, int64_t chunks,
+                             hipStream_t stream);
 
 } // namespace pcl

@@ -1,0 +1,735 @@
+// Attention of a step's new tokens over a paged KV cache where a KV head has more
+// than eight query rows: units of 16 U rows, 256-key chunks, on 16 x 16 x 4 f32 MFMAs.
+//
+// The mathematics and the arithmetic are those of paged_kv.hpp and its tree
+// launches. Four waves score 64 keys each against all the unit's rows and leave the
+// probabilities in LDS; then each runs the P.V chains of a quarter of the dims over
+// the whole chunk. So each byte of K and V is read from LDS once, by one wave, and
+// feeds U instructions of 16 rows; a lane of the result is a row, and a tile's
+// maximum and sum take two exchanges between lanes (a lane a key takes five).
+#pragma once
+
+#include "paged_kv.hpp"
+
+namespace pcl {
+
+template <int DK, typename T, int U> struct RowsCfg {
+    static constexpr int NW = 4;
+    static constexpr int kThreads = 64 * NW;
+    static constexpr int kRowsUnit = 16 * U;
+    static constexpr int kLine = 128 / (int)sizeof(T); // dims of a K unit
+    static constexpr int UK = (DK + kLine - 1) / kLine; // K units
+    static constexpr int SU = kLine / 32;              // score chain steps (32 dims) of a unit
+    static constexpr int VL = DK / 64;                 // 16-dim blocks of a wave's dims
+    static constexpr int kRowV = 16 * VL * (int)sizeof(T); // bytes of a V row of the wave
+    static constexpr int kLanesV = kRowV / 16;         // lanes that copy it
+    static constexpr int kKeysV = 8192 / kRowV < kChunk ? 8192 / kRowV : kChunk;
+    static constexpr int NQ = U * DK / 64; // query quads of a thread
+    static_assert(kKeysV >= 16, "units of 16 keys and more");
+};
+
+template <int DK, int U> struct RowsLds {
+    f4 q[U][DK / 32][2][64];              // [rows][32 dims][half of a lane's eight][lane]
+    f4 p[U][kTilesPerChunk][2][64];       // [rows][tile][16 keys][lane]
+    float max[kTilesPerChunk][16 * U], alpha[kTilesPerChunk][16 * U], sum[kTilesPerChunk][16 * U];
+    int32_t slots[2][kChunk];             // of this item and the next
+    int32_t attended[2][4];               // each wave's first attended key
+};
+
+constexpr size_t rows_ring_bytes(int buffers)
+{
+    return (size_t)4 * buffers * 8192;
+}
+
+// What a lane requests of an item's trees: of its row in each 16 of the unit's the
+// 64 mask bits of the wave's keys (two words) and the position; and of its key.
+template <int U> struct RowsFetched {
+    uint64_t mask[U][2];
+    int position[U], key;
+};
+
+// The lane's row in 16 rows rg of the unit: the new token (the last one's past the
+// rows).
+__device__ __forceinline__ int row_token(const TreeParams &p, const TreeItem &x, int rg)
+{
+    return (x.first_row + min(16 * rg + (int)(threadIdx.x & 15), x.nrows - 1)) / p.group;
+}
+
+template <int U>
+__device__ __forceinline__ void fetch_rows(const TreeParams &p, const TreeItem &x, int k0,
+                                           RowsFetched<U> &f)
+{
+#pragma unroll
+    for (int rg = 0; rg < U; ++rg) {
+        f.mask[rg][0] = f.mask[rg][1] = 0;
+        f.position[rg] = 0;
+    }
+    f.key = 0;
+    if (!p.masks)
+        return;
+    const int n0 = x.cbase + k0 - x.held; // new token of the wave's first key
+    if (n0 + 63 >= 0 && n0 < x.n) {
+        const int w0 = n0 < 0 ? -1 : n0 / 64;
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg) {
+            if (16 * rg >= x.nrows)
+                continue;
+            const uint64_t *row =
+                p.masks + (int64_t)(x.row + row_token(p, x, rg)) * p.mask_words;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (w0 + h >= 0 && w0 + h < p.mask_words)
+                    f.mask[rg][h] = row[w0 + h];
+        }
+    }
+    if (!p.window)
+        return;
+#pragma unroll
+    for (int rg = 0; rg < U; ++rg)
+        if (16 * rg < x.nrows)
+            f.position[rg] = p.positions[x.row + row_token(p, x, rg)];
+    const int n = n0 + (int)(threadIdx.x & 63);
+    if (n >= 0 && n < x.n)
+        f.key = p.positions[x.row + n];
+}
+
+// Bits [lo, hi] of 64 (none where hi < lo; lo and hi any).
+__device__ __forceinline__ uint64_t bit_range(int lo, int hi)
+{
+    lo = max(lo, 0);
+    hi = min(hi, 63);
+    return hi < lo ? 0 : ~(uint64_t)0 >> (63 - (hi - lo)) << lo;
+}
+
+// The wave's keys k0 .. k0 + 63 that the lane's rows attend, bit k for key k0 + k.
+template <int U>
+__device__ __forceinline__ void attended_keys(const TreeParams &p, const TreeItem &x, int k0,
+                                              const RowsFetched<U> &f, uint64_t (&see)[U])
+{
+    const int n0 = x.cbase + k0 - x.held;
+    const uint64_t in = x.empty ? 0 : bit_range(x.lo - k0, x.hi - k0);
+    const uint64_t held = bit_range(0, -n0 - 1); // keys held before the step
+#pragma unroll
+    for (int rg = 0; rg < U; ++rg) {
+        see[rg] = 0;
+        if (16 * rg >= x.nrows)
+            continue;
+        if (16 * rg + (int)(threadIdx.x & 15) >= x.nrows)
+            continue;
+        const int token = row_token(p, x, rg);
+        if (!p.masks) {
+            const int to = x.held + token, from = first_tree_key(p, to);
+            see[rg] = in & bit_range(from - x.cbase - k0, to - x.cbase - k0);
+            continue;
+        }
+        // the mask's bits from n0 on
+        const int s = n0 & 63;
+        const uint64_t bits =
+            s ? f.mask[rg][0] >> s | f.mask[rg][1] << (64 - s) : f.mask[rg][0];
+        see[rg] = in & (held | (bits & ~held));
+        if (p.window)
+            see[rg] &= ~held | bit_range(first_tree_key(p, f.position[rg]) - x.cbase - k0, 63);
+    }
+    // a window that is shorter than the trees
+    if (p.masks && p.window && x.n > p.window && n0 + 63 >= 0) {
+        for (int k = max(-n0, 0); k < 64; ++k) {
+            const int at = __builtin_amdgcn_readlane(f.key, k);
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg)
+                if (f.position[rg] - at >= p.window)
+                    see[rg] &= ~((uint64_t)1 << k);
+        }
+    }
+}
+
+// The bits that any lane with another lane % 16 has, on all of them.
+__device__ __forceinline__ uint32_t or_rows(uint32_t x)
+{
+    x |= __builtin_amdgcn_update_dpp(0, x, kDppXor1, 0xf, 0xf, true);
+    x |= __builtin_amdgcn_update_dpp(0, x, kDppXor2, 0xf, 0xf, true);
+    x |= __builtin_amdgcn_update_dpp(0, x, kDppMirror8, 0xf, 0xf, true);
+    x |= __builtin_amdgcn_update_dpp(0, x, kDppMirror16, 0xf, 0xf, true);
+    return x;
+}
+
+template <int DK, typename T, bool FULL, int U, int NB>
+__global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) void paged_rows_kernel(
+    TreeParams p)
+{
+    using C = RowsCfg<DK, T, U>;
+    constexpr int UK = C::UK, VL = C::VL, NQ = C::NQ;
+    static_assert(NB <= UK, "the ring holds one row's lines");
+    extern __shared__ __attribute__((aligned(16))) uint32_t dyn[];
+    using Lds = RowsLds<DK, U>;
+    Lds &s = *reinterpret_cast<Lds *>(dyn);
+    uint32_t *const rings = dyn + sizeof(Lds) / 4;
+    __shared__ uint64_t waves[C::NW];
+    const TreeWords req = tree_words(rings + rows_ring_bytes(NB) / 4, p.requests);
+    const int tid = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int k0 = 64 * w; // the wave's keys
+
+    fill_request_words(p, req, waves, C::kRowsUnit);
+    if (blockIdx.x == 0)
+        for (int i = tid; i < p.requests; i += C::kThreads) {
+            const TreeKeys k = {req.row[i], req.held[i], req.len[i]};
+            p.ws_req[i] = int4{k.row, tree_chunks(p, k), k.held, k.len - k.held};
+        }
+    const uint32_t items =
+        __builtin_amdgcn_readfirstlane(req.off[p.requests]) * (uint32_t)p.kvheads;
+    if (blockIdx.x >= items)
+        return;
+
+    struct Fetched {
+        int page;
+        RowsFetched<U> tree;
+    };
+    auto position = [&](const TreeItem &x) {
+        return (uint32_t)(x.cbase + min(max(k0 + lane, x.lo), x.hi));
+    };
+    auto fetch = [&](const TreeItem &x, Fetched &f) {
+        f.page = p.table[x.b * p.table_stride + position(x) / p.page_tokens];
+        fetch_rows(p, x, k0, f.tree);
+    };
+    auto fetch_q = [&](const TreeItem &x, f4 (&fq)[NQ]) {
+        const float *q = p.q + (int64_t)x.kh * p.group * p.dim;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int r = (tid + C::kThreads * i) / (DK / 4);
+            const int d = 4 * ((tid + C::kThreads * i) % (DK / 4));
+            const int at = x.first_row + min(r, x.nrows - 1);
+            const int token = at / p.group, head = at - token * p.group;
+            fq[i] = ldg4(q + (x.row + token) * p.q_stride + head * p.dim +
+                         (FULL || d < p.dim ? d : 0));
+        }
+    };
+    auto store_q = [&](const TreeItem &x, const f4 (&fq)[NQ]) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int r = (tid + C::kThreads * i) / (DK / 4);
+            const int d = 4 * ((tid + C::kThreads * i) % (DK / 4));
+            const bool in = r < x.nrows && (FULL || d < p.dim);
+            f4 v = fq[i] * p.q_scale;
+            v = in ? v : f4{0.f, 0.f, 0.f, 0.f};
+            s.q[r / 16][d / 32][d % 8 / 4][d % 32 / 8 * 16 + r % 16] = v;
+        }
+    };
+    uint64_t see[U], see_next[U]; // the wave's keys that the lane's rows attend
+    auto store = [&](const TreeItem &x, const Fetched &f, int to) {
+        int page = f.page;
+        if (page < 0 || page >= p.pages) {
+            atomicOr(p.err, kErrPages);
+            page = 0;
+        }
+        int slot = page * (int32_t)p.page_tokens + (int32_t)(position(x) % p.page_tokens);
+        attended_keys(p, x, k0, f.tree, see_next);
+        uint64_t any = 0;
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg)
+            any |= see_next[rg];
+        any = (uint64_t)or_rows((uint32_t)(any >> 32)) << 32 | or_rows((uint32_t)any);
+        if (!(any >> lane & 1))
+            slot = -1;
+        s.slots[to][k0 + lane] = slot;
+        if (lane == 0)
+            s.attended[to][w] = any ? k0 + __builtin_ctzll(any) : kChunk;
+    };
+    // (paged_kv.hpp has the ring and its units)
+    uint32_t *const ring = rings + (size_t)w * NB * 2048;
+    int at = 0;
+    const uint32_t row_bytes = (uint32_t)(p.row_stride * sizeof(T));
+    struct Sources {
+        const char *from[8];
+    };
+    int spare = 0, spare_next = 0;
+    auto spare_slot = [&](int to) {
+        int first = kChunk;
+#pragma unroll
+        for (int i = 0; i < C::NW; ++i)
+            first = min(first, s.attended[to][i]);
+        return first == kChunk ? 0 : s.slots[to][first];
+    };
+    auto slot_at = [&](const int32_t *slots, int key, int other) {
+        const int32_t slot = slots[key];
+        return (uint32_t)(slot < 0 ? other : slot);
+    };
+    const int piece = (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
+    auto rows_k = [&](const int32_t *slots, int other, int kh) {
+        const char *base =
+            static_cast<const char *>(p.k) + ((int64_t)kh * p.dim + piece) * sizeof(T);
+        const int32_t *mine = slots + k0 + lane / 8;
+        Sources c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            c.from[e] = base + (uint64_t)slot_at(mine, 8 * e, other) * row_bytes;
+        return c;
+    };
+    auto line_k = [&](const Sources &rows, int line) {
+        const int d = C::kLine * line;
+        const int64_t step = (FULL || d + piece < p.dim ? d : -piece) * (int64_t)sizeof(T);
+        Sources c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            c.from[e] = rows.from[e] + step;
+        return c;
+    };
+    auto sources_v = [&](const int32_t *slots, int kh, int t0, int t1, int i) {
+        const int d = 16 * VL * w + lane % C::kLanesV * (16 / (int)sizeof(T));
+        const char *base = static_cast<const char *>(p.v) +
+                           ((int64_t)kh * p.dim + (FULL || d < p.dim ? d : 0)) * sizeof(T);
+        Sources c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int n = C::kKeysV * i + (e * 64 + lane) / C::kLanesV; // chain step from tile t0 on
+            const int t = min(t0 + n / kTile, t1), k = n % kTile;
+            c.from[e] = base + (uint64_t)slot_at(slots, kTile * t + chain_key(k), spare) * row_bytes;
+        }
+        return c;
+    };
+    auto issue = [&](const Sources &c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            __builtin_amdgcn_global_load_lds((global_ptr)c.from[e],
+                                             (lds_ptr)(ring + at * 2048 + e * 256), 16, 0,
+                                             U == 1 ? kStreamed : 0);
+    };
+    auto wait_unit = [&]() {
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(8 * (NB - 1)));
+        asm volatile("" ::: "memory");
+    };
+    auto free_unit = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+    auto next_buffer = [&]() { at = at + 1 == NB ? 0 : at + 1; };
+
+    TreeItem x = find_item(p, req, blockIdx.x, C::kRowsUnit);
+    {
+        Fetched f;
+        f4 fq[NQ];
+        fetch(x, f);
+        fetch_q(x, fq);
+        store(x, f, 0);
+        store_q(x, fq);
+    }
+    __syncthreads();
+    spare = spare_slot(0);
+    {
+        const Sources rows = rows_k(s.slots[0], spare, x.kh);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            issue(line_k(rows, i));
+            next_buffer();
+        }
+    }
+
+    int buf = 0;
+    for (uint32_t item = blockIdx.x;; buf ^= 1) {
+        const uint32_t next = item + gridDim.x;
+        const bool more = next < items;
+        // (without a next item this one is requested again, and not used)
+        const TreeItem y = find_item(p, req, more ? next : item, C::kRowsUnit);
+        Fetched f;
+        fetch(y, f);
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg)
+            see[rg] = see_next[rg];
+        const int groups = (x.nrows + 15) / 16;
+        const int t0 = x.lo / kTile, t1 = x.hi / kTile; // tiles with attended keys
+        const bool mine = k0 <= x.hi && k0 + 63 >= x.lo;
+
+        // scores: D of 16 keys x 16 rows
+        f4 acc[U][4];
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                acc[rg][b] = f4{0.f, 0.f, 0.f, 0.f};
+        const Sources rows = rows_k(s.slots[buf], spare, x.kh);
+        Sources c = NB < UK ? line_k(rows, NB) : sources_v(s.slots[buf], x.kh, t0, t1, NB - UK);
+#pragma unroll 1
+        for (int i = 0; i < UK; ++i) {
+            wait_unit();
+            u4 kw[4][2];
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // f32: halves of a lane's eight dims; bf16: the eight of two steps
+                    const int j = sizeof(T) == 4 ? 2 * g + h : 4 * h + g;
+                    const int d = C::kLine * i + j * (16 / (int)sizeof(T));
+                    u4 v = *(const u4 *)(ring + at * 2048 + 32 * (16 * b + col) +
+                                         4 * (j ^ (col & 7)));
+                    if (!FULL && d >= p.dim)
+                        v = u4{0u, 0u, 0u, 0u};
+                    kw[b][h] = v;
+                }
+            free_unit();
+            issue(c);
+            next_buffer();
+            if (i + 1 < UK)
+                c = i + 1 + NB < UK ? line_k(rows, i + 1 + NB)
+                                    : sources_v(s.slots[buf], x.kh, t0, t1, i + 1 + NB - UK);
+            if (!mine)
+                continue;
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                if (rg >= groups)
+                    continue;
+#pragma unroll
+                for (int u = 0; u < C::SU; ++u) {
+                    if (C::SU * i + u >= DK / 32)
+                        continue;
+                    const f4 qa = s.q[rg][C::SU * i + u][0][lane], qb = s.q[rg][C::SU * i + u][1][lane];
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            float k;
+                            if constexpr (sizeof(T) == 4)
+                                k = __uint_as_float(kw[b][jj / 4][jj % 4]);
+                            else
+                                k = jj % 2 ? bf16_high(kw[b][u][jj / 2])
+                                           : bf16_low(kw[b][u][jj / 2]);
+                            acc[rg][b] = mfma(k, jj < 4 ? qa[jj % 4] : qb[jj % 4], acc[rg][b]);
+                        }
+                }
+            }
+        }
+        f4 fq[NQ];
+        fetch_q(y, fq);
+
+        bool bad = false;
+        auto ok_of = [&](int rg, int t, bool ok[2][4]) { // of the wave's tile t
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    ok[b][r] = (uint32_t)(see[rg] >> (32 * t)) >> (16 * b + 4 * g + r) & 1;
+        };
+        if (mine) {
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                if (rg >= groups)
+                    continue;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    bool ok[2][4];
+                    float v[2][4];
+                    ok_of(rg, t, ok);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            v[b][r] = acc[rg][2 * t + b][r];
+                            if (p.softcap > 0.f)
+                                v[b][r] = soft_cap(v[b][r], p.softcap, p.inv_softcap);
+                            acc[rg][2 * t + b][r] = v[b][r];
+                        }
+                    bad |= bad_scores(v, ok);
+                    const float m = tile_max(v, ok);
+                    if (g == 0)
+                        s.max[2 * w + t][16 * rg + col] = m;
+                }
+            }
+        }
+        if (bad)
+            atomicOr(p.err, kErrScore);
+        lds_barrier(); // every tile's maximum; the query is used
+
+        if (mine) {
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                if (rg >= groups)
+                    continue;
+                float before = kNegInf;
+                for (int t = t0; t < 2 * w; ++t)
+                    before = fmaxf(before, s.max[t][16 * rg + col]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int tile = 2 * w + t;
+                    if (tile < t0 || tile > t1)
+                        continue;
+                    bool ok[2][4];
+                    float v[2][4], pr[2][4];
+                    ok_of(rg, t, ok);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            v[b][r] = acc[rg][2 * t + b][r];
+                    const float m = fmaxf(before, s.max[tile][16 * rg + col]);
+                    const float ms = safe_max(m);
+                    const float sum = tile_probs(v, ok, ms, pr);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        s.p[rg][tile][b][lane] = f4{pr[b][0], pr[b][1], pr[b][2], pr[b][3]};
+                    if (g == 0) {
+                        s.alpha[tile][16 * rg + col] = fexp(before - ms);
+                        s.sum[tile][16 * rg + col] = sum;
+                    }
+                    before = m;
+                }
+            }
+        }
+        float last[U]; // the chunk's maximum
+        if (w == 0) {
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                last[rg] = kNegInf;
+                for (int t = t0; t <= t1 && rg < groups; ++t)
+                    last[rg] = fmaxf(last[rg], s.max[t][16 * rg + col]);
+            }
+        }
+        store(y, f, buf ^ 1);
+        store_q(y, fq);
+        lds_barrier(); // probabilities, row sums and factors; the next query
+        spare_next = spare_slot(buf ^ 1);
+
+        // the l chain and the P.V chains of the wave's dims: D of 16 dims x 16 rows
+        float l[U];
+        f4 O[U][VL];
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg) {
+            l[rg] = 0.f;
+#pragma unroll
+            for (int j = 0; j < VL; ++j)
+                O[rg][j] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        const int units = ((t1 - t0 + 1) * kTile + C::kKeysV - 1) / C::kKeysV;
+        const int rounds = max(units, NB);
+        auto behind_v = [&](int i) {
+            const int n = i + NB - rounds; // the next item's first units follow this one's
+            return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
+                         : line_k(rows_k(s.slots[buf ^ 1], spare_next, y.kh), n);
+        };
+        c = behind_v(0);
+#pragma unroll 1
+        for (int i = 0; i < rounds; ++i) {
+            wait_unit();
+            // 16 keys at a time: four chain steps of 4 keys (r), each with the lane's
+            // own key and VL dims
+            constexpr int WV = (VL * (int)sizeof(T) + 3) / 4; // words of a lane's values
+            constexpr int kSixteens = C::kKeysV / 16, kHeld = kSixteens < 4 ? kSixteens : 4;
+#pragma unroll 1
+            for (int h0 = 0; h0 < kSixteens; h0 += kHeld) {
+                uint32_t vw[kHeld][4][WV];
+#pragma unroll
+                for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const char *row = reinterpret_cast<const char *>(ring + at * 2048) +
+                                          (16 * (h0 + h) + 4 * r + g) * C::kRowV;
+                        if constexpr (WV >= 4) {
+#pragma unroll
+                            for (int k = 0; k < WV / 4; ++k) {
+                                const u4 v = *(const u4 *)(row + 256 * k + 16 * col);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    vw[h][r][4 * k + e] = v[e];
+                            }
+                        } else if constexpr (WV == 2) {
+                            const u2 v = *(const u2 *)(row + 8 * col);
+                            vw[h][r][0] = v.x;
+                            vw[h][r][1] = v.y;
+                        } else if constexpr (VL * sizeof(T) == 4) {
+                            vw[h][r][0] = *(const uint32_t *)(row + 4 * col);
+                        } else {
+                            vw[h][r][0] = *(const uint16_t *)(row + 2 * col);
+                        }
+                    }
+                if (h0 + kHeld >= kSixteens) {
+                    free_unit();
+                    issue(c);
+                    next_buffer();
+                    if (i + 1 < rounds)
+                        c = behind_v(i + 1);
+                }
+                if (i >= units)
+                    continue;
+#pragma unroll
+                for (int h = 0; h < kHeld; ++h) {
+                    const int n = C::kKeysV * i + 16 * (h0 + h), t = t0 + n / kTile;
+                    if (C::kKeysV > kTile && t > t1)
+                        continue;
+                    const int b = C::kKeysV < kTile ? i % 2 : h % 2;
+#pragma unroll
+                    for (int rg = 0; rg < U; ++rg) {
+                        if (rg >= groups)
+                            continue;
+                        if (b == 0) {
+                            const float alpha = s.alpha[t][16 * rg + col];
+                            l[rg] = __builtin_fmaf(l[rg], alpha, s.sum[t][16 * rg + col]);
+#pragma unroll
+                            for (int j = 0; j < VL; ++j)
+                                O[rg][j] = O[rg][j] * alpha;
+                        }
+                        const f4 pr = s.p[rg][t][b][lane];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int j = 0; j < VL; ++j)
+                                O[rg][j] = mfma(value_of<T>(vw[h][r], j), pr[r], O[rg][j]);
+                    }
+                }
+            }
+        }
+
+        // D's dim 4 g + e of block j: the dim that lane 4 g + e of the operand had
+        auto dim_of = [&](int j, int e) {
+            const int lane16 = 4 * g + e;
+            if (VL == 8 && sizeof(T) == 4)
+                return 16 * VL * w + 64 * (j / 4) + 4 * lane16 + j % 4;
+            return 16 * VL * w + VL * lane16 + j;
+        };
+        bool nonfinite = false;
+        if (!x.empty) {
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                const int r = 16 * rg + col;
+                if (r >= x.nrows)
+                    continue;
+                const int f0 = x.first_row + r, token = f0 / p.group;
+                const int head = x.kh * p.group + f0 - token * p.group;
+                const int64_t part = ((int64_t)(x.row + token) * p.row_chunks + x.ci) * p.qheads + head;
+                const bool some = l[rg] != 0.f; // a key that the row attends
+                float *dst = x.only ? p.out + (x.row + token) * p.o_stride + (int64_t)head * p.dim
+                                    : p.ws_o + part * p.dim;
+                if (x.only && !some)
+                    continue;
+                auto value = [&](int j, int e) {
+                    const float v = x.only ? O[rg][j][e] / l[rg] : some ? O[rg][j][e] : 0.f;
+                    return v;
+                };
+                if constexpr (VL >= 4) {
+#pragma unroll
+                    for (int j = 0; j < VL; j += 4)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int d = dim_of(j, e);
+                            if (!FULL && d >= p.dim)
+                                continue;
+                            f4 v;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                v[k] = value(j + k, e);
+                                nonfinite |= x.only && !is_finite(v[k]);
+                            }
+                            stg4(dst + d, v);
+                        }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VL; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int d = dim_of(j, e);
+                            if (!FULL && d >= p.dim)
+                                continue;
+                            const float v = value(j, e);
+                            nonfinite |= x.only && !is_finite(v);
+                            stg(dst + d, v);
+                        }
+                }
+                if (!x.only && w == 0 && g == 0) {
+                    stg(p.ws_ml + 2 * part, last[rg]);
+                    stg(p.ws_ml + 2 * part + 1, l[rg]);
+                }
+            }
+        }
+        if (nonfinite)
+            atomicOr(p.err, kErrOutput);
+        if (!more)
+            break;
+        item = next;
+        x = y;
+        spare = spare_next;
+    }
+    // no copy may land in LDS that another workgroup owns by then
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+}
+
+// The LDS of a CU, less the kernel's static words.
+constexpr size_t kRowsLds = 160 * 1024 - 64;
+
+template <int DK, int U, int NB> constexpr size_t rows_lds_bytes(int requests)
+{
+    return sizeof(RowsLds<DK, U>) + rows_ring_bytes(NB) + tree_words_bytes(requests);
+}
+
+// Workgroups that a CU holds at once (as resident_groups of paged_kv.hpp).
+template <int DK, typename T, bool FULL, int U, int NB>
+static hipError_t resident_rows(int requests, int *groups)
+{
+    const auto kernel = (const void *)paged_rows_kernel<DK, T, FULL, U, NB>;
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess)
+        return e;
+    if (dev < 0 || dev >= kMaxDevices)
+        return hipErrorInvalidDevice;
+    *groups = known[dev].load(std::memory_order_acquire);
+    if (*groups > 0 && requests <= kFewRequests)
+        return hipSuccess;
+    constexpr auto bytes = rows_lds_bytes<DK, U, NB>;
+    static_assert(bytes(kFewRequests) <= kRowsLds, "the LDS of a CU");
+    if (*groups == 0) {
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)std::min(bytes(kMaxRequests), kRowsLds));
+        if (e != hipSuccess)
+            return e;
+    }
+    const int most = requests <= kFewRequests ? kFewRequests : requests;
+    e = hipOccupancyMaxActiveBlocksPerMultiprocessor(groups, kernel, 256, bytes(most));
+    if (e != hipSuccess)
+        return e;
+    *groups = std::max(*groups, 1);
+    if (requests <= kFewRequests)
+        known[dev].store(*groups, std::memory_order_release);
+    return hipSuccess;
+}
+
+template <int DK, typename T, bool FULL, int U, int NB>
+static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
+{
+    int groups = 0;
+    const hipError_t e = resident_rows<DK, T, FULL, U, NB>(p.requests, &groups);
+    if (e != hipSuccess)
+        return e;
+    const int64_t units = (rows + 16 * U - 1) / (16 * U);
+    const int64_t grid = std::min<int64_t>(chunks * p.kvheads * units,
+                                           (int64_t)groups * std::max(device_cus(), 1));
+    paged_rows_kernel<DK, T, FULL, U, NB>
+        <<<(unsigned)grid, 256, rows_lds_bytes<DK, U, NB>(p.requests), stream>>>(p);
+    return hipGetLastError();
+}
+
+// Rows of 16 of the largest unit: what the LDS of a CU holds beside the rings.
+constexpr int most_groups(int dk)
+{
+    return dk == 512 ? 2 : dk == 256 ? 3 : 4;
+}
+
+template <int DK, typename T, bool FULL>
+static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
+{
+    // (the words of many requests leave less LDS)
+    constexpr int M = most_groups(DK);
+    static_assert(rows_lds_bytes<DK, 1, 1>(kMaxRequests) <= kRowsLds, "one always fits");
+    if (rows > 32 && rows_lds_bytes<DK, M, 1>(p.requests) <= kRowsLds)
+        return launch_rows<DK, T, FULL, M, 1>(p, rows, chunks, stream);
+    if (rows > 16 && rows_lds_bytes<DK, 2, 1>(p.requests) <= kRowsLds)
+        return launch_rows<DK, T, FULL, 2, 1>(p, rows, chunks, stream);
+    return launch_rows<DK, T, FULL, 1, 1>(p, rows, chunks, stream);
+}
+
+template <int DK>
+hipError_t launch_paged_rows(const TreeParams &p, bool bf16, int64_t rows, int64_t chunks,
+                             hipStream_t stream)
+{
+    if (p.dim == DK)
+        return bf16 ? launch_rows<DK, __bf16, true>(p, rows, chunks, stream)
+                    : launch_rows<DK, float, true>(p, rows, chunks, stream);
+    return bf16 ? launch_rows<DK, __bf16, false>(p, rows, chunks, stream)
+                : launch_rows<DK, float, false>(p, rows, chunks, stream);
+}
+
+} // namespace pcl
