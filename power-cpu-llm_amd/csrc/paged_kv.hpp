@@ -351,8 +351,8 @@ __device__ __forceinline__ TreeItem find_item(const TreeParams &p, const TreeWor
                                               uint32_t item, int unit)
 {
     TreeItem x;
-    const uint32_t ci = item / (uint32_t)p.kvheads;
-    x.kh = (int)(item % (uint32_t)p.kvheads);
+    const uint32_t ci = divided(item, p.by_kvheads);
+    x.kh = (int)(item - ci * (uint32_t)p.kvheads);
     x.b = __builtin_amdgcn_readfirstlane(find_range_wave(r.off, p.requests, ci));
     const int len = __builtin_amdgcn_readfirstlane(r.len[x.b]);
     x.held = __builtin_amdgcn_readfirstlane(r.held[x.b]);
@@ -371,8 +371,8 @@ __device__ __forceinline__ TreeItem find_item(const TreeParams &p, const TreeWor
     x.nrows = min(rows - x.first_row, unit);
     int from = first, to = len - 1;
     if (!p.masks) {
-        from = first_tree_key(p, x.held + x.first_row / p.group);
-        to = x.held + (x.first_row + x.nrows - 1) / p.group;
+        from = first_tree_key(p, x.held + (int)divided(x.first_row, p.by_group));
+        to = x.held + (int)divided(x.first_row + x.nrows - 1, p.by_group);
     }
     x.lo = max(from - x.cbase, 0);
     x.hi = min(to - x.cbase, kChunk - 1);
@@ -402,8 +402,8 @@ __device__ __forceinline__ void fetch_tree(const TreeParams &p, const TreeItem &
         f.key[kg] = 0;
     if (!p.masks)
         return;
-    const int i0 = x.first_row / p.group;
-    const int last = (x.first_row + x.nrows - 1) / p.group;
+    const int i0 = (int)divided(x.first_row, p.by_group);
+    const int last = (int)divided(x.first_row + x.nrows - 1, p.by_group);
     if (x.cbase + x.hi >= x.held && lane % 8 < p.mask_words) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -441,7 +441,7 @@ __device__ __forceinline__ void attending_rows(const TreeParams &p, const TreeIt
     }
     if (whole)
         return;
-    const int i0 = x.first_row / p.group;
+    const int i0 = (int)divided(x.first_row, p.by_group);
     int i = 0, j = x.first_row - i0 * p.group; // token (from i0 on) and head of row r
     bool sees[KG];
     for (int r = 0; r < x.nrows; ++r) {
@@ -531,6 +531,12 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
         const int key = 64 * (w * KG + kg) + lane;
         return (uint32_t)(x.cbase + min(max(key, x.lo), x.hi));
     };
+    auto page_of = [&](uint32_t position) {
+        if constexpr (TREE)
+            return divided(position, p.by_page_tokens);
+        else
+            return position / p.page_tokens;
+    };
     auto rows_of = [&](const Item &x) {
         if constexpr (TREE)
             return x.nrows;
@@ -540,7 +546,7 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
     auto fetch = [&](const Item &x, Fetched &f) {
 #pragma unroll
         for (int kg = 0; kg < KG; ++kg)
-            f.page[kg] = p.table[x.b * p.table_stride + position(x, kg) / p.page_tokens];
+            f.page[kg] = p.table[x.b * p.table_stride + page_of(position(x, kg))];
         const int nrows = rows_of(x);
         if constexpr (TREE) {
             fetch_tree(p, x, 64 * w * KG, f.tree);
@@ -550,7 +556,7 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
                 const int r = (tid + C::kThreads * i) / (DK / 4);
                 const int d = 4 * ((tid + C::kThreads * i) % (DK / 4));
                 const int at = x.first_row + min(r, nrows - 1); // row of the request
-                const int token = at / p.group, head = at - token * p.group;
+                const int token = (int)divided(at, p.by_group), head = at - token * p.group;
                 f.q[i] = ldg4(q + (x.row + token) * p.q_stride + head * p.dim +
                               (FULL || d < p.dim ? d : 0));
             }
@@ -577,8 +583,9 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
                 atomicOr(p.err, kErrPages);
                 page = 0;
             }
+            const uint32_t t = position(x, kg);
             slots[64 * (w * KG + kg) + lane] =
-                page * (int32_t)p.page_tokens + (int32_t)(position(x, kg) % p.page_tokens);
+                page * (int32_t)p.page_tokens + (int32_t)(t - page_of(t) * p.page_tokens);
         }
         if constexpr (TREE) {
             attending_rows(p, x, 64 * w * KG, f.tree, seen_next);
@@ -967,7 +974,8 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
         if (FULL || vd < p.dim) {
             if constexpr (TREE) {
                 if (!x.empty) {
-                    int token = x.first_row / p.group, h = x.first_row - token * p.group;
+                    int token = (int)divided(x.first_row, p.by_group);
+                    int h = x.first_row - token * p.group;
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll

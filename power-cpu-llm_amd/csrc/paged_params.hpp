@@ -59,6 +59,28 @@ __device__ __forceinline__ int request_chunks(const RequestKeys &r)
     return r.len ? (r.len - 1) / kChunk + 1 - r.first / kChunk : 0;
 }
 
+// Division of a value below 2^31 by a divisor of the launch, at most 2^12: with s =
+// ceil(log2 d) - 1 and mul = ceil(2^(32 + s) / d), (x mul) >> (32 + s) is exact as
+// mul d - 2^(32 + s) < d <= 2^(s + 1) and x below 2^31 (1: x itself).
+struct Divisor {
+    uint32_t mul, shift; // mul 0: by 1
+};
+
+inline Divisor divisor(uint32_t d)
+{
+    if (d == 1)
+        return {0, 0};
+    uint32_t s = 0;
+    while ((2u << s) < d)
+        ++s;
+    return {(uint32_t)((((uint64_t)1 << (32 + s)) + d - 1) / d), s};
+}
+
+__device__ __forceinline__ uint32_t divided(uint32_t x, const Divisor &d)
+{
+    return d.mul ? __umulhi(x, d.mul) >> d.shift : x;
+}
+
 // Of a launch over every new token of a step (lengths: with the step's tokens).
 struct TreeParams : PagedParams {
     const int32_t *held, *newest;  // [requests] tokens before the step, row of the last one
@@ -66,6 +88,7 @@ struct TreeParams : PagedParams {
     const int32_t *positions;      // [q_rows], with masks and a window
     int mask_words, max_new;
     int row_chunks; // partials of a row: chunks that one request may have
+    Divisor by_group, by_kvheads, by_page_tokens;
 };
 
 // A request's keys [0, len), the tokens that it held before the step, and the

@@ -13,19 +13,27 @@
 
 namespace pcl {
 
+// Eight waves of 32 keys at head dims 256 and 512, four of 64 below (a wave's part of
+// a V row is 16 dims at least). Units of the ring are a 128-byte line of the wave's K
+// rows or its dims of some V rows.
 template <int DK, typename T, int U> struct RowsCfg {
-    static constexpr int NW = 4;
+    static constexpr int NW = DK >= 256 ? 8 : 4;
     static constexpr int kThreads = 64 * NW;
     static constexpr int kRowsUnit = 16 * U;
+    static constexpr int KW = kChunk / NW;             // keys of a wave
+    static constexpr int TW = KW / kTile;              // tiles of them
+    static constexpr int kUnit = 128 * KW;             // bytes of a ring unit
+    static constexpr int NE = kUnit / 1024;            // copies of one
     static constexpr int kLine = 128 / (int)sizeof(T); // dims of a K unit
     static constexpr int UK = (DK + kLine - 1) / kLine; // K units
     static constexpr int SU = kLine / 32;              // score chain steps (32 dims) of a unit
-    static constexpr int VL = DK / 64;                 // 16-dim blocks of a wave's dims
+    static constexpr int VL = DK / 16 / NW;            // 16-dim blocks of a wave's dims
     static constexpr int kRowV = 16 * VL * (int)sizeof(T); // bytes of a V row of the wave
     static constexpr int kLanesV = kRowV / 16;         // lanes that copy it
-    static constexpr int kKeysV = 8192 / kRowV < kChunk ? 8192 / kRowV : kChunk;
-    static constexpr int NQ = U * DK / 64; // query quads of a thread
+    static constexpr int kKeysV = kUnit / kRowV < kChunk ? kUnit / kRowV : kChunk;
+    static constexpr int NQ = U * DK / 16 / NW; // copies of the query by a wave
     static_assert(kKeysV >= 16, "units of 16 keys and more");
+    static_assert(VL == 1 || VL == 2 || VL == 4, "a lane's values are one read");
 };
 
 template <int DK, int U> struct RowsLds {
@@ -33,12 +41,13 @@ template <int DK, int U> struct RowsLds {
     f4 p[U][kTilesPerChunk][2][64];       // [rows][tile][16 keys][lane]
     float max[kTilesPerChunk][16 * U], alpha[kTilesPerChunk][16 * U], sum[kTilesPerChunk][16 * U];
     int32_t slots[2][kChunk];             // of this item and the next
-    int32_t attended[2][4];               // each wave's first attended key
+    int32_t attended[2][8];               // each wave's first attended key
 };
 
+// The rings of all waves.
 constexpr size_t rows_ring_bytes(int buffers)
 {
-    return (size_t)4 * buffers * 8192;
+    return (size_t)buffers * 128 * kChunk;
 }
 
 // What a lane requests of an item's trees: of its row in each 16 of the unit's the
@@ -52,7 +61,8 @@ template <int U> struct RowsFetched {
 // rows).
 __device__ __forceinline__ int row_token(const TreeParams &p, const TreeItem &x, int rg)
 {
-    return (x.first_row + min(16 * rg + (int)(threadIdx.x & 15), x.nrows - 1)) / p.group;
+    return (int)divided(x.first_row + min(16 * rg + (int)(threadIdx.x & 15), x.nrows - 1),
+                        p.by_group);
 }
 
 template <int U>
@@ -153,22 +163,21 @@ __device__ __forceinline__ uint32_t or_rows(uint32_t x)
 }
 
 template <int DK, typename T, bool FULL, int U, int NB>
-__global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) void paged_rows_kernel(
-    TreeParams p)
+__global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_kernel(TreeParams p)
 {
     using C = RowsCfg<DK, T, U>;
-    constexpr int UK = C::UK, VL = C::VL, NQ = C::NQ;
+    constexpr int NW = C::NW, KW = C::KW, TW = C::TW, UK = C::UK, VL = C::VL, SU = C::SU;
     static_assert(NB <= UK, "the ring holds one row's lines");
     extern __shared__ __attribute__((aligned(16))) uint32_t dyn[];
     using Lds = RowsLds<DK, U>;
     Lds &s = *reinterpret_cast<Lds *>(dyn);
     uint32_t *const rings = dyn + sizeof(Lds) / 4;
-    __shared__ uint64_t waves[C::NW];
+    __shared__ uint64_t waves[NW];
     const TreeWords req = tree_words(rings + rows_ring_bytes(NB) / 4, p.requests);
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, col = lane & 15, g = lane >> 4;
-    const int k0 = 64 * w; // the wave's keys
+    const int k0 = KW * w; // the wave's keys
 
     fill_request_words(p, req, waves, C::kRowsUnit);
     if (blockIdx.x == 0)
@@ -186,34 +195,35 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
         RowsFetched<U> tree;
     };
     auto position = [&](const TreeItem &x) {
-        return (uint32_t)(x.cbase + min(max(k0 + lane, x.lo), x.hi));
+        return (uint32_t)(x.cbase + min(max(k0 + lane % KW, x.lo), x.hi));
     };
     auto fetch = [&](const TreeItem &x, Fetched &f) {
-        f.page = p.table[x.b * p.table_stride + position(x) / p.page_tokens];
+        f.page = p.table[x.b * p.table_stride + divided(position(x), p.by_page_tokens)];
         fetch_rows(p, x, k0, f.tree);
     };
-    auto fetch_q = [&](const TreeItem &x, f4 (&fq)[NQ]) {
-        const float *q = p.q + (int64_t)x.kh * p.group * p.dim;
+    // The unit's query rows into LDS (as they are: they are scaled where they are
+    // read): a copy is four of the eight dims of a lane, for 16 rows and 32 dims. Rows
+    // past the last are the last one's, dims past the head dim the first ones.
+    auto issue_q = [&](const TreeItem &x) {
+        const float *row[U];
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int r = (tid + C::kThreads * i) / (DK / 4);
-            const int d = 4 * ((tid + C::kThreads * i) % (DK / 4));
-            const int at = x.first_row + min(r, x.nrows - 1);
-            const int token = at / p.group, head = at - token * p.group;
-            fq[i] = ldg4(q + (x.row + token) * p.q_stride + head * p.dim +
-                         (FULL || d < p.dim ? d : 0));
+        for (int rg = 0; rg < U; ++rg) {
+            const int token = row_token(p, x, rg);
+            const int head = x.first_row + min(16 * rg + col, x.nrows - 1) - token * p.group;
+            row[rg] = p.q + (x.row + token) * p.q_stride +
+                      (int64_t)(x.kh * p.group + head) * p.dim;
         }
-    };
-    auto store_q = [&](const TreeItem &x, const f4 (&fq)[NQ]) {
+        constexpr int kPart = DK / 16 / NW; // copies of 16 rows by a wave
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int r = (tid + C::kThreads * i) / (DK / 4);
-            const int d = 4 * ((tid + C::kThreads * i) % (DK / 4));
-            const bool in = r < x.nrows && (FULL || d < p.dim);
-            f4 v = fq[i] * p.q_scale;
-            v = in ? v : f4{0.f, 0.f, 0.f, 0.f};
-            s.q[r / 16][d / 32][d % 8 / 4][d % 32 / 8 * 16 + r % 16] = v;
-        }
+        for (int rg = 0; rg < U; ++rg)
+#pragma unroll
+            for (int i = 0; i < kPart; ++i) {
+                const int n = w * kPart + i, u = n / 2, hh = n % 2;
+                const int d = 32 * u + 8 * g + 4 * hh;
+                __builtin_amdgcn_global_load_lds(
+                    (global_ptr)(row[rg] + (FULL || d < p.dim ? d : 0)),
+                    (lds_ptr)(&s.q[rg][u][hh][0]), 16, 0, 0);
+            }
     };
     uint64_t see[U], see_next[U]; // the wave's keys that the lane's rows attend
     auto store = [&](const TreeItem &x, const Fetched &f, int to) {
@@ -222,7 +232,9 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
             atomicOr(p.err, kErrPages);
             page = 0;
         }
-        int slot = page * (int32_t)p.page_tokens + (int32_t)(position(x) % p.page_tokens);
+        const uint32_t t = position(x);
+        int slot = page * (int32_t)p.page_tokens +
+                   (int32_t)(t - divided(t, p.by_page_tokens) * p.page_tokens);
         attended_keys(p, x, k0, f.tree, see_next);
         uint64_t any = 0;
 #pragma unroll
@@ -231,22 +243,24 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
         any = (uint64_t)or_rows((uint32_t)(any >> 32)) << 32 | or_rows((uint32_t)any);
         if (!(any >> lane & 1))
             slot = -1;
-        s.slots[to][k0 + lane] = slot;
+        if (lane < KW)
+            s.slots[to][k0 + lane] = slot;
         if (lane == 0)
             s.attended[to][w] = any ? k0 + __builtin_ctzll(any) : kChunk;
     };
     // (paged_kv.hpp has the ring and its units)
-    uint32_t *const ring = rings + (size_t)w * NB * 2048;
+    constexpr int kWords = C::kUnit / 4;
+    uint32_t *const ring = rings + (size_t)w * NB * kWords;
     int at = 0;
     const uint32_t row_bytes = (uint32_t)(p.row_stride * sizeof(T));
     struct Sources {
-        const char *from[8];
+        const char *from[C::NE];
     };
     int spare = 0, spare_next = 0;
     auto spare_slot = [&](int to) {
         int first = kChunk;
 #pragma unroll
-        for (int i = 0; i < C::NW; ++i)
+        for (int i = 0; i < NW; ++i)
             first = min(first, s.attended[to][i]);
         return first == kChunk ? 0 : s.slots[to][first];
     };
@@ -261,7 +275,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
         const int32_t *mine = slots + k0 + lane / 8;
         Sources c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < C::NE; ++e)
             c.from[e] = base + (uint64_t)slot_at(mine, 8 * e, other) * row_bytes;
         return c;
     };
@@ -270,7 +284,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
         const int64_t step = (FULL || d + piece < p.dim ? d : -piece) * (int64_t)sizeof(T);
         Sources c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < C::NE; ++e)
             c.from[e] = rows.from[e] + step;
         return c;
     };
@@ -280,7 +294,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                            ((int64_t)kh * p.dim + (FULL || d < p.dim ? d : 0)) * sizeof(T);
         Sources c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < C::NE; ++e) {
             const int n = C::kKeysV * i + (e * 64 + lane) / C::kLanesV; // chain step from tile t0 on
             const int t = min(t0 + n / kTile, t1), k = n % kTile;
             c.from[e] = base + (uint64_t)slot_at(slots, kTile * t + chain_key(k), spare) * row_bytes;
@@ -289,13 +303,13 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
     };
     auto issue = [&](const Sources &c) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < C::NE; ++e)
             __builtin_amdgcn_global_load_lds((global_ptr)c.from[e],
-                                             (lds_ptr)(ring + at * 2048 + e * 256), 16, 0,
+                                             (lds_ptr)(ring + at * kWords + e * 256), 16, 0,
                                              U == 1 ? kStreamed : 0);
     };
     auto wait_unit = [&]() {
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(8 * (NB - 1)));
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::NE * (NB - 1)));
         asm volatile("" ::: "memory");
     };
     auto free_unit = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
@@ -304,12 +318,11 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
     TreeItem x = find_item(p, req, blockIdx.x, C::kRowsUnit);
     {
         Fetched f;
-        f4 fq[NQ];
+        issue_q(x);
         fetch(x, f);
-        fetch_q(x, fq);
         store(x, f, 0);
-        store_q(x, fq);
     }
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // the query's copies
     __syncthreads();
     spare = spare_slot(0);
     {
@@ -334,29 +347,41 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
             see[rg] = see_next[rg];
         const int groups = (x.nrows + 15) / 16;
         const int t0 = x.lo / kTile, t1 = x.hi / kTile; // tiles with attended keys
-        const bool mine = k0 <= x.hi && k0 + 63 >= x.lo;
+        const bool mine = k0 <= x.hi && k0 + KW - 1 >= x.lo;
 
         // scores: D of 16 keys x 16 rows
-        f4 acc[U][4];
+        f4 acc[U][2 * TW];
 #pragma unroll
         for (int rg = 0; rg < U; ++rg)
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < 2 * TW; ++b)
                 acc[rg][b] = f4{0.f, 0.f, 0.f, 0.f};
         const Sources rows = rows_k(s.slots[buf], spare, x.kh);
         Sources c = NB < UK ? line_k(rows, NB) : sources_v(s.slots[buf], x.kh, t0, t1, NB - UK);
 #pragma unroll 1
         for (int i = 0; i < UK; ++i) {
-            wait_unit();
-            u4 kw[4][2];
+            f4 q[U][SU][2]; // read ahead of the wait
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int rg = 0; rg < U; ++rg)
+#pragma unroll
+                for (int u = 0; u < SU; ++u)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const int n = min(SU * i + u, DK / 32 - 1);
+                        q[rg][u][hh] = s.q[rg][n][hh][lane] * p.q_scale;
+                        if (!FULL && 32 * n + 8 * g + 4 * hh >= p.dim)
+                            q[rg][u][hh] = f4{0.f, 0.f, 0.f, 0.f};
+                    }
+            wait_unit();
+            u4 kw[2 * TW][2];
+#pragma unroll
+            for (int b = 0; b < 2 * TW; ++b)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // f32: halves of a lane's eight dims; bf16: the eight of two steps
                     const int j = sizeof(T) == 4 ? 2 * g + h : 4 * h + g;
                     const int d = C::kLine * i + j * (16 / (int)sizeof(T));
-                    u4 v = *(const u4 *)(ring + at * 2048 + 32 * (16 * b + col) +
+                    u4 v = *(const u4 *)(ring + at * kWords + 32 * (16 * b + col) +
                                          4 * (j ^ (col & 7)));
                     if (!FULL && d >= p.dim)
                         v = u4{0u, 0u, 0u, 0u};
@@ -370,32 +395,36 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                                     : sources_v(s.slots[buf], x.kh, t0, t1, i + 1 + NB - UK);
             if (!mine)
                 continue;
+            // (bf16: widened once for all rows)
+            float k[SU][2 * TW][8];
+#pragma unroll
+            for (int u = 0; u < SU; ++u)
+#pragma unroll
+                for (int b = 0; b < 2 * TW; ++b)
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) {
+                        if constexpr (sizeof(T) == 4)
+                            k[u][b][jj] = __uint_as_float(kw[b][jj / 4][jj % 4]);
+                        else
+                            k[u][b][jj] = jj % 2 ? bf16_high(kw[b][u][jj / 2])
+                                                 : bf16_low(kw[b][u][jj / 2]);
+                    }
 #pragma unroll
             for (int rg = 0; rg < U; ++rg) {
                 if (rg >= groups)
                     continue;
 #pragma unroll
-                for (int u = 0; u < C::SU; ++u) {
-                    if (C::SU * i + u >= DK / 32)
+                for (int u = 0; u < SU; ++u) {
+                    if (SU * i + u >= DK / 32)
                         continue;
-                    const f4 qa = s.q[rg][C::SU * i + u][0][lane], qb = s.q[rg][C::SU * i + u][1][lane];
 #pragma unroll
                     for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            float k;
-                            if constexpr (sizeof(T) == 4)
-                                k = __uint_as_float(kw[b][jj / 4][jj % 4]);
-                            else
-                                k = jj % 2 ? bf16_high(kw[b][u][jj / 2])
-                                           : bf16_low(kw[b][u][jj / 2]);
-                            acc[rg][b] = mfma(k, jj < 4 ? qa[jj % 4] : qb[jj % 4], acc[rg][b]);
-                        }
+                        for (int b = 0; b < 2 * TW; ++b)
+                            acc[rg][b] = mfma(k[u][b][jj], q[rg][u][jj / 4][jj % 4], acc[rg][b]);
                 }
             }
         }
-        f4 fq[NQ];
-        fetch_q(y, fq);
 
         bool bad = false;
         auto ok_of = [&](int rg, int t, bool ok[2][4]) { // of the wave's tile t
@@ -411,7 +440,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                 if (rg >= groups)
                     continue;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < TW; ++t) {
                     bool ok[2][4];
                     float v[2][4];
                     ok_of(rg, t, ok);
@@ -427,13 +456,14 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                     bad |= bad_scores(v, ok);
                     const float m = tile_max(v, ok);
                     if (g == 0)
-                        s.max[2 * w + t][16 * rg + col] = m;
+                        s.max[TW * w + t][16 * rg + col] = m;
                 }
             }
         }
         if (bad)
             atomicOr(p.err, kErrScore);
         lds_barrier(); // every tile's maximum; the query is used
+        issue_q(y);
 
         if (mine) {
 #pragma unroll
@@ -441,11 +471,11 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                 if (rg >= groups)
                     continue;
                 float before = kNegInf;
-                for (int t = t0; t < 2 * w; ++t)
+                for (int t = t0; t < TW * w; ++t)
                     before = fmaxf(before, s.max[t][16 * rg + col]);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int tile = 2 * w + t;
+                for (int t = 0; t < TW; ++t) {
+                    const int tile = TW * w + t;
                     if (tile < t0 || tile > t1)
                         continue;
                     bool ok[2][4];
@@ -480,8 +510,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
             }
         }
         store(y, f, buf ^ 1);
-        store_q(y, fq);
-        lds_barrier(); // probabilities, row sums and factors; the next query
+        lds_barrier(); // probabilities, row sums and factors
         spare_next = spare_slot(buf ^ 1);
 
         // the l chain and the P.V chains of the wave's dims: D of 16 dims x 16 rows
@@ -516,16 +545,13 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                 for (int h = 0; h < kHeld; ++h)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const char *row = reinterpret_cast<const char *>(ring + at * 2048) +
+                        const char *row = reinterpret_cast<const char *>(ring + at * kWords) +
                                           (16 * (h0 + h) + 4 * r + g) * C::kRowV;
-                        if constexpr (WV >= 4) {
+                        if constexpr (WV == 4) {
+                            const u4 v = *(const u4 *)(row + 16 * col);
 #pragma unroll
-                            for (int k = 0; k < WV / 4; ++k) {
-                                const u4 v = *(const u4 *)(row + 256 * k + 16 * col);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    vw[h][r][4 * k + e] = v[e];
-                            }
+                            for (int e = 0; e < 4; ++e)
+                                vw[h][r][e] = v[e];
                         } else if constexpr (WV == 2) {
                             const u2 v = *(const u2 *)(row + 8 * col);
                             vw[h][r][0] = v.x;
@@ -573,13 +599,11 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
             }
         }
 
-        // D's dim 4 g + e of block j: the dim that lane 4 g + e of the operand had
-        auto dim_of = [&](int j, int e) {
-            const int lane16 = 4 * g + e;
-            if (VL == 8 && sizeof(T) == 4)
-                return 16 * VL * w + 64 * (j / 4) + 4 * lane16 + j % 4;
-            return 16 * VL * w + VL * lane16 + j;
-        };
+        // (the next query's copies are older than its first units')
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::NE * NB));
+        // D's row 4 g + e of block j is the dim that lane 4 g + e of the operand had:
+        // a lane has 4 VL dims in a row
+        const int d0 = 16 * VL * w + 4 * VL * g;
         bool nonfinite = false;
         if (!x.empty) {
 #pragma unroll
@@ -587,7 +611,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                 const int r = 16 * rg + col;
                 if (r >= x.nrows)
                     continue;
-                const int f0 = x.first_row + r, token = f0 / p.group;
+                const int f0 = x.first_row + r, token = (int)divided(f0, p.by_group);
                 const int head = x.kh * p.group + f0 - token * p.group;
                 const int64_t part = ((int64_t)(x.row + token) * p.row_chunks + x.ci) * p.qheads + head;
                 const bool some = l[rg] != 0.f; // a key that the row attends
@@ -595,38 +619,18 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
                                     : p.ws_o + part * p.dim;
                 if (x.only && !some)
                     continue;
-                auto value = [&](int j, int e) {
-                    const float v = x.only ? O[rg][j][e] / l[rg] : some ? O[rg][j][e] : 0.f;
-                    return v;
-                };
-                if constexpr (VL >= 4) {
 #pragma unroll
-                    for (int j = 0; j < VL; j += 4)
+                for (int k = 0; k < VL; ++k) {
+                    if (!FULL && d0 + 4 * k >= p.dim)
+                        continue;
+                    f4 v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int d = dim_of(j, e);
-                            if (!FULL && d >= p.dim)
-                                continue;
-                            f4 v;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                v[k] = value(j + k, e);
-                                nonfinite |= x.only && !is_finite(v[k]);
-                            }
-                            stg4(dst + d, v);
-                        }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VL; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int d = dim_of(j, e);
-                            if (!FULL && d >= p.dim)
-                                continue;
-                            const float v = value(j, e);
-                            nonfinite |= x.only && !is_finite(v);
-                            stg(dst + d, v);
-                        }
+                    for (int a = 0; a < 4; ++a) {
+                        const float o = O[rg][(4 * k + a) % VL][(4 * k + a) / VL];
+                        v[a] = x.only ? o / l[rg] : some ? o : 0.f;
+                        nonfinite |= x.only && !is_finite(v[a]);
+                    }
+                    stg4(dst + d0 + 4 * k, v);
                 }
                 if (!x.only && w == 0 && g == 0) {
                     stg(p.ws_ml + 2 * part, last[rg]);
@@ -638,6 +642,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), (U == 1 ? 2 : 1)) vo
             atomicOr(p.err, kErrOutput);
         if (!more)
             break;
+        lds_barrier(); // the next query
         item = next;
         x = y;
         spare = spare_next;
@@ -678,7 +683,7 @@ static hipError_t resident_rows(int requests, int *groups)
             return e;
     }
     const int most = requests <= kFewRequests ? kFewRequests : requests;
-    e = hipOccupancyMaxActiveBlocksPerMultiprocessor(groups, kernel, 256, bytes(most));
+    e = hipOccupancyMaxActiveBlocksPerMultiprocessor(groups, kernel, RowsCfg<DK, T, U>::kThreads, bytes(most));
     if (e != hipSuccess)
         return e;
     *groups = std::max(*groups, 1);
@@ -698,7 +703,7 @@ static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks,
     const int64_t grid = std::min<int64_t>(chunks * p.kvheads * units,
                                            (int64_t)groups * std::max(device_cus(), 1));
     paged_rows_kernel<DK, T, FULL, U, NB>
-        <<<(unsigned)grid, 256, rows_lds_bytes<DK, U, NB>(p.requests), stream>>>(p);
+        <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, U, NB>(p.requests), stream>>>(p);
     return hipGetLastError();
 }
 

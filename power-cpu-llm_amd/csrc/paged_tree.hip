@@ -185,6 +185,9 @@ int pcl_paged_tree_attention(pcl_context *ctx, const pcl_paged_tree_desc *desc)
     p.mask_words = (int)d.mask_words;
     p.max_new = (int)std::min(d.max_new, d.max_length);
     p.row_chunks = (int)each;
+    p.by_group = pcl::divisor((uint32_t)p.group);
+    p.by_kvheads = pcl::divisor((uint32_t)p.kvheads);
+    p.by_page_tokens = pcl::divisor(p.page_tokens);
     const int64_t chunks = d.requests * each;
     const bool bf16 = s.type == PCL_CACHE_BF16;
     int span = pcl::open_timed_span(ctx, 0);
