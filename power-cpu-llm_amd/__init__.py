@@ -620,22 +620,22 @@ class Context:
     def page_accept(self, batch, paths_ptr, counts_ptr, depth, from_ptr, to_ptr):
         """Which rows the verified branches move (slots, [requests][depth])."""
         self._check(self.lib.pcl_page_accept(
-            self.handle, ctypes.byref(batch), ctypes.c_void_p(paths_ptr),
-            ctypes.c_void_p(counts_ptr), int(depth), ctypes.c_void_p(from_ptr),
-            ctypes.c_void_p(to_ptr)))
+            self.handle, ctypes.byref(batch), paths_ptr,
+            counts_ptr, int(depth), from_ptr,
+            to_ptr))
 
     def page_fork(self, batch, sources_ptr, from_ptr, to_ptr, rows_ptr):
         """Opens a fork: request b begins as a copy of sources[b] (negative: not);
         the rows to copy go to from / to / rows ([requests])."""
         self._check(self.lib.pcl_page_fork(
-            self.handle, ctypes.byref(batch), ctypes.c_void_p(sources_ptr),
-            ctypes.c_void_p(from_ptr), ctypes.c_void_p(to_ptr), ctypes.c_void_p(rows_ptr)))
+            self.handle, ctypes.byref(batch), sources_ptr,
+            from_ptr, to_ptr, rows_ptr))
 
     def page_release_shared(self, batch, finished_ptr):
         """Requests with a nonzero flag give back the pages that nobody else
         holds."""
         self._check(self.lib.pcl_page_release_shared(self.handle, ctypes.byref(batch),
-                                                     ctypes.c_void_p(finished_ptr)))
+                                                     finished_ptr))
 
     def page_release_workspace_bytes(self, batch):
         return self.lib.pcl_page_release_workspace_bytes(ctypes.byref(batch))
@@ -645,8 +645,8 @@ class Context:
         PclPagePools): lists of entries in order, or, with rows, runs."""
         array = (PclPagePools * len(pools))(*pools)
         self._check(self.lib.pcl_paged_copy(
-            self.handle, array, len(pools), ctypes.c_void_p(from_ptr), ctypes.c_void_p(to_ptr),
-            ctypes.c_void_p(rows_ptr), int(lists), int(entries)))
+            self.handle, array, len(pools), from_ptr, to_ptr,
+            rows_ptr, int(lists), int(entries)))
 
     @staticmethod
     def paged_tree_desc(**kw):

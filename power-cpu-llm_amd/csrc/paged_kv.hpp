@@ -1119,9 +1119,14 @@ static hipError_t launch_paged(P p, int64_t rows, int64_t chunks, hipStream_t st
 template <int DK, typename T, bool FULL, typename P>
 static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    if (rows <= 4)
+    // (a tree launch of few items splits its rows over more workgroups)
+    auto few = [&](int64_t unit) {
+        return std::is_same_v<P, TreeParams> && FULL &&
+               chunks * p.kvheads * ((rows + unit - 1) / unit) <= device_cus();
+    };
+    if (rows <= 4 || few(4))
         return launch_paged<DK, T, FULL, 1>(p, rows, chunks, stream);
-    if (rows <= 8)
+    if (rows <= 8 || few(8))
         return launch_paged<DK, T, FULL, 2>(p, rows, chunks, stream);
     if constexpr (std::is_same_v<P, TreeParams>)
         return launch_paged_rows<DK>(p, std::is_same_v<T, __bf16>, rows, chunks, stream);

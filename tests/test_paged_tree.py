@@ -182,10 +182,13 @@ def test_page_calls_refuse_missing_words(pcl, no_context):
     assert lib.pcl_page_fork(None, b, w, w, w, w) == 1
     assert lib.pcl_page_release_shared(None, b, w) == 1
     assert lib.pcl_page_release_workspace_bytes(None) == 0
-    # two bits a page
-    few, many = (lib.pcl_page_release_workspace_bytes(ctypes.byref(batch_of(pcl, pages=n)))
-                 for n in (64, 64 + 32 * 512))
-    assert many - few == 2 * 4 * 512
+    # two bytes a page in whole 32, none for a small batch
+    def nbytes(**kw):
+        return lib.pcl_page_release_workspace_bytes(ctypes.byref(batch_of(pcl, **kw)))
+    base = nbytes()
+    assert nbytes(table_stride=1 << 13) == nbytes(pages=1 << 17) == base
+    assert nbytes(table_stride=1 + (1 << 13), pages=65) - base == 2 * 96 + 16
+    assert nbytes(pages=1 + (1 << 17)) - base == 2 * (32 + (1 << 17)) + 16
 
 
 def test_copy_refuses_bad_lists(pcl, no_context):
@@ -483,7 +486,10 @@ def release_call(ctx, batch, finished):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(3, 9, 7, 20, 130), (5, 40, 1, 90, 64), (37, 6, 16, 120, 700),
-                                   (300, 3, 8, 500, 900), (2048, 2, 4, 2600, 2500)],
+                                   (300, 3, 8, 500, 900), (2048, 2, 4, 2600, 2500),
+                                   # more table entries, and pages, than one workgroup takes
+                                   (2048, 9, 4, 2600, 2500), (40, 450, 1, 3001, 900),
+                                   (6, 8, 16, 131073 + 40, 300)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_shared_bookkeeping_follows_the_model(pcl, torch, ctx, shape):
     rng = np.random.default_rng(sum(shape))
