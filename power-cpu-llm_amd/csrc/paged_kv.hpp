@@ -714,10 +714,15 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
     for (uint32_t item = blockIdx.x;; buf ^= 1) {
         const uint32_t next = item + gridDim.x;
         const bool more = next < items;
-        // (without a next item this one is requested again, and not used)
-        const Item y = find_item(p, req, more ? next : item, C::kRowsUnit);
+        // (without a next item this one is requested again, and not used; a tree
+        // launch, whose items take more to find, does without)
+        Item y = x;
         Fetched f;
-        fetch(y, f);
+        if (!TREE || more) {
+            y = find_item(p, req, more ? next : item, C::kRowsUnit);
+            fetch(y, f);
+        }
+        const int behind = TREE && !more ? buf : buf ^ 1; // its slots
         const int nrows = rows_of(x);
         if constexpr (TREE) {
 #pragma unroll
@@ -858,9 +863,10 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
                     s.last[r] = m;
             }
         }
-        store(y, f, buf ^ 1);
+        if (!TREE || more)
+            store(y, f, buf ^ 1);
         lds_barrier(); // probabilities, row sums and factors; the next query
-        spare_next = spare_slot(buf ^ 1);
+        spare_next = spare_slot(behind);
 
         // the l chain and the P.V chains of the lane's VL output dims
         f4 l[R], O[R][VL];
@@ -903,7 +909,7 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
         auto behind_v = [&](int i) {
             const int n = i + NB - rounds; // the next item's first units follow this one's
             return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
-                         : line_k(rows_k(s.slots[buf ^ 1], spare_next, y.kh, n / KP), n % KP);
+                         : line_k(rows_k(s.slots[behind], spare_next, y.kh, n / KP), n % KP);
         };
         c = behind_v(0);
         for (int i = 0; i < rounds; ++i) {

@@ -338,10 +338,14 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
     for (uint32_t item = blockIdx.x;; buf ^= 1) {
         const uint32_t next = item + gridDim.x;
         const bool more = next < items;
-        // (without a next item this one is requested again, and not used)
-        const TreeItem y = find_item(p, req, more ? next : item, C::kRowsUnit);
+        // (without a next item this one's first units are copied again, and not used)
+        TreeItem y = x;
         Fetched f;
-        fetch(y, f);
+        if (more) {
+            y = find_item(p, req, next, C::kRowsUnit);
+            fetch(y, f);
+        }
+        const int behind = more ? buf ^ 1 : buf; // the next item's slots
 #pragma unroll
         for (int rg = 0; rg < U; ++rg)
             see[rg] = see_next[rg];
@@ -463,7 +467,8 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         if (bad)
             atomicOr(p.err, kErrScore);
         lds_barrier(); // every tile's maximum; the query is used
-        issue_q(y);
+        if (more)
+            issue_q(y);
 
         if (mine) {
 #pragma unroll
@@ -509,9 +514,10 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
                     last[rg] = fmaxf(last[rg], s.max[t][16 * rg + col]);
             }
         }
-        store(y, f, buf ^ 1);
+        if (more)
+            store(y, f, buf ^ 1);
         lds_barrier(); // probabilities, row sums and factors
-        spare_next = spare_slot(buf ^ 1);
+        spare_next = spare_slot(behind);
 
         // the l chain and the P.V chains of the wave's dims: D of 16 dims x 16 rows
         float l[U];
@@ -528,7 +534,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         auto behind_v = [&](int i) {
             const int n = i + NB - rounds; // the next item's first units follow this one's
             return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
-                         : line_k(rows_k(s.slots[buf ^ 1], spare_next, y.kh), n);
+                         : line_k(rows_k(s.slots[behind], spare_next, y.kh), n);
         };
         c = behind_v(0);
 #pragma unroll 1
