@@ -18,10 +18,13 @@ struct CombineShape {
     int lanes, spans, heads; // powers of two; heads: query heads of a workgroup
 };
 
-// A row's partials: chunk c's of [c0, c1) is base + c - c0.
+// A row's partials: chunk c's of [c0, c1) is base + c - first. Where the chunks come
+// in runs, those of the run that begins a span are merged already, into the place of
+// its last one; first and end bound the request's chunks.
 struct RowParts {
     uint32_t base;
     int c0, c1;
+    int first, end, run;
 };
 
 // Merges them for the workgroup's heads and dims and calls write(head, dim, the
@@ -45,14 +48,22 @@ __device__ __forceinline__ void combine_row(const PagedParams &p, const CombineS
     for (int r0 = s0; r0 < s1; r0 += c.spans) {
         Merged4 s = {kNegInf, 0.f, f4{0.f, 0.f, 0.f, 0.f}};
         if (r0 + gi < s1) {
-            const int e = min((r0 + gi + 1) * kSpanChunks, c1);
-            for (int a = max((r0 + gi) * kSpanChunks, c0); a < e; a += BATCH) {
+            int e = min((r0 + gi + 1) * kSpanChunks, c1);
+            int a = max((r0 + gi) * kSpanChunks, c0);
+            if (r.run > 1) {
+                const int merged = run_end(max((r0 + gi) * kSpanChunks, r.first), r.end, r.run);
+                if (a < merged) {
+                    a = merged - 1;
+                    e = max(e, merged);
+                }
+            }
+            for (; a < e; a += BATCH) {
                 f2 ml[BATCH];
                 f4 ov[BATCH];
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
                     const int64_t part =
-                        (int64_t)(r.base + (uint32_t)(min(a + i, e - 1) - c0)) * p.qheads + row;
+                        (int64_t)(r.base + (uint32_t)(min(a + i, e - 1) - r.first)) * p.qheads + row;
                     ml[i] = ldg2(p.ws_ml + 2 * part);
                     ov[i] = ldg4(p.ws_o + part * p.dim + at);
                 }

@@ -1035,7 +1035,8 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
 }
 
 template <int DK, typename T, bool FULL, int R, int NB>
-__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads)) void paged_tree_kernel(TreeParams p)
+__global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
+                             (FULL && R == 1 && NB == 1 ? 3 : 1)) void paged_tree_kernel(TreeParams p)
 {
     paged_kv_body<DK, T, FULL, R, NB, true>(p);
 }
@@ -1126,13 +1127,10 @@ template <int DK, typename T, bool FULL, typename P>
 static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
     // (a tree launch of few items splits its rows over more workgroups)
-    auto few = [&](int64_t unit) {
-        return std::is_same_v<P, TreeParams> && FULL &&
-               chunks * p.kvheads * ((rows + unit - 1) / unit) <= device_cus();
-    };
-    if (rows <= 4 || few(4))
+    constexpr bool TREE = std::is_same_v<P, TreeParams>;
+    if (rows <= 4 || (TREE && few_items(FULL, chunks * p.kvheads, rows, 4)))
         return launch_paged<DK, T, FULL, 1>(p, rows, chunks, stream);
-    if (rows <= 8 || few(8))
+    if (rows <= 8 || (TREE && few_items(FULL, chunks * p.kvheads, rows, 8)))
         return launch_paged<DK, T, FULL, 2>(p, rows, chunks, stream);
     if constexpr (std::is_same_v<P, TreeParams>)
         return launch_paged_rows<DK>(p, std::is_same_v<T, __bf16>, rows, chunks, stream);

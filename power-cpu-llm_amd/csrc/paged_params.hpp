@@ -81,6 +81,35 @@ __device__ __forceinline__ uint32_t divided(uint32_t x, const Divisor &d)
     return d.mul ? __umulhi(x, d.mul) >> d.shift : x;
 }
 
+// An item of a launch of many rows: a run of chunks of one request, KV head and unit
+// of query rows, all in one span and one aligned group of `run` chunks.
+struct PlanItem {
+    int b, kh;
+    int row, held, n;     // as TreeItem's
+    int first_row, nrows; // of the unit
+    int from, to;         // the first and the last key that any row may attend
+    int chunk, chunks;    // first one, and how many (0: no key, nothing to do)
+    int slot;             // partial (of a row's) of the first chunk, or of the merged run
+    int merged;           // the run begins its span: its chunks are merged as they come
+    int only;             // and is all of the request
+    int spare[2];
+};
+
+struct PlanHead {
+    int items, run;
+    int taken[8]; // items that each XCD's workgroups have taken, of its own
+    int spare[6];
+};
+
+static_assert(sizeof(PlanItem) == 64 && sizeof(PlanHead) == 64, "whole scalar loads");
+
+// The run that begins a span at `first` (the request's first chunk in it) ends before
+// this chunk; `end`: behind the request's last.
+__device__ __forceinline__ int run_end(int first, int end, int run)
+{
+    return min((first / run + 1) * run, end);
+}
+
 // Of a launch over every new token of a step (lengths: with the step's tokens).
 struct TreeParams : PagedParams {
     const int32_t *held, *newest;  // [requests] tokens before the step, row of the last one
@@ -88,6 +117,10 @@ struct TreeParams : PagedParams {
     const int32_t *positions;      // [q_rows], with masks and a window
     int mask_words, max_new;
     int row_chunks; // partials of a row: chunks that one request may have
+    // of a launch of many rows, written by its plan kernel: the items' count and the
+    // chunks of a run, then the items (null: every chunk is an item)
+    PlanHead *plan;
+    int max_items;
     Divisor by_group, by_kvheads, by_page_tokens;
 };
 
@@ -133,6 +166,12 @@ template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream);
 template <int DK>
 hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream);
+// Whether units of `unit` rows leave a tree launch at most an item per CU, each with a
+// CU to itself; `whole`: the head dim is one that needs no padding. `items`: at one
+// unit, `rows`: of a KV head that one request has at most.
+bool few_items(bool whole, int64_t items, int64_t rows, int64_t unit);
+// Whether such a launch takes the kernels of many rows (paged_rows.hpp).
+bool many_rows(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows);
 // `rows`: query rows of a KV head that one request has at most, above eight.
 template <int DK>
 hipError_t launch_paged_rows(const TreeParams &p, bool bf16, int64_t rows, int64_t chunks,

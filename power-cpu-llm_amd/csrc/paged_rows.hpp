@@ -39,9 +39,11 @@ template <int DK, typename T, int U> struct RowsCfg {
 template <int DK, int U> struct RowsLds {
     f4 q[U][DK / 32][2][64];              // [rows][32 dims][half of a lane's eight][lane]
     f4 p[U][kTilesPerChunk][2][64];       // [rows][tile][16 keys][lane]
-    float max[kTilesPerChunk][16 * U], alpha[kTilesPerChunk][16 * U], sum[kTilesPerChunk][16 * U];
-    int32_t slots[2][kChunk];             // of this item and the next
-    int32_t attended[2][8];               // each wave's first attended key
+    float max[16 * U][kTilesPerChunk];    // -inf outside the attended tiles
+    f2 factors[kTilesPerChunk][16 * U];   // alpha and the row sum
+    int32_t slots[2][kChunk];             // of this chunk and the next
+    int32_t live[2][kTilesPerChunk];      // tiles with a key that any row attends
+    uint32_t taken;                       // the item behind the next one
 };
 
 // The rings of all waves.
@@ -124,9 +126,7 @@ __device__ __forceinline__ void attended_keys(const TreeParams &p, const TreeIte
         see[rg] = 0;
         if (16 * rg >= x.nrows)
             continue;
-        if (16 * rg + (int)(threadIdx.x & 15) >= x.nrows)
-            continue;
-        const int token = row_token(p, x, rg);
+        const int token = row_token(p, x, rg); // (past the rows the last one's again)
         if (!p.masks) {
             const int to = x.held + token, from = first_tree_key(p, to);
             see[rg] = in & bit_range(from - x.cbase - k0, to - x.cbase - k0);
@@ -162,8 +162,149 @@ __device__ __forceinline__ uint32_t or_rows(uint32_t x)
     return x;
 }
 
+// The items of a launch, by all its threads: chunks in runs of as many as leave each
+// workgroup kRounds items or more, up to a span. Of a run that begins its span the
+// chunks are merged in registers, in their order; others write a partial each, but
+// share the query and the search for them.
+constexpr int kRounds = 24;
+constexpr int kPlanThreads = 256;
+
+template <int UNIT>
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(TreeParams p, int workgroups)
+{
+    extern __shared__ uint32_t dyn[];
+    __shared__ uint64_t waves[kPlanThreads / 64];
+    const TreeWords r = tree_words(dyn, p.requests);
+    const int tid = threadIdx.x;
+    const int per = (p.requests + kPlanThreads - 1) / kPlanThreads;
+    const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
+    auto units_of = [&](int n) { return ((uint32_t)n * (uint32_t)p.group + UNIT - 1) / UNIT; };
+    uint64_t sum = 0; // (requests that share rows may add up past 2^32)
+    bool bad = false;
+    for (int i = i0; i < i1; ++i) {
+        const TreeKeys k = tree_keys(p, i, &bad);
+        r.len[i] = k.len;
+        r.held[i] = k.held;
+        r.row[i] = k.row;
+        sum += (uint64_t)tree_chunks(p, k) * units_of(k.len - k.held);
+    }
+    uint64_t total;
+    block_offsets(sum, waves, &total);
+    int run = kSpanChunks;
+    while (run > 1 && total * p.kvheads < (uint64_t)run * kRounds * workgroups)
+        run /= 2;
+    // groups of `run` chunks that a request's lie in, over the units
+    sum = 0;
+    for (int i = i0; i < i1; ++i) {
+        const TreeKeys k = {r.row[i], r.held[i], r.len[i]};
+        const int chunks = tree_chunks(p, k), first = first_tree_key(p, k.held) / kChunk;
+        const uint32_t runs = chunks ? (first + chunks - 1) / run - first / run + 1 : 0;
+        r.off[i] = runs * units_of(k.len - k.held);
+        sum += r.off[i];
+        if (blockIdx.x == 0)
+            p.ws_req[i] = int4{k.row, chunks, k.held, k.len - k.held};
+    }
+    uint64_t at = block_offsets(sum, waves, &total);
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t items = r.off[i];
+        r.off[i] = (uint32_t)at;
+        at += items;
+    }
+    const bool fits = total * p.kvheads <= (uint64_t)p.max_items;
+    bad |= !fits;
+    const uint32_t items = fits ? (uint32_t)total : 0;
+    if (tid == 0) {
+        r.off[p.requests] = items;
+        if (blockIdx.x == 0) {
+            p.plan->items = (int)(items * (uint32_t)p.kvheads);
+            p.plan->run = run;
+            // (the first one of a workgroup is its own)
+            for (int i = 0; i < 8; ++i)
+                p.plan->taken[i] = workgroups % 8 ? workgroups : workgroups / 8;
+        }
+    }
+    if (bad && blockIdx.x == 0)
+        atomicOr(p.err, kErrPages);
+    __syncthreads();
+    PlanItem *out = reinterpret_cast<PlanItem *>(p.plan + 1);
+    const uint32_t all = items * (uint32_t)p.kvheads;
+    for (uint32_t n = blockIdx.x * kPlanThreads + tid; n < all; n += gridDim.x * kPlanThreads) {
+        // units of a run and KV head side by side: they share its keys
+        PlanItem x;
+        x.b = 0;
+        for (int lo = 0, hi = p.requests; hi - lo > 1;) {
+            const int mid = (lo + hi) / 2;
+            if (r.off[mid] * (uint64_t)p.kvheads <= n)
+                lo = mid;
+            else
+                hi = mid;
+            x.b = lo;
+        }
+        const TreeKeys k = {r.row[x.b], r.held[x.b], r.len[x.b]};
+        x.row = k.row;
+        x.held = k.held;
+        x.n = k.len - k.held;
+        const uint32_t rest = n - r.off[x.b] * (uint32_t)p.kvheads, units = units_of(x.n);
+        const int unit = (int)(rest % units);
+        x.kh = (int)(rest / units % (uint32_t)p.kvheads);
+        const int group = (int)(rest / units / (uint32_t)p.kvheads); // of chunks
+        x.first_row = unit * UNIT;
+        x.nrows = min(x.n * p.group - x.first_row, UNIT);
+        x.from = first_tree_key(p, k.held);
+        const int first = x.from / kChunk, end = (k.len - 1) / kChunk + 1;
+        x.to = k.len - 1;
+        if (!p.masks) {
+            x.from = first_tree_key(p, k.held + x.first_row / p.group);
+            x.to = k.held + (x.first_row + x.nrows - 1) / p.group;
+        }
+        const int g0 = (first / run + group) * run; // the group's chunks
+        const int c0 = max(g0, x.from / kChunk), c1 = min(g0 + run, x.to / kChunk + 1);
+        x.chunk = c0;
+        x.chunks = max(c1 - c0, 0);
+        const int span = max(g0 / kSpanChunks * kSpanChunks, first); // its first chunk
+        x.merged = span / run == g0 / run;
+        x.slot = (x.merged ? run_end(span, end, run) - 1 : c0) - first;
+        x.only = (end - 1) / run == first / run;
+        x.spare[0] = x.spare[1] = 0;
+        out[n] = x;
+    }
+}
+
+// Words of the plan, by scalar loads (the same for the whole wave).
+typedef int32_t int16w __attribute__((ext_vector_type(16)));
+typedef const __attribute__((address_space(4))) int16w *plan_ptr;
+
+__device__ __forceinline__ PlanItem plan_item(plan_ptr at)
+{
+    const int16w w = *at;
+    return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], w[11], w[12], w[13],
+            {0, 0}};
+}
+
+// Chunk k of an item.
+__device__ __forceinline__ TreeItem chunk_item(const PlanItem &i, int k)
+{
+    TreeItem x;
+    x.b = i.b;
+    x.kh = i.kh;
+    x.held = i.held;
+    x.n = i.n;
+    x.row = i.row;
+    x.first_row = i.first_row;
+    x.nrows = i.nrows;
+    x.unit = 0;
+    x.ci = (uint32_t)(i.merged ? i.slot : i.slot + k);
+    x.only = i.only;
+    x.empty = false;
+    x.cbase = (i.chunk + k) * kChunk;
+    x.lo = max(i.from - x.cbase, 0);
+    x.hi = min(i.to - x.cbase, kChunk - 1);
+    return x;
+}
+
 template <int DK, typename T, bool FULL, int U, int NB>
-__global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_kernel(TreeParams p)
+__global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
+                             (DK == 256 && U == 1 ? 4 : 2)) void paged_rows_kernel(TreeParams p)
 {
     using C = RowsCfg<DK, T, U>;
     constexpr int NW = C::NW, KW = C::KW, TW = C::TW, UK = C::UK, VL = C::VL, SU = C::SU;
@@ -172,23 +313,52 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
     using Lds = RowsLds<DK, U>;
     Lds &s = *reinterpret_cast<Lds *>(dyn);
     uint32_t *const rings = dyn + sizeof(Lds) / 4;
-    __shared__ uint64_t waves[NW];
-    const TreeWords req = tree_words(rings + rows_ring_bytes(NB) / 4, p.requests);
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int k0 = KW * w; // the wave's keys
 
-    fill_request_words(p, req, waves, C::kRowsUnit);
-    if (blockIdx.x == 0)
-        for (int i = tid; i < p.requests; i += C::kThreads) {
-            const TreeKeys k = {req.row[i], req.held[i], req.len[i]};
-            p.ws_req[i] = int4{k.row, tree_chunks(p, k), k.held, k.len - k.held};
+    // Workgroups take items as they come to them: chunks differ in their keys, and so
+    // do the runs. Of each round of the grid's items an XCD (they have the workgroups
+    // in turn) has those side by side, whose units share its L2, and its workgroups
+    // take them from a counter of its own. One is taken while the one before the last
+    // runs, so that nobody waits for the counter.
+    const plan_ptr plan = (plan_ptr)p.plan;
+    const uint32_t items = (uint32_t)(*plan)[0];
+    const uint32_t parts = gridDim.x % 8 ? 1 : 8, each = gridDim.x / parts;
+    const uint32_t part = blockIdx.x % parts;
+    auto place = [&](uint32_t n) { return n / each * gridDim.x + part * each + n % each; };
+    auto take = [&]() { return place((uint32_t)atomicAdd(&p.plan->taken[part], 1)); };
+    // (an item past the last has no chunks, and is not skipped)
+    auto load_item = [&](uint32_t n) {
+        PlanItem i;
+        i.chunks = -1;
+        if (n < items)
+            i = plan_item(plan + 1 + n);
+        return i;
+    };
+    auto taken_item = [&]() { // by the whole workgroup, behind a barrier
+        PlanItem i = load_item(__builtin_amdgcn_readfirstlane(s.taken));
+        while (i.chunks == 0) { // (a chain's early units have none of the last keys)
+            __syncthreads();
+            if (tid == 0)
+                s.taken = take();
+            __syncthreads();
+            i = load_item(__builtin_amdgcn_readfirstlane(s.taken));
         }
-    const uint32_t items =
-        __builtin_amdgcn_readfirstlane(req.off[p.requests]) * (uint32_t)p.kvheads;
-    if (blockIdx.x >= items)
+        return i;
+    };
+    if (tid == 0)
+        s.taken = place(blockIdx.x / parts);
+    __syncthreads();
+    PlanItem now = taken_item();
+    if (now.chunks < 0)
         return;
+    __syncthreads();
+    if (tid == 0)
+        s.taken = take();
+    PlanItem next; // (taken below)
+    int chunk = 0; // of `now`
 
     struct Fetched {
         int page;
@@ -201,8 +371,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         f.page = p.table[x.b * p.table_stride + divided(position(x), p.by_page_tokens)];
         fetch_rows(p, x, k0, f.tree);
     };
-    // The unit's query rows into LDS (as they are: they are scaled where they are
-    // read): a copy is four of the eight dims of a lane, for 16 rows and 32 dims. Rows
+    // The unit's query rows into LDS: a copy is four of the eight dims of a lane, for 16 rows and 32 dims. Rows
     // past the last are the last one's, dims past the head dim the first ones.
     auto issue_q = [&](const TreeItem &x) {
         const float *row[U];
@@ -225,7 +394,23 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
                     (lds_ptr)(&s.q[rg][u][hh][0]), 16, 0, 0);
             }
     };
+    // Scales the wave's copies where they lie, once they are there.
+    auto scale_q = [&]() {
+        constexpr int kPart = DK / 16 / NW;
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg)
+#pragma unroll
+            for (int i = 0; i < kPart; ++i) {
+                const int n = w * kPart + i, u = n / 2, hh = n % 2;
+                const f4 v = s.q[rg][u][hh][lane] * p.q_scale;
+                s.q[rg][u][hh][lane] =
+                    FULL || 32 * u + 8 * g + 4 * hh < p.dim ? v : f4{0.f, 0.f, 0.f, 0.f};
+            }
+    };
     uint64_t see[U], see_next[U]; // the wave's keys that the lane's rows attend
+    // A chunk's slots and live tiles. A key that no row attends takes the slot of one of
+    // the wave's that some row does, so that no value is multiplied that the rows' own
+    // results do not hold; tiles without one are copied, but not multiplied.
     auto store = [&](const TreeItem &x, const Fetched &f, int to) {
         int page = f.page;
         if (page < 0 || page >= p.pages) {
@@ -241,12 +426,13 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         for (int rg = 0; rg < U; ++rg)
             any |= see_next[rg];
         any = (uint64_t)or_rows((uint32_t)(any >> 32)) << 32 | or_rows((uint32_t)any);
+        const int spare = __builtin_amdgcn_readlane(slot, any ? __builtin_ctzll(any) & (KW - 1) : 0);
         if (!(any >> lane & 1))
-            slot = -1;
+            slot = spare;
         if (lane < KW)
             s.slots[to][k0 + lane] = slot;
-        if (lane == 0)
-            s.attended[to][w] = any ? k0 + __builtin_ctzll(any) : kChunk;
+        if (lane < TW)
+            s.live[to][TW * w + lane] = (uint32_t)(any >> (kTile * lane)) != 0;
     };
     // (paged_kv.hpp has the ring and its units)
     constexpr int kWords = C::kUnit / 4;
@@ -256,27 +442,15 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
     struct Sources {
         const char *from[C::NE];
     };
-    int spare = 0, spare_next = 0;
-    auto spare_slot = [&](int to) {
-        int first = kChunk;
-#pragma unroll
-        for (int i = 0; i < NW; ++i)
-            first = min(first, s.attended[to][i]);
-        return first == kChunk ? 0 : s.slots[to][first];
-    };
-    auto slot_at = [&](const int32_t *slots, int key, int other) {
-        const int32_t slot = slots[key];
-        return (uint32_t)(slot < 0 ? other : slot);
-    };
     const int piece = (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
-    auto rows_k = [&](const int32_t *slots, int other, int kh) {
+    auto rows_k = [&](const int32_t *slots, int kh) {
         const char *base =
             static_cast<const char *>(p.k) + ((int64_t)kh * p.dim + piece) * sizeof(T);
         const int32_t *mine = slots + k0 + lane / 8;
         Sources c;
 #pragma unroll
         for (int e = 0; e < C::NE; ++e)
-            c.from[e] = base + (uint64_t)slot_at(mine, 8 * e, other) * row_bytes;
+            c.from[e] = base + (uint64_t)(uint32_t)mine[8 * e] * row_bytes;
         return c;
     };
     auto line_k = [&](const Sources &rows, int line) {
@@ -297,7 +471,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         for (int e = 0; e < C::NE; ++e) {
             const int n = C::kKeysV * i + (e * 64 + lane) / C::kLanesV; // chain step from tile t0 on
             const int t = min(t0 + n / kTile, t1), k = n % kTile;
-            c.from[e] = base + (uint64_t)slot_at(slots, kTile * t + chain_key(k), spare) * row_bytes;
+            c.from[e] = base + (uint64_t)(uint32_t)slots[kTile * t + chain_key(k)] * row_bytes;
         }
         return c;
     };
@@ -315,7 +489,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
     auto free_unit = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
     auto next_buffer = [&]() { at = at + 1 == NB ? 0 : at + 1; };
 
-    TreeItem x = find_item(p, req, blockIdx.x, C::kRowsUnit);
+    TreeItem x = chunk_item(now, 0);
     {
         Fetched f;
         issue_q(x);
@@ -323,10 +497,11 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         store(x, f, 0);
     }
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // the query's copies
+    scale_q();
     __syncthreads();
-    spare = spare_slot(0);
+    next = taken_item();
     {
-        const Sources rows = rows_k(s.slots[0], spare, x.kh);
+        const Sources rows = rows_k(s.slots[0], x.kh);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             issue(line_k(rows, i));
@@ -334,18 +509,24 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         }
     }
 
-    int buf = 0;
-    for (uint32_t item = blockIdx.x;; buf ^= 1) {
-        const uint32_t next = item + gridDim.x;
-        const bool more = next < items;
-        // (without a next item this one's first units are copied again, and not used)
+    // the run's chunks merged so far
+    float M1[U], L1[U];
+    f4 merged[U][VL];
+    for (int buf = 0;; buf ^= 1) {
+        const bool last_chunk = chunk + 1 == now.chunks;
+        const bool more = !last_chunk || next.chunks > 0;
+        const bool new_q = last_chunk && more;
+        uint32_t behind_next = 0; // (its atomic returns during the products)
+        if (new_q && tid == 0)
+            behind_next = take();
+        // (without a next chunk this one's first units are copied again, and not used)
         TreeItem y = x;
         Fetched f;
         if (more) {
-            y = find_item(p, req, next, C::kRowsUnit);
+            y = last_chunk ? chunk_item(next, 0) : chunk_item(now, chunk + 1);
             fetch(y, f);
         }
-        const int behind = more ? buf ^ 1 : buf; // the next item's slots
+        const int behind = more ? buf ^ 1 : buf; // the next chunk's slots
 #pragma unroll
         for (int rg = 0; rg < U; ++rg)
             see[rg] = see_next[rg];
@@ -360,7 +541,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
 #pragma unroll
             for (int b = 0; b < 2 * TW; ++b)
                 acc[rg][b] = f4{0.f, 0.f, 0.f, 0.f};
-        const Sources rows = rows_k(s.slots[buf], spare, x.kh);
+        const Sources rows = rows_k(s.slots[buf], x.kh);
         Sources c = NB < UK ? line_k(rows, NB) : sources_v(s.slots[buf], x.kh, t0, t1, NB - UK);
 #pragma unroll 1
         for (int i = 0; i < UK; ++i) {
@@ -372,9 +553,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         const int n = min(SU * i + u, DK / 32 - 1);
-                        q[rg][u][hh] = s.q[rg][n][hh][lane] * p.q_scale;
-                        if (!FULL && 32 * n + 8 * g + 4 * hh >= p.dim)
-                            q[rg][u][hh] = f4{0.f, 0.f, 0.f, 0.f};
+                        q[rg][u][hh] = s.q[rg][n][hh][lane];
                     }
             wait_unit();
             u4 kw[2 * TW][2];
@@ -430,15 +609,22 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
             }
         }
 
-        bool bad = false;
-        auto ok_of = [&](int rg, int t, bool ok[2][4]) { // of the wave's tile t
+        // `whole`: every row of the unit attends all of the wave's keys, as mostly
+        uint64_t seen = ~(uint64_t)0;
+#pragma unroll
+        for (int rg = 0; rg < U; ++rg)
+            seen &= rg < groups ? see[rg] : ~(uint64_t)0;
+        const bool whole = __all((seen << (64 - KW)) == ~(uint64_t)0 << (64 - KW));
+        auto ok_of = [&](auto all, int rg, int t, bool ok[2][4]) { // of the wave's tile t
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    ok[b][r] = (uint32_t)(see[rg] >> (32 * t)) >> (16 * b + 4 * g + r) & 1;
+                    ok[b][r] = decltype(all)::value ||
+                               ((uint32_t)(see[rg] >> (32 * t)) >> (16 * b + 4 * g + r) & 1);
         };
-        if (mine) {
+        auto maxima = [&](auto all) {
+            float zero = 0.f; // a NaN once an attended score is not finite
 #pragma unroll
             for (int rg = 0; rg < U; ++rg) {
                 if (rg >= groups)
@@ -447,7 +633,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
                 for (int t = 0; t < TW; ++t) {
                     bool ok[2][4];
                     float v[2][4];
-                    ok_of(rg, t, ok);
+                    ok_of(all, rg, t, ok);
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -456,68 +642,76 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
                             if (p.softcap > 0.f)
                                 v[b][r] = soft_cap(v[b][r], p.softcap, p.inv_softcap);
                             acc[rg][2 * t + b][r] = v[b][r];
+                            zero = __builtin_fmaf(ok[b][r] ? v[b][r] : 0.f, 0.f, zero);
                         }
-                    bad |= bad_scores(v, ok);
                     const float m = tile_max(v, ok);
                     if (g == 0)
-                        s.max[TW * w + t][16 * rg + col] = m;
+                        s.max[16 * rg + col][TW * w + t] = m;
                 }
             }
-        }
-        if (bad)
-            atomicOr(p.err, kErrScore);
+            if (zero != 0.f)
+                atomicOr(p.err, kErrScore);
+        };
+        if (whole)
+            maxima(std::true_type{});
+        else
+            maxima(std::false_type{});
         lds_barrier(); // every tile's maximum; the query is used
-        if (more)
+        if (new_q)
             issue_q(y);
 
-        if (mine) {
+        float last[U]; // the chunk's maximum
+        auto probabilities = [&](auto all) {
 #pragma unroll
             for (int rg = 0; rg < U; ++rg) {
+                last[rg] = kNegInf;
                 if (rg >= groups)
                     continue;
+                float tm[kTilesPerChunk];
+                *(f4 *)tm = *(const f4 *)&s.max[16 * rg + col][0];
+                *(f4 *)(tm + 4) = *(const f4 *)&s.max[16 * rg + col][4];
                 float before = kNegInf;
-                for (int t = t0; t < TW * w; ++t)
-                    before = fmaxf(before, s.max[t][16 * rg + col]);
+#pragma unroll
+                for (int t = 0; t < kTilesPerChunk; ++t) {
+                    before = t < TW * w ? fmaxf(before, tm[t]) : before;
+                    last[rg] = fmaxf(last[rg], tm[t]);
+                }
 #pragma unroll
                 for (int t = 0; t < TW; ++t) {
                     const int tile = TW * w + t;
-                    if (tile < t0 || tile > t1)
-                        continue;
                     bool ok[2][4];
                     float v[2][4], pr[2][4];
-                    ok_of(rg, t, ok);
+                    ok_of(all, rg, t, ok);
+                    float m = before;
+#pragma unroll
+                    for (int i = 0; i < kTilesPerChunk; ++i)
+                        m = i == tile ? fmaxf(m, tm[i]) : m;
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             v[b][r] = acc[rg][2 * t + b][r];
-                    const float m = fmaxf(before, s.max[tile][16 * rg + col]);
                     const float ms = safe_max(m);
                     const float sum = tile_probs(v, ok, ms, pr);
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
                         s.p[rg][tile][b][lane] = f4{pr[b][0], pr[b][1], pr[b][2], pr[b][3]};
-                    if (g == 0) {
-                        s.alpha[tile][16 * rg + col] = fexp(before - ms);
-                        s.sum[tile][16 * rg + col] = sum;
-                    }
+                    if (g == 0)
+                        s.factors[tile][16 * rg + col] = f2{fexp(before - ms), sum};
                     before = m;
                 }
             }
-        }
-        float last[U]; // the chunk's maximum
-        if (w == 0) {
-#pragma unroll
-            for (int rg = 0; rg < U; ++rg) {
-                last[rg] = kNegInf;
-                for (int t = t0; t <= t1 && rg < groups; ++t)
-                    last[rg] = fmaxf(last[rg], s.max[t][16 * rg + col]);
-            }
-        }
+        };
+        if (whole)
+            probabilities(std::true_type{});
+        else
+            probabilities(std::false_type{});
+        if (new_q && tid == 0)
+            s.taken = behind_next;
         if (more)
             store(y, f, buf ^ 1);
         lds_barrier(); // probabilities, row sums and factors
-        spare_next = spare_slot(behind);
+        const uint32_t live = (uint32_t)__ballot(lane < kTilesPerChunk && s.live[buf][lane % 8]);
 
         // the l chain and the P.V chains of the wave's dims: D of 16 dims x 16 rows
         float l[U];
@@ -534,16 +728,36 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         auto behind_v = [&](int i) {
             const int n = i + NB - rounds; // the next item's first units follow this one's
             return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
-                         : line_k(rows_k(s.slots[behind], spare_next, y.kh), n);
+                         : line_k(rows_k(s.slots[behind], y.kh), n);
         };
         c = behind_v(0);
+        // The probabilities and factors of the 16 keys behind n of the tiles' from t0 on,
+        // for all rows (of keys past the last tile: any).
+        struct Weights {
+            f4 p[U];
+            f2 factors[U];
+        };
+        auto weights = [&](int n, int b) {
+            const int t = min(t0 + n / kTile, kTilesPerChunk - 1);
+            Weights x;
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                x.p[rg] = s.p[rg][t][b][lane];
+                if (b == 0)
+                    x.factors[rg] = s.factors[t][16 * rg + col];
+            }
+            return x;
+        };
 #pragma unroll 1
         for (int i = 0; i < rounds; ++i) {
-            wait_unit();
             // 16 keys at a time: four chain steps of 4 keys (r), each with the lane's
             // own key and VL dims
             constexpr int WV = (VL * (int)sizeof(T) + 3) / 4; // words of a lane's values
             constexpr int kSixteens = C::kKeysV / 16, kHeld = kSixteens < 4 ? kSixteens : 4;
+            auto half = [&](int h) { return C::kKeysV < kTile ? i % 2 : h % 2; };
+            Weights x[2];
+            x[0] = weights(C::kKeysV * i, half(0));
+            wait_unit();
 #pragma unroll 1
             for (int h0 = 0; h0 < kSixteens; h0 += kHeld) {
                 uint32_t vw[kHeld][4][WV];
@@ -580,26 +794,27 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
 #pragma unroll
                 for (int h = 0; h < kHeld; ++h) {
                     const int n = C::kKeysV * i + 16 * (h0 + h), t = t0 + n / kTile;
-                    if (C::kKeysV > kTile && t > t1)
+                    // the next one's behind these products (of this unit)
+                    if (h + 1 < kHeld || kHeld < kSixteens)
+                        x[(h + 1) % 2] = weights(n + 16, half(h + 1));
+                    if ((C::kKeysV > kTile && t > t1) || !(live >> t & 1))
                         continue;
-                    const int b = C::kKeysV < kTile ? i % 2 : h % 2;
 #pragma unroll
                     for (int rg = 0; rg < U; ++rg) {
                         if (rg >= groups)
                             continue;
-                        if (b == 0) {
-                            const float alpha = s.alpha[t][16 * rg + col];
-                            l[rg] = __builtin_fmaf(l[rg], alpha, s.sum[t][16 * rg + col]);
+                        if (half(h) == 0) {
+                            const f2 f = x[h % 2].factors[rg];
+                            l[rg] = __builtin_fmaf(l[rg], f.x, f.y);
 #pragma unroll
                             for (int j = 0; j < VL; ++j)
-                                O[rg][j] = O[rg][j] * alpha;
+                                O[rg][j] = O[rg][j] * f.x;
                         }
-                        const f4 pr = s.p[rg][t][b][lane];
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
 #pragma unroll
                             for (int j = 0; j < VL; ++j)
-                                O[rg][j] = mfma(value_of<T>(vw[h][r], j), pr[r], O[rg][j]);
+                                O[rg][j] = mfma(value_of<T>(vw[h][r], j), x[h % 2].p[rg][r], O[rg][j]);
                     }
                 }
             }
@@ -607,11 +822,38 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
 
         // (the next query's copies are older than its first units')
         __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::NE * NB));
+        if (new_q)
+            scale_q();
+
+        // a row without a key in the chunk merges as an empty part
+        const bool merging = now.merged && now.chunks > 1;
+        if (merging) {
+#pragma unroll
+            for (int rg = 0; rg < U; ++rg) {
+                if (chunk == 0) {
+                    M1[rg] = kNegInf;
+                    L1[rg] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < VL; ++j)
+                        merged[rg][j] = f4{0.f, 0.f, 0.f, 0.f};
+                }
+                const bool some = l[rg] != 0.f;
+                const MergeFactors mf = merge_factors(M1[rg], last[rg]);
+                L1[rg] = merge_value(L1[rg], l[rg], mf);
+                M1[rg] = mf.m;
+#pragma unroll
+                for (int j = 0; j < VL; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        merged[rg][j][e] =
+                            merge_value(merged[rg][j][e], some ? O[rg][j][e] : 0.f, mf);
+            }
+        }
         // D's row 4 g + e of block j is the dim that lane 4 g + e of the operand had:
         // a lane has 4 VL dims in a row
         const int d0 = 16 * VL * w + 4 * VL * g;
         bool nonfinite = false;
-        if (!x.empty) {
+        if (!merging || last_chunk) {
 #pragma unroll
             for (int rg = 0; rg < U; ++rg) {
                 const int r = 16 * rg + col;
@@ -620,7 +862,8 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
                 const int f0 = x.first_row + r, token = (int)divided(f0, p.by_group);
                 const int head = x.kh * p.group + f0 - token * p.group;
                 const int64_t part = ((int64_t)(x.row + token) * p.row_chunks + x.ci) * p.qheads + head;
-                const bool some = l[rg] != 0.f; // a key that the row attends
+                const float sum = merging ? L1[rg] : l[rg];
+                const bool some = sum != 0.f; // a key that the row attends
                 float *dst = x.only ? p.out + (x.row + token) * p.o_stride + (int64_t)head * p.dim
                                     : p.ws_o + part * p.dim;
                 if (x.only && !some)
@@ -632,15 +875,16 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
                     f4 v;
 #pragma unroll
                     for (int a = 0; a < 4; ++a) {
-                        const float o = O[rg][(4 * k + a) % VL][(4 * k + a) / VL];
-                        v[a] = x.only ? o / l[rg] : some ? o : 0.f;
+                        const int j = (4 * k + a) % VL, e = (4 * k + a) / VL;
+                        const float o = merging ? merged[rg][j][e] : O[rg][j][e];
+                        v[a] = x.only ? o / sum : some ? o : 0.f;
                         nonfinite |= x.only && !is_finite(v[a]);
                     }
                     stg4(dst + d0 + 4 * k, v);
                 }
                 if (!x.only && w == 0 && g == 0) {
-                    stg(p.ws_ml + 2 * part, last[rg]);
-                    stg(p.ws_ml + 2 * part + 1, l[rg]);
+                    stg(p.ws_ml + 2 * part, merging ? M1[rg] : last[rg]);
+                    stg(p.ws_ml + 2 * part + 1, sum);
                 }
             }
         }
@@ -649,9 +893,13 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
         if (!more)
             break;
         lds_barrier(); // the next query
-        item = next;
         x = y;
-        spare = spare_next;
+        ++chunk;
+        if (last_chunk) {
+            now = next;
+            next = taken_item();
+            chunk = 0;
+        }
     }
     // no copy may land in LDS that another workgroup owns by then
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
@@ -660,14 +908,13 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads), 2) void paged_rows_k
 // The LDS of a CU, less the kernel's static words.
 constexpr size_t kRowsLds = 160 * 1024 - 64;
 
-template <int DK, int U, int NB> constexpr size_t rows_lds_bytes(int requests)
+template <int DK, int U, int NB> constexpr size_t rows_lds_bytes()
 {
-    return sizeof(RowsLds<DK, U>) + rows_ring_bytes(NB) + tree_words_bytes(requests);
+    return sizeof(RowsLds<DK, U>) + rows_ring_bytes(NB);
 }
 
-// Workgroups that a CU holds at once (as resident_groups of paged_kv.hpp).
-template <int DK, typename T, bool FULL, int U, int NB>
-static hipError_t resident_rows(int requests, int *groups)
+// Workgroups that a CU holds at once, asked once per device.
+template <int DK, typename T, bool FULL, int U, int NB> static hipError_t resident_rows(int *groups)
 {
     const auto kernel = (const void *)paged_rows_kernel<DK, T, FULL, U, NB>;
     static std::atomic<int> known[kMaxDevices];
@@ -678,23 +925,18 @@ static hipError_t resident_rows(int requests, int *groups)
     if (dev < 0 || dev >= kMaxDevices)
         return hipErrorInvalidDevice;
     *groups = known[dev].load(std::memory_order_acquire);
-    if (*groups > 0 && requests <= kFewRequests)
+    if (*groups > 0)
         return hipSuccess;
-    constexpr auto bytes = rows_lds_bytes<DK, U, NB>;
-    static_assert(bytes(kFewRequests) <= kRowsLds, "the LDS of a CU");
-    if (*groups == 0) {
-        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)std::min(bytes(kMaxRequests), kRowsLds));
-        if (e != hipSuccess)
-            return e;
-    }
-    const int most = requests <= kFewRequests ? kFewRequests : requests;
-    e = hipOccupancyMaxActiveBlocksPerMultiprocessor(groups, kernel, RowsCfg<DK, T, U>::kThreads, bytes(most));
+    constexpr size_t bytes = rows_lds_bytes<DK, U, NB>();
+    static_assert(bytes <= kRowsLds, "the LDS of a CU");
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess)
+        e = hipOccupancyMaxActiveBlocksPerMultiprocessor(groups, kernel,
+                                                         RowsCfg<DK, T, U>::kThreads, bytes);
     if (e != hipSuccess)
         return e;
     *groups = std::max(*groups, 1);
-    if (requests <= kFewRequests)
-        known[dev].store(*groups, std::memory_order_release);
+    known[dev].store(*groups, std::memory_order_release);
     return hipSuccess;
 }
 
@@ -702,14 +944,18 @@ template <int DK, typename T, bool FULL, int U, int NB>
 static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
     int groups = 0;
-    const hipError_t e = resident_rows<DK, T, FULL, U, NB>(p.requests, &groups);
+    const hipError_t e = resident_rows<DK, T, FULL, U, NB>(&groups);
     if (e != hipSuccess)
         return e;
+    // (the items at the requests' longest)
     const int64_t units = (rows + 16 * U - 1) / (16 * U);
-    const int64_t grid = std::min<int64_t>(chunks * p.kvheads * units,
-                                           (int64_t)groups * std::max(device_cus(), 1));
+    const int64_t items = std::min<int64_t>(chunks * p.kvheads * units, p.max_items);
+    const int64_t grid = std::min<int64_t>(items, (int64_t)groups * std::max(device_cus(), 1));
+    const int64_t plans = std::min<int64_t>((items + kPlanThreads - 1) / kPlanThreads, 256);
+    paged_plan_kernel<16 * U>
+        <<<(unsigned)plans, kPlanThreads, tree_words_bytes(p.requests), stream>>>(p, (int)grid);
     paged_rows_kernel<DK, T, FULL, U, NB>
-        <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, U, NB>(p.requests), stream>>>(p);
+        <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, U, NB>(), stream>>>(p);
     return hipGetLastError();
 }
 
@@ -722,14 +968,9 @@ constexpr int most_groups(int dk)
 template <int DK, typename T, bool FULL>
 static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    // (the words of many requests leave less LDS)
-    constexpr int M = most_groups(DK);
-    static_assert(rows_lds_bytes<DK, 1, 1>(kMaxRequests) <= kRowsLds, "one always fits");
-    if (rows > 32 && rows_lds_bytes<DK, M, 1>(p.requests) <= kRowsLds)
-        return launch_rows<DK, T, FULL, M, 1>(p, rows, chunks, stream);
-    if (rows > 16 && rows_lds_bytes<DK, 2, 1>(p.requests) <= kRowsLds)
-        return launch_rows<DK, T, FULL, 2, 1>(p, rows, chunks, stream);
-    return launch_rows<DK, T, FULL, 1, 1>(p, rows, chunks, stream);
+    return rows <= 16   ? launch_rows<DK, T, FULL, 1, 1>(p, rows, chunks, stream)
+           : rows <= 32 ? launch_rows<DK, T, FULL, 2, 1>(p, rows, chunks, stream)
+                        : launch_rows<DK, T, FULL, most_groups(DK), 1>(p, rows, chunks, stream);
 }
 
 template <int DK>

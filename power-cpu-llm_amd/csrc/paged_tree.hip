@@ -27,14 +27,17 @@ __global__ __launch_bounds__(kCombineMost) void tree_combine_kernel(TreeParams p
     if (req.y <= 1)
         return;
     const int row0 = req.x, held = req.z, n = req.w;
-    const int first = first_tree_key(p, held) / kChunk;
+    const int first = first_tree_key(p, held) / kChunk, end = first + req.y;
+    const int run = p.plan ? p.plan->run : 1;
+    if ((end - 1) / run == first / run)
+        return; // one run: written already
     for (int i = blockIdx.x / p.requests; i < n; i += gridDim.x / p.requests) {
         int c0 = first, c1 = c0 + req.y;
         if (!p.masks) {
             c0 = first_tree_key(p, held + i) / kChunk;
             c1 = (held + i) / kChunk + 1;
         }
-        const RowParts r = {(uint32_t)((row0 + i) * p.row_chunks + c0 - first), c0, c1};
+        const RowParts r = {(uint32_t)((row0 + i) * p.row_chunks), c0, c1, first, end, run};
         combine_row<BATCH>(p, c, r, blockIdx.y * c.heads, 4 * c.lanes * blockIdx.z,
                            [&](int h, int d, const Merged4 &t) {
                                if (t.L != 0.f)
@@ -77,6 +80,17 @@ static int64_t most_rows(const pcl_paged_tree_desc &d)
     return std::min(d.q_rows, d.requests * std::min(d.max_new, d.max_length));
 }
 
+bool few_items(bool whole, int64_t items, int64_t rows, int64_t unit)
+{
+    return whole && items * ((rows + unit - 1) / unit) <= device_cus();
+}
+
+bool many_rows(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows)
+{
+    const bool whole = dim == 64 || dim == 128 || dim == 256 || dim == 512;
+    return rows > 8 && !few_items(whole, chunks * kvheads, rows, 8);
+}
+
 static int check_tree(const pcl_paged_tree_desc &d)
 {
     const pcl_page_pools &s = d.pools;
@@ -104,21 +118,34 @@ static int check_tree(const pcl_paged_tree_desc &d)
             4)
         return PCL_INVALID_SHAPE;
     // item and partial indices of the whole batch stay below 2^31 (an item has a
-    // row at least)
-    if (most_chunks(d) > kMaxSlots / (d.q_rows * d.qheads))
+    // row at least, or ends a request's)
+    if (most_chunks(d) > kMaxSlots / ((d.q_rows + d.requests) * d.qheads))
         return PCL_INVALID_SHAPE;
     return PCL_OK;
 }
 
-// Workspace bytes: four words of every request, then the rows' chunk partials at
-// the requests' longest (none where no request can have two chunks).
+// Items of a launch of many rows, at most (a unit has sixteen rows at least, and every
+// request may end in part of one); 0 for a launch of few rows.
+static int64_t most_items(const pcl_paged_tree_desc &d)
+{
+    const int64_t group = d.qheads / d.pools.kvheads;
+    if (!many_rows(d.pools.dim, most_chunks(d) * d.requests, d.pools.kvheads,
+                   std::min(d.max_new, d.max_length) * group))
+        return 0;
+    return most_chunks(d) * d.pools.kvheads * (most_rows(d) * group / 16 + d.requests);
+}
+
+// Workspace bytes: the plan, four words of every request, then the rows' chunk
+// partials at the requests' longest (none where no request can have two chunks).
 static size_t tree_bytes(const pcl_paged_tree_desc &d)
 {
     if (d.requests == 0)
         return 0;
     const int64_t each = most_chunks(d);
     const size_t parts = each > 1 ? (size_t)(d.q_rows * each) * d.qheads : 0;
-    return d.requests * sizeof(int4) + parts * (d.pools.dim + 2) * sizeof(float);
+    const int64_t items = most_items(d);
+    return (items ? sizeof(PlanHead) + items * sizeof(PlanItem) : 0) +
+           d.requests * sizeof(int4) + parts * (d.pools.dim + 2) * sizeof(float);
 }
 
 } // namespace pcl
@@ -160,6 +187,10 @@ int pcl_paged_tree_attention(pcl_context *ctx, const pcl_paged_tree_desc *desc)
     p.row_stride = s.kvheads * s.dim;
     p.out = d.out;
     p.o_stride = d.o_stride;
+    const int64_t items = pcl::most_items(d);
+    p.max_items = (int)items;
+    p.plan = items ? reinterpret_cast<pcl::PlanHead *>(body) : nullptr;
+    body += items ? 16 * (1 + items) : 0;
     p.ws_req = reinterpret_cast<int4 *>(body);
     p.ws_o = body + 4 * d.requests;
     p.ws_ml = p.ws_o + parts * s.dim;
