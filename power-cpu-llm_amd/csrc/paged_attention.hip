@@ -20,7 +20,7 @@ __global__ __launch_bounds__(kCombineMost) void paged_combine_kernel(PagedParams
     const int4 req = p.ws_req[blockIdx.x]; // (one load; all that a request's lanes need)
     if (req.y <= 1)
         return;
-    const RowParts r = {(uint32_t)req.x, req.z, req.z + req.y, req.z, req.z + req.y, 1};
+    const RowParts r = {(uint32_t)req.x, req.z, req.z + req.y, req.z, 0};
     combine_row<BATCH>(p, c, r, blockIdx.y * c.heads, 4 * c.lanes * blockIdx.z,
                        [&](int h, int d, const Merged4 &t) {
                            write_merged(p, t,

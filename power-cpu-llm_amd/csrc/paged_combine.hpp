@@ -18,13 +18,12 @@ struct CombineShape {
     int lanes, spans, heads; // powers of two; heads: query heads of a workgroup
 };
 
-// A row's partials: chunk c's of [c0, c1) is base + c - first. Where the chunks come
-// in runs, those of the run that begins a span are merged already, into the place of
-// its last one; first and end bound the request's chunks.
+// A row's partials: chunk c's of [c0, c1) is base + c - first. The chunks of a span
+// that ends at `split` or before it are merged already, into the place of the last one.
 struct RowParts {
     uint32_t base;
     int c0, c1;
-    int first, end, run;
+    int first, split;
 };
 
 // Merges them for the workgroup's heads and dims and calls write(head, dim, the
@@ -50,12 +49,9 @@ __device__ __forceinline__ void combine_row(const PagedParams &p, const CombineS
         if (r0 + gi < s1) {
             int e = min((r0 + gi + 1) * kSpanChunks, c1);
             int a = max((r0 + gi) * kSpanChunks, c0);
-            if (r.run > 1) {
-                const int merged = run_end(max((r0 + gi) * kSpanChunks, r.first), r.end, r.run);
-                if (a < merged) {
-                    a = merged - 1;
-                    e = max(e, merged);
-                }
+            if (a < r.split) {
+                e = min((r0 + gi + 1) * kSpanChunks, r.split);
+                a = e - 1;
             }
             for (; a < e; a += BATCH) {
                 f2 ml[BATCH];

@@ -81,34 +81,26 @@ __device__ __forceinline__ uint32_t divided(uint32_t x, const Divisor &d)
     return d.mul ? __umulhi(x, d.mul) >> d.shift : x;
 }
 
-// An item of a launch of many rows: a run of chunks of one request, KV head and unit
-// of query rows, all in one span and one aligned group of `run` chunks.
+// An item of a launch of many rows: the chunks of a span, or one, of one request, KV
+// head and unit of query rows.
 struct PlanItem {
     int b, kh;
     int row, held, n;     // as TreeItem's
     int first_row, nrows; // of the unit
     int from, to;         // the first and the last key that any row may attend
     int chunk, chunks;    // first one, and how many (0: no key, nothing to do)
-    int slot;             // partial (of a row's) of the first chunk, or of the merged run
-    int merged;           // the run begins its span: its chunks are merged as they come
-    int only;             // and is all of the request
-    int spare[2];
+    int slot;             // partial (of a row's) of the last chunk, the result's
+    int only;             // the chunks are all of the request's
+    int spare[3];
 };
 
 struct PlanHead {
-    int items, run;
+    int items, uneven; // uneven: some have several chunks
     int taken[8]; // items that each XCD's workgroups have taken, of its own
     int spare[6];
 };
 
 static_assert(sizeof(PlanItem) == 64 && sizeof(PlanHead) == 64, "whole scalar loads");
-
-// The run that begins a span at `first` (the request's first chunk in it) ends before
-// this chunk; `end`: behind the request's last.
-__device__ __forceinline__ int run_end(int first, int end, int run)
-{
-    return min((first / run + 1) * run, end);
-}
 
 // Of a launch over every new token of a step (lengths: with the step's tokens).
 struct TreeParams : PagedParams {
@@ -117,9 +109,11 @@ struct TreeParams : PagedParams {
     const int32_t *positions;      // [q_rows], with masks and a window
     int mask_words, max_new;
     int row_chunks; // partials of a row: chunks that one request may have
-    // of a launch of many rows, written by its plan kernel: the items' count and the
-    // chunks of a run, then the items (null: every chunk is an item)
+    // of a launch of many rows, written by its plan kernel: the items behind their
+    // count, and of every request the first chunk that is an item of its own, those
+    // before it being of whole spans (null: every chunk is an item)
     PlanHead *plan;
+    int32_t *split; // [requests]
     int max_items;
     Divisor by_group, by_kvheads, by_page_tokens;
 };
@@ -166,6 +160,8 @@ template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream);
 template <int DK>
 hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream);
+// Rows of a KV head and request up to which one wave's MFMAs hold a unit (paged_kv.hpp).
+constexpr int64_t kFewRows = 8;
 // Whether units of `unit` rows leave a tree launch at most an item per CU, each with a
 // CU to itself; `whole`: the head dim is one that needs no padding. `items`: at one
 // unit, `rows`: of a KV head that one request has at most.

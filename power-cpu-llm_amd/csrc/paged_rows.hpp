@@ -162,92 +162,185 @@ __device__ __forceinline__ uint32_t or_rows(uint32_t x)
     return x;
 }
 
-// The items of a launch, by all its threads: chunks in runs of as many as leave each
-// workgroup kRounds items or more, up to a span. Of a run that begins its span the
-// chunks are merged in registers, in their order; others write a partial each, but
-// share the query and the search for them.
-constexpr int kRounds = 24;
+// The items of a launch. A span of a request, over a unit, is one item while that
+// leaves the workgroups evenly loaded: its chunks are merged in registers, in their
+// order, and it leaves one partial (none where it is all of the request). The rest are
+// items of a chunk each, which come last and fill what the spans leave uneven: with T
+// chunks in all, W workgroups and no span longer than s chunks, the spans are the first
+// W (where T >= s W) and those that begin in the first T - s W chunks. With the combine,
+// against a chunk each (MI355X): trees of 12 tokens behind up to 32K keys of d512 (T = 25
+// W) 0.97 ms and 1.16 ms, prompt parts of 512 tokens (T = 60 W) 1.84 ms and 1.97 ms. (W
+// floor(T / (s W)) spans left XCDs unevenly loaded: 2.01 ms; spans in the first T - s W /
+// 2 chunks as well, and 257 us instead of 194 for windows of T = 4 W.)
 constexpr int kPlanThreads = 256;
+
+// The requests' words: items of spans and of chunks before each (over the KV heads),
+// its tokens with the step's and without, its first row, and its first chunk that is
+// an item of its own.
+struct PlanWords {
+    uint32_t *spans, *singles;
+    int32_t *len, *held, *row, *split;
+};
+
+constexpr size_t plan_words_bytes(int requests)
+{
+    return (6 * (size_t)requests + 2) * sizeof(uint32_t);
+}
+
+// The last request of [0, requests) whose items begin at n or before it.
+__device__ __forceinline__ int plan_request(const uint32_t *off, int requests, uint32_t n)
+{
+    int lo = 0;
+    for (int hi = requests; hi - lo > 1;) {
+        const int mid = (lo + hi) / 2;
+        if (off[mid] <= n)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// block_offsets of two values, and b's total.
+__device__ __forceinline__ void block_offsets2(uint64_t a, uint64_t b,
+                                               uint64_t (&waves)[2][kPlanThreads / 64],
+                                               uint64_t *a_at, uint64_t *b_at, uint64_t *total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t x = a, y = b;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t xo = __shfl_up(x, o), yo = __shfl_up(y, o);
+        if (lane >= o) {
+            x += xo;
+            y += yo;
+        }
+    }
+    if (lane == 63) {
+        waves[0][wave] = x;
+        waves[1][wave] = y;
+    }
+    __syncthreads();
+    x -= a;
+    y -= b;
+    *total = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 64; ++i) {
+        x += i < wave ? waves[0][i] : 0;
+        y += i < wave ? waves[1][i] : 0;
+        *total += waves[1][i];
+    }
+    __syncthreads();
+    *a_at = x;
+    *b_at = y;
+}
 
 template <int UNIT>
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(TreeParams p, int workgroups)
 {
     extern __shared__ uint32_t dyn[];
-    __shared__ uint64_t waves[kPlanThreads / 64];
-    const TreeWords r = tree_words(dyn, p.requests);
+    __shared__ uint64_t waves[2][kPlanThreads / 64];
+    __shared__ int longest;
+    const int n = p.requests;
+    int32_t *words = reinterpret_cast<int32_t *>(dyn) + 2 * (n + 1);
+    const PlanWords r = {dyn, dyn + n + 1, words, words + n, words + 2 * n, words + 3 * n};
     const int tid = threadIdx.x;
-    const int per = (p.requests + kPlanThreads - 1) / kPlanThreads;
-    const int i0 = min(tid * per, p.requests), i1 = min(i0 + per, p.requests);
-    auto units_of = [&](int n) { return ((uint32_t)n * (uint32_t)p.group + UNIT - 1) / UNIT; };
-    uint64_t sum = 0; // (requests that share rows may add up past 2^32)
+    const int per = (n + kPlanThreads - 1) / kPlanThreads;
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    const uint32_t kvheads = (uint32_t)p.kvheads;
+    auto units_of = [&](int m) { return ((uint32_t)m * (uint32_t)p.group + UNIT - 1) / UNIT; };
+    auto spans_of = [](int first, int chunks) {
+        return chunks ? (first + chunks - 1) / kSpanChunks - first / kSpanChunks + 1 : 0;
+    };
+    if (tid == 0)
+        longest = 1;
+    __syncthreads();
+    uint64_t chunk_sum = 0, span_sum = 0; // (requests that share rows may add up past 2^32)
     bool bad = false;
+    int most = 0;
     for (int i = i0; i < i1; ++i) {
         const TreeKeys k = tree_keys(p, i, &bad);
         r.len[i] = k.len;
         r.held[i] = k.held;
         r.row[i] = k.row;
-        sum += (uint64_t)tree_chunks(p, k) * units_of(k.len - k.held);
+        const int chunks = tree_chunks(p, k), first = first_tree_key(p, k.held) / kChunk;
+        const int spans = spans_of(first, chunks);
+        chunk_sum += (uint64_t)chunks * units_of(k.len - k.held) * kvheads;
+        span_sum += (uint64_t)spans * units_of(k.len - k.held) * kvheads;
+        const int begin = min(kSpanChunks - first % kSpanChunks, chunks);
+        most = max(most, spans > 2 ? kSpanChunks : max(begin, chunks - begin));
     }
-    uint64_t total;
-    block_offsets(sum, waves, &total);
-    int run = kSpanChunks;
-    while (run > 1 && total * p.kvheads < (uint64_t)run * kRounds * workgroups)
-        run /= 2;
-    // groups of `run` chunks that a request's lie in, over the units
-    sum = 0;
+    if (most > 1)
+        atomicMax(&longest, most);
+    uint64_t spans_at, chunks_at, total; // (barriers: longest)
+    block_offsets2(span_sum, chunk_sum, waves, &spans_at, &chunks_at, &total);
+    const bool fits = total <= (uint64_t)p.max_items;
+    bad |= !fits;
+    const uint64_t round = (uint64_t)longest * (uint32_t)workgroups;
+    const uint64_t by_count = total >= round ? (uint32_t)workgroups : 0;
+    const uint64_t by_chunks = total > round ? total - round : 0;
+    span_sum = chunk_sum = 0;
     for (int i = i0; i < i1; ++i) {
         const TreeKeys k = {r.row[i], r.held[i], r.len[i]};
-        const int chunks = tree_chunks(p, k), first = first_tree_key(p, k.held) / kChunk;
-        const uint32_t runs = chunks ? (first + chunks - 1) / run - first / run + 1 : 0;
-        r.off[i] = runs * units_of(k.len - k.held);
-        sum += r.off[i];
-        if (blockIdx.x == 0)
-            p.ws_req[i] = int4{k.row, chunks, k.held, k.len - k.held};
-    }
-    uint64_t at = block_offsets(sum, waves, &total);
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t items = r.off[i];
-        r.off[i] = (uint32_t)at;
-        at += items;
-    }
-    const bool fits = total * p.kvheads <= (uint64_t)p.max_items;
-    bad |= !fits;
-    const uint32_t items = fits ? (uint32_t)total : 0;
-    if (tid == 0) {
-        r.off[p.requests] = items;
-        if (blockIdx.x == 0) {
-            p.plan->items = (int)(items * (uint32_t)p.kvheads);
-            p.plan->run = run;
-            // (the first one of a workgroup is its own)
-            for (int i = 0; i < 8; ++i)
-                p.plan->taken[i] = workgroups % 8 ? workgroups : workgroups / 8;
+        const int chunks = fits ? tree_chunks(p, k) : 0;
+        const int first = first_tree_key(p, k.held) / kChunk, spans = spans_of(first, chunks);
+        const uint32_t units = units_of(k.len - k.held), each = units * kvheads;
+        int whole = 0; // spans that are items
+        if (spans) {
+            const uint64_t a = by_count > spans_at ? (by_count - spans_at) / each : 0;
+            const uint64_t left = by_chunks > chunks_at ? (by_chunks - chunks_at) / each : 0;
+            const uint64_t b = left ? (first % kSpanChunks + left - 1) / kSpanChunks + 1 : 0;
+            whole = (int)min(max(a, b), (uint64_t)spans);
         }
+        const int split =
+            whole ? min((first / kSpanChunks + whole) * kSpanChunks, first + chunks) : first;
+        spans_at += (uint64_t)spans * each;
+        chunks_at += (uint64_t)chunks * each;
+        r.split[i] = split;
+        r.spans[i] = whole * each;
+        r.singles[i] = (first + chunks - split) * each;
+        span_sum += r.spans[i];
+        chunk_sum += r.singles[i];
+        if (blockIdx.x == 0) {
+            p.ws_req[i] = int4{k.row, chunks, k.held, k.len - k.held};
+            p.split[i] = split;
+        }
+    }
+    // (at most max_items together: halves of a word)
+    uint64_t both, before = block_offsets(span_sum << 32 | chunk_sum, waves[0], &both);
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t a = r.spans[i], b = r.singles[i];
+        r.spans[i] = (uint32_t)(before >> 32);
+        r.singles[i] = (uint32_t)before;
+        before += (uint64_t)a << 32 | b;
+    }
+    const uint32_t spans = (uint32_t)(both >> 32), all = spans + (uint32_t)both;
+    if (tid == 0 && blockIdx.x == 0) {
+        p.plan->items = (int)all;
+        p.plan->uneven = spans != 0;
+        // (the first one of a workgroup is its own)
+        for (int i = 0; i < 8; ++i)
+            p.plan->taken[i] = workgroups % 8 ? workgroups : workgroups / 8;
     }
     if (bad && blockIdx.x == 0)
         atomicOr(p.err, kErrPages);
     __syncthreads();
     PlanItem *out = reinterpret_cast<PlanItem *>(p.plan + 1);
-    const uint32_t all = items * (uint32_t)p.kvheads;
-    for (uint32_t n = blockIdx.x * kPlanThreads + tid; n < all; n += gridDim.x * kPlanThreads) {
-        // units of a run and KV head side by side: they share its keys
+    for (uint32_t i = blockIdx.x * kPlanThreads + tid; i < all; i += gridDim.x * kPlanThreads) {
+        // units of a span or chunk and KV head side by side: they share its keys
+        const bool span = i < spans;
+        const uint32_t at = span ? i : i - spans;
+        const uint32_t *off = span ? r.spans : r.singles;
         PlanItem x;
-        x.b = 0;
-        for (int lo = 0, hi = p.requests; hi - lo > 1;) {
-            const int mid = (lo + hi) / 2;
-            if (r.off[mid] * (uint64_t)p.kvheads <= n)
-                lo = mid;
-            else
-                hi = mid;
-            x.b = lo;
-        }
+        x.b = plan_request(off, n, at);
         const TreeKeys k = {r.row[x.b], r.held[x.b], r.len[x.b]};
         x.row = k.row;
         x.held = k.held;
         x.n = k.len - k.held;
-        const uint32_t rest = n - r.off[x.b] * (uint32_t)p.kvheads, units = units_of(x.n);
+        const uint32_t rest = at - off[x.b], units = units_of(x.n);
         const int unit = (int)(rest % units);
-        x.kh = (int)(rest / units % (uint32_t)p.kvheads);
-        const int group = (int)(rest / units / (uint32_t)p.kvheads); // of chunks
+        x.kh = (int)(rest / units % kvheads);
+        const int part = (int)(rest / units / kvheads);
         x.first_row = unit * UNIT;
         x.nrows = min(x.n * p.group - x.first_row, UNIT);
         x.from = first_tree_key(p, k.held);
@@ -257,16 +350,15 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(TreeParams p, 
             x.from = first_tree_key(p, k.held + x.first_row / p.group);
             x.to = k.held + (x.first_row + x.nrows - 1) / p.group;
         }
-        const int g0 = (first / run + group) * run; // the group's chunks
-        const int c0 = max(g0, x.from / kChunk), c1 = min(g0 + run, x.to / kChunk + 1);
+        const int g0 = span ? (first / kSpanChunks + part) * kSpanChunks : r.split[x.b] + part;
+        const int g1 = min(g0 + (span ? kSpanChunks : 1), end);
+        const int c0 = max(g0, x.from / kChunk), c1 = min(g1, x.to / kChunk + 1);
         x.chunk = c0;
         x.chunks = max(c1 - c0, 0);
-        const int span = max(g0 / kSpanChunks * kSpanChunks, first); // its first chunk
-        x.merged = span / run == g0 / run;
-        x.slot = (x.merged ? run_end(span, end, run) - 1 : c0) - first;
-        x.only = (end - 1) / run == first / run;
-        x.spare[0] = x.spare[1] = 0;
-        out[n] = x;
+        x.slot = g1 - 1 - first;
+        x.only = max(g0, first) == first && g1 == end;
+        x.spare[0] = x.spare[1] = x.spare[2] = 0;
+        out[i] = x;
     }
 }
 
@@ -277,8 +369,8 @@ typedef const __attribute__((address_space(4))) int16w *plan_ptr;
 __device__ __forceinline__ PlanItem plan_item(plan_ptr at)
 {
     const int16w w = *at;
-    return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], w[11], w[12], w[13],
-            {0, 0}};
+    return {w[0], w[1], w[2], w[3], w[4],  w[5],  w[6],
+            w[7], w[8], w[9], w[10], w[11], w[12], {0, 0, 0}};
 }
 
 // Chunk k of an item.
@@ -293,7 +385,7 @@ __device__ __forceinline__ TreeItem chunk_item(const PlanItem &i, int k)
     x.first_row = i.first_row;
     x.nrows = i.nrows;
     x.unit = 0;
-    x.ci = (uint32_t)(i.merged ? i.slot : i.slot + k);
+    x.ci = (uint32_t)i.slot;
     x.only = i.only;
     x.empty = false;
     x.cbase = (i.chunk + k) * kChunk;
@@ -321,14 +413,32 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
     // Workgroups take items as they come to them: chunks differ in their keys, and so
     // do the runs. Of each round of the grid's items an XCD (they have the workgroups
     // in turn) has those side by side, whose units share its L2, and its workgroups
-    // take them from a counter of its own. One is taken while the one before the last
+    // take them from a counter of its own; where items differ in their chunks they take
+    // the other XCDs' behind their last one. One is taken while the one before the last
     // runs, so that nobody waits for the counter.
     const plan_ptr plan = (plan_ptr)p.plan;
     const uint32_t items = (uint32_t)(*plan)[0];
     const uint32_t parts = gridDim.x % 8 ? 1 : 8, each = gridDim.x / parts;
-    const uint32_t part = blockIdx.x % parts;
+    const bool uneven = parts == 8 && (*plan)[1] != 0;
+    uint32_t part = blockIdx.x % parts; // (by thread 0, as what follows)
     auto place = [&](uint32_t n) { return n / each * gridDim.x + part * each + n % each; };
     auto take = [&]() { return place((uint32_t)atomicAdd(&p.plan->taken[part], 1)); };
+    auto settle = [&](uint32_t n) { // n, or another XCD's item where that is past the last
+        if (n < items || !uneven)
+            return n;
+        uint32_t taken[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            taken[i] = (uint32_t)__hip_atomic_load(&p.plan->taken[i], __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            part = i;
+            if (n >= items && place(taken[i]) < items)
+                n = take();
+        }
+        return n;
+    };
     // (an item past the last has no chunks, and is not skipped)
     auto load_item = [&](uint32_t n) {
         PlanItem i;
@@ -342,7 +452,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         while (i.chunks == 0) { // (a chain's early units have none of the last keys)
             __syncthreads();
             if (tid == 0)
-                s.taken = take();
+                s.taken = settle(take());
             __syncthreads();
             i = load_item(__builtin_amdgcn_readfirstlane(s.taken));
         }
@@ -356,7 +466,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         return;
     __syncthreads();
     if (tid == 0)
-        s.taken = take();
+        s.taken = settle(take());
     PlanItem next; // (taken below)
     int chunk = 0; // of `now`
 
@@ -707,7 +817,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         else
             probabilities(std::false_type{});
         if (new_q && tid == 0)
-            s.taken = behind_next;
+            s.taken = settle(behind_next);
         if (more)
             store(y, f, buf ^ 1);
         lds_barrier(); // probabilities, row sums and factors
@@ -826,7 +936,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
             scale_q();
 
         // a row without a key in the chunk merges as an empty part
-        const bool merging = now.merged && now.chunks > 1;
+        const bool merging = now.chunks > 1;
         if (merging) {
 #pragma unroll
             for (int rg = 0; rg < U; ++rg) {
@@ -853,7 +963,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         // a lane has 4 VL dims in a row
         const int d0 = 16 * VL * w + 4 * VL * g;
         bool nonfinite = false;
-        if (!merging || last_chunk) {
+        if (last_chunk) {
 #pragma unroll
             for (int rg = 0; rg < U; ++rg) {
                 const int r = 16 * rg + col;
@@ -953,7 +1063,7 @@ static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks,
     const int64_t grid = std::min<int64_t>(items, (int64_t)groups * std::max(device_cus(), 1));
     const int64_t plans = std::min<int64_t>((items + kPlanThreads - 1) / kPlanThreads, 256);
     paged_plan_kernel<16 * U>
-        <<<(unsigned)plans, kPlanThreads, tree_words_bytes(p.requests), stream>>>(p, (int)grid);
+        <<<(unsigned)plans, kPlanThreads, plan_words_bytes(p.requests), stream>>>(p, (int)grid);
     paged_rows_kernel<DK, T, FULL, U, NB>
         <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, U, NB>(), stream>>>(p);
     return hipGetLastError();

@@ -14,8 +14,10 @@
 namespace pcl {
 
 constexpr int64_t kMaxMaskWords = 8;
-// Rows of a request that the combine's grid holds at once.
-constexpr int kCombineTokens = 32;
+// Workgroups of the combine's grid; each goes on to rows past them. (Prompt parts of
+// 4 x 512 tokens, 16 heads, behind up to 8192 keys: 95 us with a workgroup for every
+// row and head, 111 us with 2048 workgroups for 16 rows each.)
+constexpr unsigned kCombineGroups = 65536;
 
 // Rows of requests of one chunk are written already, and so is nothing of a row
 // that attends no key. A chain's token has partials of its own chunks alone.
@@ -28,16 +30,16 @@ __global__ __launch_bounds__(kCombineMost) void tree_combine_kernel(TreeParams p
         return;
     const int row0 = req.x, held = req.z, n = req.w;
     const int first = first_tree_key(p, held) / kChunk, end = first + req.y;
-    const int run = p.plan ? p.plan->run : 1;
-    if ((end - 1) / run == first / run)
-        return; // one run: written already
+    const int split = p.plan ? p.split[b] : 0;
+    if (split == end && (end - 1) / kSpanChunks == first / kSpanChunks)
+        return; // one span: written already
     for (int i = blockIdx.x / p.requests; i < n; i += gridDim.x / p.requests) {
         int c0 = first, c1 = c0 + req.y;
         if (!p.masks) {
             c0 = first_tree_key(p, held + i) / kChunk;
             c1 = (held + i) / kChunk + 1;
         }
-        const RowParts r = {(uint32_t)((row0 + i) * p.row_chunks), c0, c1, first, end, run};
+        const RowParts r = {(uint32_t)((row0 + i) * p.row_chunks), c0, c1, first, split};
         combine_row<BATCH>(p, c, r, blockIdx.y * c.heads, 4 * c.lanes * blockIdx.z,
                            [&](int h, int d, const Merged4 &t) {
                                if (t.L != 0.f)
@@ -53,8 +55,9 @@ static hipError_t launch_tree_combine(const TreeParams &p, int64_t rows, int64_t
                                       hipStream_t stream)
 {
     const CombineShape c = combine_shape(p, rows, chunks);
-    const int tokens = std::min(p.max_new, kCombineTokens);
-    const dim3 grid = combine_grid(p, c, (unsigned)p.requests * tokens);
+    dim3 grid = combine_grid(p, c, (unsigned)p.requests);
+    const unsigned each = grid.x * grid.y * grid.z;
+    grid.x *= std::max(1u, std::min((unsigned)p.max_new, kCombineGroups / each));
     const int threads = c.lanes * c.spans * c.heads;
     if (c.spans >= 16)
         tree_combine_kernel<16><<<grid, threads, 0, stream>>>(p, c);
@@ -88,7 +91,7 @@ bool few_items(bool whole, int64_t items, int64_t rows, int64_t unit)
 bool many_rows(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows)
 {
     const bool whole = dim == 64 || dim == 128 || dim == 256 || dim == 512;
-    return rows > 8 && !few_items(whole, chunks * kvheads, rows, 8);
+    return rows > kFewRows && !few_items(whole, chunks * kvheads, rows, kFewRows);
 }
 
 static int check_tree(const pcl_paged_tree_desc &d)
@@ -125,14 +128,18 @@ static int check_tree(const pcl_paged_tree_desc &d)
 }
 
 // Items of a launch of many rows, at most (a unit has sixteen rows at least, and every
-// request may end in part of one); 0 for a launch of few rows.
+// request may end in part of one); 0 where no launch of the shape is one on any device.
 static int64_t most_items(const pcl_paged_tree_desc &d)
 {
     const int64_t group = d.qheads / d.pools.kvheads;
-    if (!many_rows(d.pools.dim, most_chunks(d) * d.requests, d.pools.kvheads,
-                   std::min(d.max_new, d.max_length) * group))
+    if (std::min(d.max_new, d.max_length) * group <= kFewRows)
         return 0;
     return most_chunks(d) * d.pools.kvheads * (most_rows(d) * group / 16 + d.requests);
+}
+
+static size_t split_bytes(const pcl_paged_tree_desc &d) // (whole 16 bytes)
+{
+    return (size_t)((d.requests + 3) / 4) * 16;
 }
 
 // Workspace bytes: the plan, four words of every request, then the rows' chunk
@@ -144,7 +151,7 @@ static size_t tree_bytes(const pcl_paged_tree_desc &d)
     const int64_t each = most_chunks(d);
     const size_t parts = each > 1 ? (size_t)(d.q_rows * each) * d.qheads : 0;
     const int64_t items = most_items(d);
-    return (items ? sizeof(PlanHead) + items * sizeof(PlanItem) : 0) +
+    return (items ? sizeof(PlanHead) + items * sizeof(PlanItem) + split_bytes(d) : 0) +
            d.requests * sizeof(int4) + parts * (d.pools.dim + 2) * sizeof(float);
 }
 
@@ -189,8 +196,11 @@ int pcl_paged_tree_attention(pcl_context *ctx, const pcl_paged_tree_desc *desc)
     p.o_stride = d.o_stride;
     const int64_t items = pcl::most_items(d);
     p.max_items = (int)items;
-    p.plan = items ? reinterpret_cast<pcl::PlanHead *>(body) : nullptr;
-    body += items ? 16 * (1 + items) : 0;
+    const bool many = pcl::many_rows(s.dim, d.requests * each, s.kvheads,
+                                     std::min(d.max_new, d.max_length) * (d.qheads / s.kvheads));
+    p.plan = many ? reinterpret_cast<pcl::PlanHead *>(body) : nullptr;
+    p.split = many ? reinterpret_cast<int32_t *>(body + 16 * (1 + items)) : nullptr;
+    body += items ? 16 * (1 + items) + pcl::split_bytes(d) / sizeof(float) : 0;
     p.ws_req = reinterpret_cast<int4 *>(body);
     p.ws_o = body + 4 * d.requests;
     p.ws_ml = p.ws_o + parts * s.dim;

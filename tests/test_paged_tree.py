@@ -185,10 +185,10 @@ def test_page_calls_refuse_missing_words(pcl, no_context):
     # two bytes a page in whole 32, none for a small batch
     def nbytes(**kw):
         return lib.pcl_page_release_workspace_bytes(ctypes.byref(batch_of(pcl, **kw)))
-    base = nbytes()
-    assert nbytes(table_stride=1 << 13) == nbytes(pages=1 << 17) == base
-    assert nbytes(table_stride=1 + (1 << 13), pages=65) - base == 2 * 96 + 16
-    assert nbytes(pages=1 + (1 << 17)) - base == 2 * (32 + (1 << 17)) + 16
+    assert nbytes() == nbytes(table_stride=1 << 13) == nbytes(pages=1 << 17) == 0
+    wide = nbytes(table_stride=1 + (1 << 13), pages=65)
+    assert wide >= 2 * 96 + 16
+    assert nbytes(pages=1 + (1 << 17)) - wide == 2 * (32 + (1 << 17) - 96)
 
 
 def test_copy_refuses_bad_lists(pcl, no_context):
@@ -271,15 +271,29 @@ def test_workspace_holds_every_chunk_of_every_row(pcl):
     # in at most (keys + 254) div 256 + 1 chunks
     assert nbytes(max_length=16384, window=1, max_new=1) == base
     assert nbytes(max_length=16384, window=1, max_new=2) - base == 8 * 2 * part
-    assert nbytes(max_length=16384, window=1021, max_new=5) - base == 8 * 5 * part
-    assert nbytes(max_length=16384, window=1022, max_new=258) - base == 8 * 6 * part
-    assert nbytes(max_length=1000, window=(1 << 63) - 1, max_new=5) - base == 8 * 4 * part
+    assert nbytes(max_length=16384, window=1022, max_new=4) - base == 8 * 5 * part
+    assert nbytes(max_length=16384, window=1023, max_new=4) - base == 8 * 6 * part
+    assert nbytes(max_length=1000, window=(1 << 63) - 1, max_new=4) - base == 8 * 4 * part
+
+    def plan(chunks):
+        # above eight rows of a KV head: 64 bytes, and for each chunk, KV head and unit
+        # of sixteen rows (16 in all, and one that every request ends in); 16 for the
+        # requests' words
+        return 64 * (1 + chunks * 2 * (16 // 16 + 2)) + 16
+
+    assert nbytes(max_length=16384, window=1021, max_new=5) - base == 8 * 5 * part + plan(5)
+    assert nbytes(max_length=16384, window=1022, max_new=258) - base == 8 * 6 * part + plan(6)
+    assert nbytes(max_length=200, max_new=258) - base == plan(1)
     assert nbytes(requests=0) == 0
 
 
 @pytest.mark.parametrize("source,kernel", [
     ("paged_tree_d256.hip", "_ZN3pcl17paged_tree_kernelILi256EfLb1ELi1ELi1EEEvNS_10TreeParamsE"),
-    ("paged_tree_d256.hip", "_ZN3pcl17paged_tree_kernelILi256EDF16bLb1ELi4ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EfLb1ELi1ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EDF16bLb1ELi1ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EfLb1ELi3ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EDF16bLb1ELi3ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d512.hip", "_ZN3pcl17paged_rows_kernelILi512EfLb1ELi2ELi1EEEvNS_10TreeParamsE"),
     ("paged_tree.hip",
      "_ZN3pcl19tree_combine_kernelILi8EEEvNS_10TreeParamsENS_12CombineShapeE"),
 ])
@@ -1294,6 +1308,36 @@ def test_many_requests(pcl, torch, ctx):
     assert ctx.sync() == 0
     cache.check(ctx, q, out, exact=False,
                 requests=[0, 1, 7, 500, 999, 1000, 1001, 2046, 2047] + list(range(40, 80)))
+
+
+# Launches whose first spans of 16 chunks are items: those have at least as many chunks
+# (over units of 16, 32, 48 or 64 rows and KV heads) as one span for each of 256 CUs'
+# workgroups. Requests of one span, of a whole and a part, and of several with single
+# chunks behind; a request without new tokens among them.
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dtype,held,counts,window", [
+    ((16, 8, 256), "bf16", [1900, 200, 0, 5000], [700, 500, 0, 129], 0),
+    ((16, 8, 256), "f32", [30, 9000], [3, 400], 0),
+    ((16, 8, 256), "bf16", [15000, 4090], [700, 16], 0),
+    ((16, 8, 256), "f32", [20000, 600], [700, 500], 4200),
+    ((16, 2, 512), "f32", [9000, 8190, 8000, 100, 10000, 7000], [64, 80, 64, 3, 64, 70], 0),
+    ((10, 2, 208), "bf16", [9000, 16000, 4000], [300, 400, 100], 0),
+    ((16, 4, 64), "f32", [100 + i for i in range(12)], [600] * 12, 0),
+], ids=str)
+@pytest.mark.parametrize("tree", [False, True], ids=["chain", "tree"])
+def test_spans_as_items(pcl, torch, ctx, heads, dtype, held, counts, window, tree):
+    counts = [min(n, 500) for n in counts] if tree else counts
+    masks = positions = None
+    if tree:
+        masks, positions = random_trees(np.random.default_rng(19), held, counts)
+    cache = TreeCache(pcl, torch, heads, held, counts, 64, dtype, 23, masks, positions)
+    q = cache.queries()
+    out = cache.tree_attend(ctx, q, window=window)
+    assert ctx.sync() == 0
+    again = cache.tree_attend(ctx, q, window=window)
+    assert np.array_equal(bits(out), bits(again))
+    cache.check(ctx, q, out, window=window, exact=False)
+    assert ctx.sync() == 0
 
 
 @pytest.mark.gpu
