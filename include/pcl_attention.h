@@ -709,7 +709,8 @@ int pcl_page_fork(pcl_context *ctx, const pcl_page_batch *batch, const int32_t *
  * it is not grown: pcl_context_reserve the bytes before). */
 int pcl_page_release_shared(pcl_context *ctx, const pcl_page_batch *batch,
                             const int32_t *finished);
-/* Workspace bytes of that call (0 for a batch that is refused). */
+/* Workspace bytes of that call (0 where it needs none, and for a batch that is
+ * refused). */
 size_t pcl_page_release_workspace_bytes(const pcl_page_batch *batch);
 
 /* Copies rows of pages, K and V, from slot to slot in the pools of `layers` layers
@@ -734,9 +735,8 @@ int pcl_paged_copy(pcl_context *ctx, const pcl_page_pools *pools, int64_t layers
  * bit j of masks[row] (any bits; pcl_page_tree_masks makes a tree's). With a window a
  * token attends only keys whose position is less than `window` before its own (the
  * new tokens' by positions, which lie from lengths[b] to step_lengths[b] - 1).
- * Requests without new tokens
- * or with a negative newest are left out, and a token that attends no key too: their
- * output rows stay as they were. Queries are scaled and scores capped as in
+ * Requests without new tokens or with a negative newest are left out, and a token
+ * that attends no key too: their output rows stay as they were. Queries are scaled and scores capped as in
  * pcl_attention_desc. A token's output has the bits that pcl_attention_launch gives
  * for the request's keys and values in one segment (the chain: causal, first_key 0,
  * first_query lengths[b]; masks: with the same mask as bytes), whatever else is in

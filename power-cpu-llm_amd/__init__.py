@@ -620,16 +620,14 @@ class Context:
     def page_accept(self, batch, paths_ptr, counts_ptr, depth, from_ptr, to_ptr):
         """Which rows the verified branches move (slots, [requests][depth])."""
         self._check(self.lib.pcl_page_accept(
-            self.handle, ctypes.byref(batch), paths_ptr,
-            counts_ptr, int(depth), from_ptr,
+            self.handle, ctypes.byref(batch), paths_ptr, counts_ptr, int(depth), from_ptr,
             to_ptr))
 
     def page_fork(self, batch, sources_ptr, from_ptr, to_ptr, rows_ptr):
         """Opens a fork: request b begins as a copy of sources[b] (negative: not);
         the rows to copy go to from / to / rows ([requests])."""
-        self._check(self.lib.pcl_page_fork(
-            self.handle, ctypes.byref(batch), sources_ptr,
-            from_ptr, to_ptr, rows_ptr))
+        self._check(self.lib.pcl_page_fork(self.handle, ctypes.byref(batch), sources_ptr,
+                                           from_ptr, to_ptr, rows_ptr))
 
     def page_release_shared(self, batch, finished_ptr):
         """Requests with a nonzero flag give back the pages that nobody else
@@ -645,8 +643,8 @@ class Context:
         PclPagePools): lists of entries in order, or, with rows, runs."""
         array = (PclPagePools * len(pools))(*pools)
         self._check(self.lib.pcl_paged_copy(
-            self.handle, array, len(pools), from_ptr, to_ptr,
-            rows_ptr, int(lists), int(entries)))
+            self.handle, array, len(pools), from_ptr, to_ptr, rows_ptr, int(lists),
+            int(entries)))
 
     @staticmethod
     def paged_tree_desc(**kw):

@@ -12,7 +12,12 @@
 //   pages j < L_s div P, and a page of its own for the L_s mod P tokens behind;
 //   pages that go back: those of the finished requests' tables that no other
 //   request's holds.
-// All are short calls, bound by their chains of dependent loads and by the launch.
+// All but the copies are short, bound by their chains of dependent loads and by the
+// launch (MI355X): masks of 16 trees of 12 and of 256 of 64, 3.2 and 3.6 us; accepted
+// branches 3.2; a fork 4.6 (8 from 4 of up to 512 tokens) and 6.2 (480 from 16 of up to
+// 8192); a release 9.1 in one workgroup, 2.2 + 4.4 + 4.4 of its three launches. Copies
+// of 192 part-filled pages of three layers, 402 MB read and written, 89 us (4.5 TB/s; a
+// plain copy of 4 GiB 4.7), of 64 branches of up to 5 rows in six layers 6.2 us.
 #include "context.hpp"
 #include "page_batch.hpp"
 #include "paged.hpp"

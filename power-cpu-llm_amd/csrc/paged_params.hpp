@@ -164,7 +164,11 @@ hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hip
 constexpr int64_t kFewRows = 8;
 // Whether units of `unit` rows leave a tree launch at most an item per CU, each with a
 // CU to itself; `whole`: the head dim is one that needs no padding. `items`: at one
-// unit, `rows`: of a KV head that one request has at most.
+// unit, `rows`: of a KV head that one request has at most. Such launches split their
+// rows over more workgroups of paged_kv.hpp (one request of 8 new tokens behind 1000
+// keys, f32: 21 us and 26 in units of sixteen rows at 16 x 8 x 256 heads, 29 and 54 at
+// 16 x 2 x 512, 21 and 27 at 32 x 8 x 128, both 23 at 16 x 4 x 64; of 40 behind 500: 26
+// and 45, 36 and 57, both 43, 31 and 37).
 bool few_items(bool whole, int64_t items, int64_t rows, int64_t unit);
 // Whether such a launch takes the kernels of many rows (paged_rows.hpp).
 bool many_rows(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows);

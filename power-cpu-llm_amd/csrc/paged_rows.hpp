@@ -1,12 +1,40 @@
 // Attention of a step's new tokens over a paged KV cache where a KV head has more
 // than eight query rows: units of 16 U rows, 256-key chunks, on 16 x 16 x 4 f32 MFMAs.
 //
-// The mathematics and the arithmetic are those of paged_kv.hpp and its tree
-// launches. Four waves score 64 keys each against all the unit's rows and leave the
-// probabilities in LDS; then each runs the P.V chains of a quarter of the dims over
-// the whole chunk. So each byte of K and V is read from LDS once, by one wave, and
-// feeds U instructions of 16 rows; a lane of the result is a row, and a tile's
-// maximum and sum take two exchanges between lanes (a lane a key takes five).
+// For new token i of request b (L held tokens, row r), query head h of KV head kh:
+//   s_t = cap(q_scale * q[r][h] . K[slot_t][kh])  over the keys t that it attends,
+//   out[r][h] = sum_t exp(s_t - max s) V[slot_t][kh] / sum_t exp(s_t - max s),
+// keys [0, L + i], or with masks [0, L) and L + j for each bit j; in a window those
+// less than `window` positions before it. The arithmetic is that of paged_kv.hpp.
+//
+// Eight waves (four below head dim 256) score 32 keys (64) each against all the
+// unit's rows and leave the probabilities in LDS; then each runs the P.V chains of its
+// share of the dims over the whole chunk. So each byte of K and V is read from LDS
+// once, by one wave, and feeds U instructions of 16 rows; a lane of the result is a
+// row, and a tile's maximum and sum take two exchanges between lanes (a lane a key, as
+// in paged_kv.hpp, takes five). The probabilities of all waves meet in LDS: three
+// barriers a chunk.
+//
+// Bound by the matrix instructions and the phases between them (MI355X, cold inputs; a
+// call with its plan and merge, this kernel in brackets, and the multiply-adds of
+// whole units at 154 TFLOP/s, which a large f32 product of the library reaches):
+//   64 trees of up to 8 over up to 8192 keys, 16 x 8 x 256 heads, bf16, 0.86 GB: 248 us
+//     (223; 96), matrix pipes 45 % busy; 220 us where all pages are the same one;
+//   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 194 us (177; 106);
+//   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 882 us (830; 537);
+//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 173 us (155;
+//     62);
+//   4 prompt parts of up to 512 over up to 8192 keys, 16 x 8 x 256, bf16: 1.86 ms (1.75;
+//     1.16).
+// Of a chunk at 48 rows the scores take 43 % (83 % of it matrix instructions), the
+// softmax 10 %, P.V 45 % (79 %) and the output 2 %.
+//
+// How it came there (the first, fourth and last case): units of 16 rows on 4 x 4 x 1
+// MFMAs 298, - and 3164 us; 16 x 16 x 4 on four waves 227, 180 and 2385 us; eight waves,
+// with which two workgroups have a CU's registers at one 16 of rows, and the query
+// copied into LDS as it is, 222, 168 and 2054 us; a chunk's softmax from one read of
+// its maxima and items as workgroups come to them 237, 170 and 1881 us with their plan;
+// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us).
 #pragma once
 
 #include "paged_kv.hpp"
@@ -14,7 +42,7 @@
 namespace pcl {
 
 // Eight waves of 32 keys at head dims 256 and 512, four of 64 below (a wave's part of
-// a V row is 16 dims at least). Units of the ring are a 128-byte line of the wave's K
+// a V row is 16 dims at least; four waves at 256 took 2385 us for the prompt parts). Units of the ring are a 128-byte line of the wave's K
 // rows or its dims of some V rows.
 template <int DK, typename T, int U> struct RowsCfg {
     static constexpr int NW = DK >= 256 ? 8 : 4;
@@ -394,9 +422,11 @@ __device__ __forceinline__ TreeItem chunk_item(const PlanItem &i, int k)
     return x;
 }
 
+// Four waves a SIMD, two workgroups a CU, where one 16 of rows leaves room for them
+// (128 registers; 64 trees of bf16 219 us, 254 us at the 148 that the compiler took).
 template <int DK, typename T, bool FULL, int U, int NB>
 __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
-                             (DK == 256 && U == 1 ? 4 : 2)) void paged_rows_kernel(TreeParams p)
+                             (DK == 256 && U == 1 ? 4 : 2)) void tree_rows_kernel(TreeParams p)
 {
     using C = RowsCfg<DK, T, U>;
     constexpr int NW = C::NW, KW = C::KW, TW = C::TW, UK = C::UK, VL = C::VL, SU = C::SU;
@@ -481,8 +511,9 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         f.page = p.table[x.b * p.table_stride + divided(position(x), p.by_page_tokens)];
         fetch_rows(p, x, k0, f.tree);
     };
-    // The unit's query rows into LDS: a copy is four of the eight dims of a lane, for 16 rows and 32 dims. Rows
-    // past the last are the last one's, dims past the head dim the first ones.
+    // The unit's query rows into LDS: a copy is four of the eight dims of a lane, for 16
+    // rows and 32 dims. Rows past the last are the last one's, dims past the head dim
+    // the first ones.
     auto issue_q = [&](const TreeItem &x) {
         const float *row[U];
 #pragma unroll
@@ -1026,7 +1057,7 @@ template <int DK, int U, int NB> constexpr size_t rows_lds_bytes()
 // Workgroups that a CU holds at once, asked once per device.
 template <int DK, typename T, bool FULL, int U, int NB> static hipError_t resident_rows(int *groups)
 {
-    const auto kernel = (const void *)paged_rows_kernel<DK, T, FULL, U, NB>;
+    const auto kernel = (const void *)tree_rows_kernel<DK, T, FULL, U, NB>;
     static std::atomic<int> known[kMaxDevices];
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -1064,17 +1095,21 @@ static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks,
     const int64_t plans = std::min<int64_t>((items + kPlanThreads - 1) / kPlanThreads, 256);
     paged_plan_kernel<16 * U>
         <<<(unsigned)plans, kPlanThreads, plan_words_bytes(p.requests), stream>>>(p, (int)grid);
-    paged_rows_kernel<DK, T, FULL, U, NB>
+    tree_rows_kernel<DK, T, FULL, U, NB>
         <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, U, NB>(), stream>>>(p);
     return hipGetLastError();
 }
 
-// Rows of 16 of the largest unit: what the LDS of a CU holds beside the rings.
+// 16s of rows of the largest unit: what the LDS of a CU holds beside the rings. Units
+// of two 16s instead of three at head dim 256, with two buffers of the ring: prompt
+// parts 2250 us (2064).
 constexpr int most_groups(int dk)
 {
     return dk == 512 ? 2 : dk == 256 ? 3 : 4;
 }
 
+// The smallest unit that holds a request's rows, so that no matrix instruction runs on
+// rows that none has.
 template <int DK, typename T, bool FULL>
 static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {

@@ -289,11 +289,11 @@ def test_workspace_holds_every_chunk_of_every_row(pcl):
 
 @pytest.mark.parametrize("source,kernel", [
     ("paged_tree_d256.hip", "_ZN3pcl17paged_tree_kernelILi256EfLb1ELi1ELi1EEEvNS_10TreeParamsE"),
-    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EfLb1ELi1ELi1EEEvNS_10TreeParamsE"),
-    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EDF16bLb1ELi1ELi1EEEvNS_10TreeParamsE"),
-    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EfLb1ELi3ELi1EEEvNS_10TreeParamsE"),
-    ("paged_rows_d256.hip", "_ZN3pcl17paged_rows_kernelILi256EDF16bLb1ELi3ELi1EEEvNS_10TreeParamsE"),
-    ("paged_rows_d512.hip", "_ZN3pcl17paged_rows_kernelILi512EfLb1ELi2ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl16tree_rows_kernelILi256EfLb1ELi1ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl16tree_rows_kernelILi256EDF16bLb1ELi1ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl16tree_rows_kernelILi256EfLb1ELi3ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d256.hip", "_ZN3pcl16tree_rows_kernelILi256EDF16bLb1ELi3ELi1EEEvNS_10TreeParamsE"),
+    ("paged_rows_d512.hip", "_ZN3pcl16tree_rows_kernelILi512EfLb1ELi2ELi1EEEvNS_10TreeParamsE"),
     ("paged_tree.hip",
      "_ZN3pcl19tree_combine_kernelILi8EEEvNS_10TreeParamsENS_12CombineShapeE"),
 ])
