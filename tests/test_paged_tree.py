@@ -1341,6 +1341,46 @@ def test_spans_as_items(pcl, torch, ctx, heads, dtype, held, counts, window, tre
 
 
 @pytest.mark.gpu
+def test_replays_over_other_requests(pcl, torch):
+    # one capture, each replay with other requests taking part: launches whose spans are
+    # items and launches of single chunks, in turn, on a stream of their own
+    heads, held, counts = (16, 8, 256), [9000, 500, 15000, 40], [400, 70, 300, 9]
+    stream = torch.cuda.Stream()
+    cache = TreeCache(pcl, torch, heads, held, counts, 16, "bf16", 31)
+    q = cache.queries()
+    out = torch.full_like(q, 9.5)
+    newest = cache.newest.clone()
+    torch.cuda.synchronize()
+    own = pcl.Context(0, stream.cuda_stream)
+    d = cache.tree_desc(own, q, out)
+    own.reserve(own.paged_tree_workspace_bytes(d))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        own.paged_tree_attention(d)
+    eager = pcl.Context(0)
+    whole = cache.tree_attend(eager, q)
+    cache.check(eager, q, whole, exact=False)
+    for taking in ([0, 1, 2, 3], [1, 3], [2], [], [0, 2], [3]):
+        cache.newest.fill_(-1)
+        cache.newest[taking] = newest[taking]
+        out.fill_(9.5)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.full_like(q, 9.5)
+        for b in taking:
+            mine = slice(cache.first[b], cache.first[b] + counts[b])
+            want[mine] = whole[mine]
+        assert np.array_equal(bits(out), bits(want)), taking
+        assert np.array_equal(bits(cache.tree_attend(eager, q)), bits(want)), taking
+    assert [c.sync() for c in (own, eager)] == [0, 0]
+    graph.reset()
+    own.close()
+    eager.close()
+
+
+@pytest.mark.gpu
 def test_prompts_beside_single_tokens(pcl, torch, ctx):
     # one launch with requests of one new token and of many
     held, counts = [700, 0, 33, 1500, 260, 90], [1, 400, 2, 1, 150, 17]
