@@ -22,7 +22,7 @@
 //     (223; 96), matrix pipes 45 % busy; 220 us where all pages are the same one;
 //   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 194 us (177; 106);
 //   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 882 us (830; 537);
-//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 173 us (155;
+//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 165 us (147;
 //     62);
 //   4 prompt parts of up to 512 over up to 8192 keys, 16 x 8 x 256, bf16: 1.86 ms (1.75;
 //     1.16).
@@ -34,12 +34,31 @@
 // with which two workgroups have a CU's registers at one 16 of rows, and the query
 // copied into LDS as it is, 222, 168 and 2054 us; a chunk's softmax from one read of
 // its maxima and items as workgroups come to them 237, 170 and 1881 us with their plan;
-// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us).
+// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us), half lines
+// of K up to head dim 128 165 us.
 #pragma once
 
 #include "paged_kv.hpp"
 
 namespace pcl {
+
+// Units of the ring that a wave's part of a K line comes in, and units that the ring
+// holds. Up to head dim 128 a wave has 64 keys: a unit is 32 of them, so that fewer
+// registers hold a unit's values (64 rows spilled 157 of them with whole lines, 74 with
+// halves), and a ring of three keeps more copies in flight at 128 (256 chains of up to 4,
+// 16 rows, 173 us with whole lines, 165 with halves; prompt parts of 512 tokens at 32 x 8
+// x 128, bf16, 2237 us with two halves, 2129 with three; at 64 as fast, and 32 rows have
+// two workgroups a CU with two). Above, halves cost more than they bring (window trees
+// 194 -> 210 us, prompt parts 1857 -> 1925 us with three of them).
+constexpr int rows_parts(int dk)
+{
+    return dk <= 128 ? 2 : 1;
+}
+
+constexpr int rows_buffers(int dk)
+{
+    return dk == 128 ? 3 : rows_parts(dk);
+}
 
 // Eight waves of 32 keys at head dims 256 and 512, four of 64 below (a wave's part of
 // a V row is 16 dims at least; four waves at 256 took 2385 us for the prompt parts). Units of the ring are a 128-byte line of the wave's K
@@ -50,11 +69,14 @@ template <int DK, typename T, int U> struct RowsCfg {
     static constexpr int kRowsUnit = 16 * U;
     static constexpr int KW = kChunk / NW;             // keys of a wave
     static constexpr int TW = KW / kTile;              // tiles of them
-    static constexpr int kUnit = 128 * KW;             // bytes of a ring unit
+    static constexpr int kParts = rows_parts(DK);      // K units of a line
+    static constexpr int BU = KW / 16 / kParts;        // 16-key blocks of one
+    static constexpr int kUnit = 128 * 16 * BU;        // bytes of a ring unit
     static constexpr int NE = kUnit / 1024;            // copies of one
     static constexpr int kLine = 128 / (int)sizeof(T); // dims of a K unit
-    static constexpr int UK = (DK + kLine - 1) / kLine; // K units
-    static constexpr int SU = kLine / 32;              // score chain steps (32 dims) of a unit
+    static constexpr int kLines = (DK + kLine - 1) / kLine;
+    static constexpr int UK = kLines * kParts; // K units
+    static constexpr int SU = kLine / 32;      // score chain steps (32 dims) of a unit
     static constexpr int VL = DK / 16 / NW;            // 16-dim blocks of a wave's dims
     static constexpr int kRowV = 16 * VL * (int)sizeof(T); // bytes of a V row of the wave
     static constexpr int kLanesV = kRowV / 16;         // lanes that copy it
@@ -74,10 +96,12 @@ template <int DK, int U> struct RowsLds {
     uint32_t taken;                       // the item behind the next one
 };
 
-// The rings of all waves.
-constexpr size_t rows_ring_bytes(int buffers)
+// The LDS of a CU, less the kernel's static words.
+constexpr size_t kRowsLds = 160 * 1024 - 64;
+
+template <int DK, typename T, int U, int NB> constexpr size_t rows_lds_bytes()
 {
-    return (size_t)buffers * 128 * kChunk;
+    return sizeof(RowsLds<DK, U>) + (size_t)NB * RowsCfg<DK, T, U>::kUnit * RowsCfg<DK, T, U>::NW;
 }
 
 // What a lane requests of an item's trees: of its row in each 16 of the unit's the
@@ -584,10 +608,10 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         const char *from[C::NE];
     };
     const int piece = (lane % 8 ^ lane / 8) * (16 / (int)sizeof(T));
-    auto rows_k = [&](const int32_t *slots, int kh) {
+    auto rows_k = [&](const int32_t *slots, int kh, int part) {
         const char *base =
             static_cast<const char *>(p.k) + ((int64_t)kh * p.dim + piece) * sizeof(T);
-        const int32_t *mine = slots + k0 + lane / 8;
+        const int32_t *mine = slots + k0 + 16 * C::BU * part + lane / 8;
         Sources c;
 #pragma unroll
         for (int e = 0; e < C::NE; ++e)
@@ -642,10 +666,9 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
     __syncthreads();
     next = taken_item();
     {
-        const Sources rows = rows_k(s.slots[0], x.kh);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            issue(line_k(rows, i));
+            issue(line_k(rows_k(s.slots[0], x.kh, i % C::kParts), i / C::kParts));
             next_buffer();
         }
     }
@@ -682,10 +705,20 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
 #pragma unroll
             for (int b = 0; b < 2 * TW; ++b)
                 acc[rg][b] = f4{0.f, 0.f, 0.f, 0.f};
-        const Sources rows = rows_k(s.slots[buf], x.kh);
-        Sources c = NB < UK ? line_k(rows, NB) : sources_v(s.slots[buf], x.kh, t0, t1, NB - UK);
+        Sources rows[C::kParts];
+#pragma unroll
+        for (int part = 0; part < C::kParts; ++part)
+            rows[part] = rows_k(s.slots[buf], x.kh, part);
+        // the unit n units behind line `line`'s first
+        auto unit_behind = [&](int line, auto nc) {
+            constexpr int n = decltype(nc)::value;
+            const int i = line + n / C::kParts;
+            return i < C::kLines ? line_k(rows[n % C::kParts], i)
+                                 : sources_v(s.slots[buf], x.kh, t0, t1, line * C::kParts + n - UK);
+        };
+        Sources c = unit_behind(0, std::integral_constant<int, NB>{});
 #pragma unroll 1
-        for (int i = 0; i < UK; ++i) {
+        for (int i = 0; i < C::kLines; ++i) {
             f4 q[U][SU][2]; // read ahead of the wait
 #pragma unroll
             for (int rg = 0; rg < U; ++rg)
@@ -696,58 +729,62 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
                         const int n = min(SU * i + u, DK / 32 - 1);
                         q[rg][u][hh] = s.q[rg][n][hh][lane];
                     }
-            wait_unit();
-            u4 kw[2 * TW][2];
+            pcl::each<C::kParts>([&](auto pc) {
+                constexpr int part = decltype(pc)::value;
+                wait_unit();
+                u4 kw[C::BU][2];
 #pragma unroll
-            for (int b = 0; b < 2 * TW; ++b)
+                for (int b = 0; b < C::BU; ++b)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    // f32: halves of a lane's eight dims; bf16: the eight of two steps
-                    const int j = sizeof(T) == 4 ? 2 * g + h : 4 * h + g;
-                    const int d = C::kLine * i + j * (16 / (int)sizeof(T));
-                    u4 v = *(const u4 *)(ring + at * kWords + 32 * (16 * b + col) +
-                                         4 * (j ^ (col & 7)));
-                    if (!FULL && d >= p.dim)
-                        v = u4{0u, 0u, 0u, 0u};
-                    kw[b][h] = v;
-                }
-            free_unit();
-            issue(c);
-            next_buffer();
-            if (i + 1 < UK)
-                c = i + 1 + NB < UK ? line_k(rows, i + 1 + NB)
-                                    : sources_v(s.slots[buf], x.kh, t0, t1, i + 1 + NB - UK);
-            if (!mine)
-                continue;
-            // (bf16: widened once for all rows)
-            float k[SU][2 * TW][8];
-#pragma unroll
-            for (int u = 0; u < SU; ++u)
-#pragma unroll
-                for (int b = 0; b < 2 * TW; ++b)
-#pragma unroll
-                    for (int jj = 0; jj < 8; ++jj) {
-                        if constexpr (sizeof(T) == 4)
-                            k[u][b][jj] = __uint_as_float(kw[b][jj / 4][jj % 4]);
-                        else
-                            k[u][b][jj] = jj % 2 ? bf16_high(kw[b][u][jj / 2])
-                                                 : bf16_low(kw[b][u][jj / 2]);
+                    for (int h = 0; h < 2; ++h) {
+                        // f32: halves of a lane's eight dims; bf16: the eight of two steps
+                        const int j = sizeof(T) == 4 ? 2 * g + h : 4 * h + g;
+                        const int d = C::kLine * i + j * (16 / (int)sizeof(T));
+                        u4 v = *(const u4 *)(ring + at * kWords + 32 * (16 * b + col) +
+                                             4 * (j ^ (col & 7)));
+                        if (!FULL && d >= p.dim)
+                            v = u4{0u, 0u, 0u, 0u};
+                        kw[b][h] = v;
                     }
+                free_unit();
+                issue(c);
+                next_buffer();
+                if (part + 1 < C::kParts || i + 1 < C::kLines)
+                    c = unit_behind(i, std::integral_constant<int, part + 1 + NB>{});
+                if (!mine)
+                    return;
+                // (bf16: widened once for all rows)
+                float k[SU][C::BU][8];
 #pragma unroll
-            for (int rg = 0; rg < U; ++rg) {
-                if (rg >= groups)
-                    continue;
+                for (int u = 0; u < SU; ++u)
 #pragma unroll
-                for (int u = 0; u < SU; ++u) {
-                    if (SU * i + u >= DK / 32)
+                    for (int b = 0; b < C::BU; ++b)
+#pragma unroll
+                        for (int jj = 0; jj < 8; ++jj) {
+                            if constexpr (sizeof(T) == 4)
+                                k[u][b][jj] = __uint_as_float(kw[b][jj / 4][jj % 4]);
+                            else
+                                k[u][b][jj] = jj % 2 ? bf16_high(kw[b][u][jj / 2])
+                                                     : bf16_low(kw[b][u][jj / 2]);
+                        }
+#pragma unroll
+                for (int rg = 0; rg < U; ++rg) {
+                    if (rg >= groups)
                         continue;
 #pragma unroll
-                    for (int jj = 0; jj < 8; ++jj)
+                    for (int u = 0; u < SU; ++u) {
+                        if (SU * i + u >= DK / 32)
+                            continue;
 #pragma unroll
-                        for (int b = 0; b < 2 * TW; ++b)
-                            acc[rg][b] = mfma(k[u][b][jj], q[rg][u][jj / 4][jj % 4], acc[rg][b]);
+                        for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+                            for (int b = 0; b < C::BU; ++b)
+                                acc[rg][C::BU * part + b] =
+                                    mfma(k[u][b][jj], q[rg][u][jj / 4][jj % 4],
+                                         acc[rg][C::BU * part + b]);
+                    }
                 }
-            }
+            });
         }
 
         // `whole`: every row of the unit attends all of the wave's keys, as mostly
@@ -869,7 +906,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         auto behind_v = [&](int i) {
             const int n = i + NB - rounds; // the next item's first units follow this one's
             return n < 0 ? sources_v(s.slots[buf], x.kh, t0, t1, i + NB)
-                         : line_k(rows_k(s.slots[behind], y.kh), n);
+                         : line_k(rows_k(s.slots[behind], y.kh, n % C::kParts), n / C::kParts);
         };
         c = behind_v(0);
         // The probabilities and factors of the 16 keys behind n of the tiles' from t0 on,
@@ -1046,14 +1083,6 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
 }
 
-// The LDS of a CU, less the kernel's static words.
-constexpr size_t kRowsLds = 160 * 1024 - 64;
-
-template <int DK, int U, int NB> constexpr size_t rows_lds_bytes()
-{
-    return sizeof(RowsLds<DK, U>) + rows_ring_bytes(NB);
-}
-
 // Workgroups that a CU holds at once, asked once per device.
 template <int DK, typename T, bool FULL, int U, int NB> static hipError_t resident_rows(int *groups)
 {
@@ -1068,7 +1097,7 @@ template <int DK, typename T, bool FULL, int U, int NB> static hipError_t reside
     *groups = known[dev].load(std::memory_order_acquire);
     if (*groups > 0)
         return hipSuccess;
-    constexpr size_t bytes = rows_lds_bytes<DK, U, NB>();
+    constexpr size_t bytes = rows_lds_bytes<DK, T, U, NB>();
     static_assert(bytes <= kRowsLds, "the LDS of a CU");
     e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == hipSuccess)
@@ -1081,9 +1110,10 @@ template <int DK, typename T, bool FULL, int U, int NB> static hipError_t reside
     return hipSuccess;
 }
 
-template <int DK, typename T, bool FULL, int U, int NB>
+template <int DK, typename T, bool FULL, int U>
 static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
+    constexpr int NB = rows_buffers(DK);
     int groups = 0;
     const hipError_t e = resident_rows<DK, T, FULL, U, NB>(&groups);
     if (e != hipSuccess)
@@ -1096,26 +1126,33 @@ static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks,
     paged_plan_kernel<16 * U>
         <<<(unsigned)plans, kPlanThreads, plan_words_bytes(p.requests), stream>>>(p, (int)grid);
     tree_rows_kernel<DK, T, FULL, U, NB>
-        <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, U, NB>(), stream>>>(p);
+        <<<(unsigned)grid, RowsCfg<DK, T, U>::kThreads, rows_lds_bytes<DK, T, U, NB>(), stream>>>(p);
     return hipGetLastError();
 }
 
-// 16s of rows of the largest unit: what the LDS of a CU holds beside the rings. Units
-// of two 16s instead of three at head dim 256, with two buffers of the ring: prompt
-// parts 2250 us (2064).
+// 16s of rows of the largest unit: what the LDS of a CU holds beside the rings (512),
+// and what its registers do (four at head dim 128 spilled 43 to 157 of them: prompt parts
+// 2290 us, 2146 with three; trees of 12 at 32 x 8 x 128, f32, 513 and 385 us). Units of two
+// instead of three at head dim 256, with two buffers: prompt parts 2250 us (2064).
 constexpr int most_groups(int dk)
 {
-    return dk == 512 ? 2 : dk == 256 ? 3 : 4;
+    return dk == 512 ? 2 : 3;
 }
 
-// The smallest unit that holds a request's rows, so that no matrix instruction runs on
-// rows that none has.
+// The fewest units that hold a request's rows, and the smallest such units: no matrix
+// instruction runs on rows that none has (64 trees of 16 at 32 x 8 x 128, 64 rows in two
+// units of 32: 577 us; as 48 and 16: 759 us).
 template <int DK, typename T, bool FULL>
 static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
 {
-    return rows <= 16   ? launch_rows<DK, T, FULL, 1, 1>(p, rows, chunks, stream)
-           : rows <= 32 ? launch_rows<DK, T, FULL, 2, 1>(p, rows, chunks, stream)
-                        : launch_rows<DK, T, FULL, most_groups(DK), 1>(p, rows, chunks, stream);
+    constexpr int most = 16 * most_groups(DK);
+    const int64_t units = (rows + most - 1) / most, unit = (rows + units - 1) / units;
+    if constexpr (most_groups(DK) > 2) {
+        if (unit > 32)
+            return launch_rows<DK, T, FULL, 3>(p, rows, chunks, stream);
+    }
+    return unit > 16 ? launch_rows<DK, T, FULL, 2>(p, rows, chunks, stream)
+                     : launch_rows<DK, T, FULL, 1>(p, rows, chunks, stream);
 }
 
 template <int DK>
