@@ -18,11 +18,11 @@
 // Bound by the matrix instructions and the phases between them (MI355X, cold inputs; a
 // call with its plan and merge, this kernel in brackets, and the multiply-adds of
 // whole units at 154 TFLOP/s, which a large f32 product of the library reaches):
-//   64 trees of up to 8 over up to 8192 keys, 16 x 8 x 256 heads, bf16, 0.86 GB: 248 us
-//     (223; 96), matrix pipes 45 % busy; 220 us where all pages are the same one;
-//   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 194 us (177; 106);
+//   64 trees of up to 8 over up to 8192 keys, 16 x 8 x 256 heads, bf16, 0.86 GB: 245 us
+//     (222; 96), matrix pipes 45 % busy; 220 us where all pages are the same one;
+//   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 193 us (177; 106);
 //   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 882 us (830; 537);
-//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 165 us (147;
+//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 162 us (147;
 //     62);
 //   4 prompt parts of up to 512 over up to 8192 keys, 16 x 8 x 256, bf16: 1.86 ms (1.75;
 //     1.16).
@@ -35,7 +35,8 @@
 // copied into LDS as it is, 222, 168 and 2054 us; a chunk's softmax from one read of
 // its maxima and items as workgroups come to them 237, 170 and 1881 us with their plan;
 // whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us), half lines
-// of K up to head dim 128 165 us.
+// of K up to head dim 128 165 us; an item's claim and the next chunk's words behind the
+// scores 245 and 162 us.
 #pragma once
 
 #include "paged_kv.hpp"
@@ -476,7 +477,8 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
     const bool uneven = parts == 8 && (*plan)[1] != 0;
     uint32_t part = blockIdx.x % parts; // (by thread 0, as what follows)
     auto place = [&](uint32_t n) { return n / each * gridDim.x + part * each + n % each; };
-    auto take = [&]() { return place((uint32_t)atomicAdd(&p.plan->taken[part], 1)); };
+    auto claim = [&]() { return (uint32_t)atomicAdd(&p.plan->taken[part], 1); };
+    auto take = [&]() { return place(claim()); };
     auto settle = [&](uint32_t n) { // n, or another XCD's item where that is past the last
         if (n < items || !uneven)
             return n;
@@ -680,16 +682,10 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         const bool last_chunk = chunk + 1 == now.chunks;
         const bool more = !last_chunk || next.chunks > 0;
         const bool new_q = last_chunk && more;
-        uint32_t behind_next = 0; // (its atomic returns during the products)
-        if (new_q && tid == 0)
-            behind_next = take();
         // (without a next chunk this one's first units are copied again, and not used)
         TreeItem y = x;
-        Fetched f;
-        if (more) {
+        if (more)
             y = last_chunk ? chunk_item(next, 0) : chunk_item(now, chunk + 1);
-            fetch(y, f);
-        }
         const int behind = more ? buf ^ 1 : buf; // the next chunk's slots
 #pragma unroll
         for (int rg = 0; rg < U; ++rg)
@@ -786,6 +782,15 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
                 }
             });
         }
+
+        // The claim of an item and the next chunk's words return during the softmax and
+        // P.V: ahead of the scores the first wait for a unit's copies waits for them too.
+        uint32_t behind_next = 0;
+        if (new_q && tid == 0)
+            behind_next = claim();
+        Fetched f;
+        if (more)
+            fetch(y, f);
 
         // `whole`: every row of the unit attends all of the wave's keys, as mostly
         uint64_t seen = ~(uint64_t)0;
@@ -884,8 +889,6 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
             probabilities(std::true_type{});
         else
             probabilities(std::false_type{});
-        if (new_q && tid == 0)
-            s.taken = settle(behind_next);
         if (more)
             store(y, f, buf ^ 1);
         lds_barrier(); // probabilities, row sums and factors
@@ -1070,6 +1073,8 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
             atomicOr(p.err, kErrOutput);
         if (!more)
             break;
+        if (new_q && tid == 0)
+            s.taken = settle(place(behind_next));
         lds_barrier(); // the next query
         x = y;
         ++chunk;
