@@ -15,7 +15,7 @@
 // All but the copies are short, bound by their chains of dependent loads and by the
 // launch (MI355X): masks of 16 trees of 12 and of 256 of 64, 3.2 and 3.6 us; accepted
 // branches 3.2; a fork 4.6 (8 from 4 of up to 512 tokens) and 6.2 (480 from 16 of up to
-// 8192); a release 9.1 in one workgroup, 2.2 + 4.4 + 4.4 of its three launches. Copies
+// 8192); a release 8.0 in one workgroup, 2.2 + 4.4 + 4.4 of its three launches. Copies
 // of 192 part-filled pages of three layers, 402 MB read and written, 89 us (4.5 TB/s; a
 // plain copy of 4 GiB 4.7), of 64 branches of up to 5 rows in six layers 6.2 us.
 #include "context.hpp"
@@ -357,20 +357,55 @@ constexpr int kReleaseThreads = 1024;
 // Pages (a bit each) and table entries of a release by one workgroup.
 constexpr int kReleaseBits = 1 << 17, kReleaseEntries = 1 << 14;
 
-// Small batches: one workgroup, the marks as bits in LDS.
+// Small batches: one workgroup, the marks as bits in LDS. The requests' words are read
+// at once, then a wave takes the tables of kReleaseAhead requests at a time, so that
+// their loads do not wait for each other's (8 forks of 4 prompts of up to 512 tokens: 8.0
+// us, 8.9 with a table after another).
+constexpr int kReleaseAhead = 4;
+
 __global__ __launch_bounds__(kReleaseThreads) void release_small_kernel(PageParams p)
 {
-    extern __shared__ uint32_t marks[]; // [2][groups]
-    __shared__ uint32_t waves[kReleaseThreads / 64];
-    const int groups = (p.pages + 31) / 32;
+    constexpr int kWaves = kReleaseThreads / 64;
+    extern __shared__ uint32_t marks[]; // [2][groups], and [requests] pages, gone in bit 31
+    __shared__ uint32_t waves[kWaves];
+    const int groups = (p.pages + 31) / 32, lane = threadIdx.x & 63;
+    uint32_t *const held = marks + 2 * groups;
+    bool bad = false;
+    for (int i = threadIdx.x; i < p.requests; i += kReleaseThreads) {
+        const uint32_t len = held_tokens(p, p.lengths, i);
+        bad |= len == ~0u;
+        held[i] = (len == ~0u ? 0 : pages_of(len, p.page_tokens)) | (p.in[i] ? 1u << 31 : 0);
+    }
     for (int i = threadIdx.x; i < 2 * groups; i += kReleaseThreads)
         marks[i] = 0;
     __syncthreads();
-    bool bad = false;
-    for (int b = threadIdx.x >> 6; b < p.requests; b += kReleaseThreads / 64)
-        bad |= mark_pages(p, b, threadIdx.x & 63, 64, [&](int page, bool gone) {
+    auto mark = [&](int32_t page, bool gone) { // (a page that stays is not looked at)
+        if (in_pools(p, page))
             atomicOr(&marks[(gone ? 0 : groups) + page / 32], 1u << (page % 32));
-        });
+        else
+            bad |= gone;
+    };
+    for (int b0 = threadIdx.x >> 6; b0 < p.requests; b0 += kReleaseAhead * kWaves) {
+        uint32_t words[kReleaseAhead];
+        int32_t page[kReleaseAhead];
+#pragma unroll
+        for (int u = 0; u < kReleaseAhead; ++u) {
+            const int b = b0 + u * kWaves;
+            words[u] = b < p.requests ? held[b] : 0;
+            page[u] = 0;
+            if (lane < (int)(words[u] & ~(1u << 31)))
+                page[u] = p.table[b * p.table_stride + lane];
+        }
+#pragma unroll
+        for (int u = 0; u < kReleaseAhead; ++u) {
+            const int pages = (int)(words[u] & ~(1u << 31));
+            const bool gone = words[u] >> 31;
+            if (lane < pages)
+                mark(page[u], gone);
+            for (int c = 64 + lane; c < pages; c += 64)
+                mark(p.table[(b0 + u * kWaves) * p.table_stride + c], gone);
+        }
+    }
     __syncthreads();
     give_back<kReleaseThreads>(
         p, bad, groups, waves, [&](int page) { return marks[page / 32] >> (page % 32) & 1; },
@@ -628,7 +663,8 @@ int pcl_page_release_shared(pcl_context *ctx, const pcl_page_batch *batch, const
         return PCL_INVALID_SHAPE;
     r.b.in = finished;
     if (release_is_small(batch)) {
-        const size_t lds = 2 * (size_t)((batch->pages + 31) / 32) * sizeof(uint32_t);
+        const size_t lds =
+            (2 * (size_t)((batch->pages + 31) / 32) + batch->requests) * sizeof(uint32_t);
         pcl::release_small_kernel<<<1, pcl::kReleaseThreads, lds, ctx->stream>>>(r.b);
         return pcl::page_launched("shared release");
     }
