@@ -221,10 +221,11 @@ __device__ __forceinline__ uint32_t or_rows(uint32_t x)
 // items of a chunk each, which come last and fill what the spans leave uneven: with T
 // chunks in all, W workgroups and no span longer than s chunks, the spans are the first
 // W (where T >= s W) and those that begin in the first T - s W chunks. With the combine,
-// against a chunk each (MI355X): trees of 12 tokens behind up to 32K keys of d512 (T = 25
-// W) 0.97 ms and 1.16 ms, prompt parts of 512 tokens (T = 60 W) 1.84 ms and 1.97 ms. (W
-// floor(T / (s W)) spans left XCDs unevenly loaded: 2.01 ms; spans in the first T - s W /
-// 2 chunks as well, and 257 us instead of 194 for windows of T = 4 W.)
+// against a chunk each (MI355X): trees of 12 tokens behind up to 32K keys of d512 (T = 19
+// W) 0.89 and 0.99 ms, prompt parts of 512 tokens (T = 55 W) 1.86 and 1.91 ms, at 32 x 8 x
+// 128 2.13 and 2.35 ms. (W floor(T / (s W)) spans left workgroups unevenly loaded: 2.01
+// ms; spans in the first T - s W / 2 chunks as well, 2.03 ms, and 257 us instead of 194
+// for windows of T = 5 W; in the first T - 2 s W 1.83 and 2.20 ms.)
 constexpr int kPlanThreads = 256;
 
 // The requests' words: items of spans and of chunks before each (over the KV heads),
