@@ -21,7 +21,7 @@
 //   64 trees of up to 8 over up to 8192 keys, 16 x 8 x 256 heads, bf16, 0.86 GB: 245 us
 //     (222; 96), matrix pipes 45 % busy; 220 us where all pages are the same one;
 //   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 193 us (177; 106);
-//   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 882 us (830; 537);
+//   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 890 us (840; 537);
 //   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 162 us (147;
 //     62);
 //   4 prompt parts of up to 512 over up to 8192 keys, 16 x 8 x 256, bf16: 1.86 ms (1.75;
@@ -34,7 +34,7 @@
 // with which two workgroups have a CU's registers at one 16 of rows, and the query
 // copied into LDS as it is, 222, 168 and 2054 us; a chunk's softmax from one read of
 // its maxima and items as workgroups come to them 237, 170 and 1881 us with their plan;
-// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us), half lines
+// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us, 890 since), half lines
 // of K up to head dim 128 165 us; an item's claim and the next chunk's words behind the
 // scores 245 and 162 us.
 #pragma once
@@ -62,8 +62,9 @@ constexpr int rows_buffers(int dk)
 }
 
 // Eight waves of 32 keys at head dims 256 and 512, four of 64 below (a wave's part of
-// a V row is 16 dims at least; four waves at 256 took 2385 us for the prompt parts). Units of the ring are a 128-byte line of the wave's K
-// rows or its dims of some V rows.
+// a V row is 16 dims at least; four waves at 256 took 2385 us for the prompt parts).
+// Units of the ring are a 128-byte line of the wave's K rows, or of half of them, or its
+// dims of some V rows.
 template <int DK, typename T, int U> struct RowsCfg {
     static constexpr int NW = DK >= 256 ? 8 : 4;
     static constexpr int kThreads = 64 * NW;
@@ -76,13 +77,12 @@ template <int DK, typename T, int U> struct RowsCfg {
     static constexpr int NE = kUnit / 1024;            // copies of one
     static constexpr int kLine = 128 / (int)sizeof(T); // dims of a K unit
     static constexpr int kLines = (DK + kLine - 1) / kLine;
-    static constexpr int UK = kLines * kParts; // K units
-    static constexpr int SU = kLine / 32;      // score chain steps (32 dims) of a unit
+    static constexpr int UK = kLines * kParts;         // K units
+    static constexpr int SU = kLine / 32;              // score chain steps (32 dims) of a unit
     static constexpr int VL = DK / 16 / NW;            // 16-dim blocks of a wave's dims
     static constexpr int kRowV = 16 * VL * (int)sizeof(T); // bytes of a V row of the wave
     static constexpr int kLanesV = kRowV / 16;         // lanes that copy it
     static constexpr int kKeysV = kUnit / kRowV < kChunk ? kUnit / kRowV : kChunk;
-    static constexpr int NQ = U * DK / 16 / NW; // copies of the query by a wave
     static_assert(kKeysV >= 16, "units of 16 keys and more");
     static_assert(VL == 1 || VL == 2 || VL == 4, "a lane's values are one read");
 };
@@ -456,7 +456,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
 {
     using C = RowsCfg<DK, T, U>;
     constexpr int NW = C::NW, KW = C::KW, TW = C::TW, UK = C::UK, VL = C::VL, SU = C::SU;
-    static_assert(NB <= UK, "the ring holds one row's lines");
+    static_assert(NB <= UK, "the ring holds units of one K row");
     extern __shared__ __attribute__((aligned(16))) uint32_t dyn[];
     using Lds = RowsLds<DK, U>;
     Lds &s = *reinterpret_cast<Lds *>(dyn);
@@ -466,8 +466,8 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
     const int lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int k0 = KW * w; // the wave's keys
 
-    // Workgroups take items as they come to them: chunks differ in their keys, and so
-    // do the runs. Of each round of the grid's items an XCD (they have the workgroups
+    // Workgroups take items as they come to them: chunks differ in their keys, and items
+    // in their chunks. Of each round of the grid's items an XCD (they have the workgroups
     // in turn) has those side by side, whose units share its L2, and its workgroups
     // take them from a counter of its own; where items differ in their chunks they take
     // the other XCDs' behind their last one. One is taken while the one before the last
@@ -676,7 +676,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         }
     }
 
-    // the run's chunks merged so far
+    // the item's chunks merged so far
     float M1[U], L1[U];
     f4 merged[U][VL];
     for (int buf = 0;; buf ^= 1) {
