@@ -389,11 +389,15 @@ __device__ __forceinline__ TreeItem find_item(const TreeParams &p, const TreeWor
     return x;
 }
 
-// What a lane requests of an item's trees: masks of two of its new tokens (lane
-// 8 i + w: word w of token i and i + 8 of the unit's), the position of one of them
-// (lane i), and of its own keys where they are new.
+// What a lane requests of an item's trees: a word of one of its new tokens' masks
+// (lane 8 i + w: word w of token i of the unit's eight at most), the position of one
+// of them (lane i), and of its own keys where they are new. (One word: an index at run
+// time into two left all that an item requests ahead in memory. 64 trees of 2 over up
+// to 8192 keys, 16 x 8 x 256, bf16: 202 -> 182 us; 256 requests of one token over up to
+// 2048, 32 x 8 x 128, bf16: 128 -> 111 us; 16 of one over up to 32K, 16 x 2 x 512, f32:
+// 325 -> 306 us; a tree of 6 behind 200 keys 16.1 -> 15.7 us.)
 template <int KG> struct TreeFetched {
-    uint64_t mask[2];
+    uint64_t mask;
     int position, key[KG];
 };
 
@@ -402,7 +406,7 @@ __device__ __forceinline__ void fetch_tree(const TreeParams &p, const TreeItem &
                                            TreeFetched<KG> &f)
 {
     const int lane = threadIdx.x & 63;
-    f.mask[0] = f.mask[1] = 0;
+    f.mask = 0;
     f.position = 0;
 #pragma unroll
     for (int kg = 0; kg < KG; ++kg)
@@ -411,14 +415,9 @@ __device__ __forceinline__ void fetch_tree(const TreeParams &p, const TreeItem &
         return;
     const int i0 = (int)divided(x.first_row, p.by_group);
     const int last = (int)divided(x.first_row + x.nrows - 1, p.by_group);
-    if (x.cbase + x.hi >= x.held && lane % 8 < p.mask_words) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = i0 + lane / 8 + 8 * h;
-            if (i <= last)
-                f.mask[h] = p.masks[(int64_t)(x.row + i) * p.mask_words + lane % 8];
-        }
-    }
+    const int mine = i0 + lane / 8;
+    if (x.cbase + x.hi >= x.held && lane % 8 < p.mask_words && mine <= last)
+        f.mask = p.masks[(int64_t)(x.row + mine) * p.mask_words + lane % 8];
     if (!p.window)
         return;
     f.position = p.positions[x.row + min(i0 + lane, last)];
@@ -462,8 +461,7 @@ __device__ __forceinline__ void attending_rows(const TreeParams &p, const TreeIt
                 if (p.masks) {
                     if (!held) {
                         const int w = min(max(n, 0), 511);
-                        const uint64_t word =
-                            __shfl((unsigned long long)f.mask[i / 8], 8 * (i % 8) + w / 64);
+                        const uint64_t word = __shfl((unsigned long long)f.mask, 8 * i + w / 64);
                         s = n < 0 || (word >> (w % 64) & 1);
                     }
                     at = n < 0 ? t : f.key[kg];
@@ -494,6 +492,7 @@ paged_kv_body(const std::conditional_t<TREE, TreeParams, PagedParams> &p)
     using C = PagedCfg<DK, T, R>;
     using Item = std::conditional_t<TREE, TreeItem, PagedItem>;
     constexpr int KG = C::KG, KP = C::KP, UK = C::UK, VL = C::VL, NQ = C::NQ;
+    static_assert(!TREE || C::kRowsUnit <= 8, "a wave holds eight tokens' masks");
     __shared__ __attribute__((aligned(16))) std::conditional_t<TREE, TreeLds<DK, R>, PagedLds<DK, R>> s;
     __shared__ std::conditional_t<TREE, uint64_t, uint32_t> waves[C::NW];
     extern __shared__ __attribute__((aligned(16))) uint32_t dyn[];
@@ -1041,9 +1040,13 @@ __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
     paged_kv_body<DK, T, FULL, R, NB, false>(p);
 }
 
+// A tree's rows take more: with bf16 pages three waves spilled 11 registers at head dim
+// 64 and 3 at 128 (128 requests of one token over up to 8192 keys, 32 x 8 heads: 126 us
+// and 112 with two waves at 64, 190 and 187 at 128).
 template <int DK, typename T, bool FULL, int R, int NB>
 __global__ __launch_bounds__((PagedCfg<DK, T, R>::kThreads),
-                             (FULL && R == 1 && NB == 1 ? 3 : 1)) void paged_tree_kernel(TreeParams p)
+                             (FULL && R == 1 && NB == 1 && (sizeof(T) == 4 || DK >= 256) ? 3 : 1))
+void paged_tree_kernel(TreeParams p)
 {
     paged_kv_body<DK, T, FULL, R, NB, true>(p);
 }
