@@ -23,7 +23,7 @@ SOURCES = ["csrc/split_kv.hip", "csrc/pipe_kv.hip", "csrc/spread_kv.hip",
            "csrc/paged_rows_d256.hip", "csrc/paged_rows_d512.hip"]
 HEADERS = ["csrc/attention_device.hpp", "csrc/context.hpp", "csrc/launch.hpp", "csrc/paged.hpp",
            "csrc/paged_params.hpp", "csrc/paged_kv.hpp", "csrc/paged_rows.hpp",
-           "csrc/paged_combine.hpp",
+           "csrc/paged_combine.hpp", "csrc/item_claims.hpp",
            "csrc/page_batch.hpp",
            os.path.join(ROOT, "include", "pcl_attention.h")]
 

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "attention_device.hpp"
+#include "item_claims.hpp"
 
 #include <cstdint>
 
@@ -96,7 +97,7 @@ struct PlanItem {
 
 struct PlanHead {
     int items, uneven; // uneven: some have several chunks
-    int taken[8]; // items that each XCD's workgroups have taken, of its own
+    int taken[kItemParts]; // items of each part that are taken
     int spare[6];
 };
 

@@ -95,6 +95,7 @@ template <int DK, int U> struct RowsLds {
     int32_t slots[2][kChunk];             // of this chunk and the next
     int32_t live[2][kTilesPerChunk];      // tiles with a key that any row attends
     uint32_t taken;                       // the item behind the next one
+    uint32_t part; // whose items the workgroup takes (a register's use costs spills)
 };
 
 // The LDS of a CU, less the kernel's static words.
@@ -373,8 +374,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(TreeParams p, 
         p.plan->items = (int)all;
         p.plan->uneven = spans != 0;
         // (the first one of a workgroup is its own)
-        for (int i = 0; i < 8; ++i)
-            p.plan->taken[i] = workgroups % 8 ? workgroups : workgroups / 8;
+        for (int i = 0; i < (int)kItemParts; ++i)
+            p.plan->taken[i] =
+                workgroups % (int)kItemParts ? workgroups : workgroups / (int)kItemParts;
     }
     if (bad && blockIdx.x == 0)
         atomicOr(p.err, kErrPages);
@@ -467,34 +469,26 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
     const int k0 = KW * w; // the wave's keys
 
     // Workgroups take items as they come to them: chunks differ in their keys, and items
-    // in their chunks. Of each round of the grid's items an XCD (they have the workgroups
-    // in turn) has those side by side, whose units share its L2, and its workgroups
-    // take them from a counter of its own; where items differ in their chunks they take
-    // the other XCDs' behind their last one. One is taken while the one before the last
+    // in their chunks. An XCD's workgroups take those of its part, whose units share its
+    // L2 (item_claims.hpp); where items differ in their chunks they go on to the others'
+    // (prompt parts 1.87 ms, 1.9 to 2.0 without; where each is one chunk it costs: 64 trees
+    // 246 -> 258 us, 256 chains 165 -> 180). One is taken while the one before the last
     // runs, so that nobody waits for the counter.
     const plan_ptr plan = (plan_ptr)p.plan;
     const uint32_t items = (uint32_t)(*plan)[0];
-    const uint32_t parts = gridDim.x % 8 ? 1 : 8, each = gridDim.x / parts;
-    const bool uneven = parts == 8 && (*plan)[1] != 0;
-    uint32_t part = blockIdx.x % parts; // (by thread 0, as what follows)
-    auto place = [&](uint32_t n) { return n / each * gridDim.x + part * each + n % each; };
-    auto claim = [&]() { return (uint32_t)atomicAdd(&p.plan->taken[part], 1); };
-    auto take = [&]() { return place(claim()); };
-    auto settle = [&](uint32_t n) { // n, or another XCD's item where that is past the last
-        if (n < items || !uneven)
-            return n;
-        uint32_t taken[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            taken[i] = (uint32_t)__hip_atomic_load(&p.plan->taken[i], __ATOMIC_RELAXED,
+    const uint32_t parts = gridDim.x % kItemParts ? 1 : kItemParts;
+    const ItemClaims claims = {items, gridDim.x, gridDim.x / parts,
+                               parts > 1 && (*plan)[1] != 0};
+    // (by thread 0)
+    auto add = [&](uint32_t part) { return (uint32_t)atomicAdd(&p.plan->taken[part], 1); };
+    auto settle = [&](uint32_t n) { // item n of the workgroup's part, or another's
+        return claims.settle(
+            claims.place(s.part, n), s.part,
+            [&](uint32_t part) {
+                return (uint32_t)__hip_atomic_load(&p.plan->taken[part], __ATOMIC_RELAXED,
                                                    __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            part = i;
-            if (n >= items && place(taken[i]) < items)
-                n = take();
-        }
-        return n;
+            },
+            add);
     };
     // (an item past the last has no chunks, and is not skipped)
     auto load_item = [&](uint32_t n) {
@@ -509,21 +503,23 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         while (i.chunks == 0) { // (a chain's early units have none of the last keys)
             __syncthreads();
             if (tid == 0)
-                s.taken = settle(take());
+                s.taken = settle(add(s.part));
             __syncthreads();
             i = load_item(__builtin_amdgcn_readfirstlane(s.taken));
         }
         return i;
     };
-    if (tid == 0)
-        s.taken = place(blockIdx.x / parts);
+    if (tid == 0) {
+        s.part = blockIdx.x % parts;
+        s.taken = claims.place(s.part, blockIdx.x / parts);
+    }
     __syncthreads();
     PlanItem now = taken_item();
     if (now.chunks < 0)
         return;
     __syncthreads();
     if (tid == 0)
-        s.taken = settle(take());
+        s.taken = settle(add(s.part));
     PlanItem next; // (taken below)
     int chunk = 0; // of `now`
 
@@ -788,7 +784,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         // P.V: ahead of the scores the first wait for a unit's copies waits for them too.
         uint32_t behind_next = 0;
         if (new_q && tid == 0)
-            behind_next = claim();
+            behind_next = add(s.part);
         Fetched f;
         if (more)
             fetch(y, f);
@@ -1075,7 +1071,7 @@ __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
         if (!more)
             break;
         if (new_q && tid == 0)
-            s.taken = settle(place(behind_next));
+            s.taken = settle(behind_next);
         lds_barrier(); // the next query
         x = y;
         ++chunk;
