@@ -1118,12 +1118,11 @@ static hipError_t launch_paged(const P &p, int64_t items, hipStream_t stream)
     return hipGetLastError();
 }
 
-// `rows`: of a KV head that one request has at most; `chunks`: of the requests at
-// their longest.
-template <int DK, typename T, bool FULL, int R, typename P>
-static hipError_t launch_paged(P p, int64_t rows, int64_t chunks, hipStream_t stream)
+// `chunks`: of the requests at their longest.
+template <int DK, typename T, bool FULL, int R>
+static hipError_t launch_newest(PagedParams p, int64_t chunks, hipStream_t stream)
 {
-    p.units = (int)((rows + PagedCfg<DK, T, R>::kRowsUnit - 1) / PagedCfg<DK, T, R>::kRowsUnit);
+    p.units = (p.group + PagedCfg<DK, T, R>::kRowsUnit - 1) / PagedCfg<DK, T, R>::kRowsUnit;
     // (the items at the requests' longest)
     const int64_t items = chunks * p.kvheads * p.units;
     if constexpr (FULL && R <= 2) {
@@ -1133,41 +1132,56 @@ static hipError_t launch_paged(P p, int64_t rows, int64_t chunks, hipStream_t st
     return launch_paged<DK, T, FULL, R, 1>(p, items, stream);
 }
 
-template <int DK, typename T, bool FULL, typename P>
-static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
+template <int DK, typename T, bool FULL>
+static hipError_t launch_newest(const PagedParams &p, int64_t chunks, hipStream_t stream)
 {
-    // (a tree launch of few items splits its rows over more workgroups)
-    constexpr bool TREE = std::is_same_v<P, TreeParams>;
-    if (rows <= 4 || (TREE && few_items(FULL, chunks * p.kvheads, rows, 4)))
-        return launch_paged<DK, T, FULL, 1>(p, rows, chunks, stream);
-    if (rows <= 8 || (TREE && few_items(FULL, chunks * p.kvheads, rows, 8)))
-        return launch_paged<DK, T, FULL, 2>(p, rows, chunks, stream);
-    if constexpr (std::is_same_v<P, TreeParams>)
-        return launch_paged_rows<DK>(p, std::is_same_v<T, __bf16>, rows, chunks, stream);
-    else
-        return launch_paged<DK, T, FULL, 4>(p, rows, chunks, stream);
+    if (p.group <= 4)
+        return launch_newest<DK, T, FULL, 1>(p, chunks, stream);
+    if (p.group <= 8)
+        return launch_newest<DK, T, FULL, 2>(p, chunks, stream);
+    return launch_newest<DK, T, FULL, 4>(p, chunks, stream);
 }
 
-template <int DK, typename T, typename P>
-static hipError_t launch_paged(const P &p, int64_t rows, int64_t chunks, hipStream_t stream)
+template <int DK, typename T>
+static hipError_t launch_newest(const PagedParams &p, int64_t chunks, hipStream_t stream)
 {
-    return p.dim == DK ? launch_paged<DK, T, true>(p, rows, chunks, stream)
-                       : launch_paged<DK, T, false>(p, rows, chunks, stream);
+    return p.dim == DK ? launch_newest<DK, T, true>(p, chunks, stream)
+                       : launch_newest<DK, T, false>(p, chunks, stream);
 }
 
 template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream)
 {
-    return bf16 ? launch_paged<DK, __bf16>(p, p.group, chunks, stream)
-                : launch_paged<DK, float>(p, p.group, chunks, stream);
+    return bf16 ? launch_newest<DK, __bf16>(p, chunks, stream)
+                : launch_newest<DK, float>(p, chunks, stream);
+}
+
+template <int DK, typename T, bool FULL>
+static hipError_t launch_tree(const TreeParams &p, const TreeVariant &v, int64_t items,
+                              hipStream_t stream)
+{
+    if constexpr (FULL) {
+        if (v.buffers == 2)
+            return v.rows == 4 ? launch_paged<DK, T, FULL, 1, 2>(p, items, stream)
+                               : launch_paged<DK, T, FULL, 2, 2>(p, items, stream);
+    }
+    return v.rows == 4 ? launch_paged<DK, T, FULL, 1, 1>(p, items, stream)
+                       : launch_paged<DK, T, FULL, 2, 1>(p, items, stream);
 }
 
 template <int DK>
-hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream)
+hipError_t launch_paged_tree(const TreeParams &p, const TreeVariant &v, bool bf16, int64_t rows,
+                             int64_t chunks, hipStream_t stream)
 {
-    const int64_t rows = (int64_t)p.max_new * p.group;
-    return bf16 ? launch_paged<DK, __bf16>(p, rows, chunks, stream)
-                : launch_paged<DK, float>(p, rows, chunks, stream);
+    if (!v.buffers)
+        return launch_paged_rows<DK>(p, v.rows, bf16, rows, chunks, stream);
+    // (the items at the requests' longest)
+    const int64_t items = chunks * p.kvheads * ((rows + v.rows - 1) / v.rows);
+    if (p.dim == DK)
+        return bf16 ? launch_tree<DK, __bf16, true>(p, v, items, stream)
+                    : launch_tree<DK, float, true>(p, v, items, stream);
+    return bf16 ? launch_tree<DK, __bf16, false>(p, v, items, stream)
+                : launch_tree<DK, float, false>(p, v, items, stream);
 }
 
 } // namespace pcl

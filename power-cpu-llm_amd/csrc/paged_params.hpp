@@ -155,27 +155,25 @@ __device__ __forceinline__ int tree_chunks(const TreeParams &p, const TreeKeys &
     return r.len > r.held ? (r.len - 1) / kChunk + 1 - first_tree_key(p, r.held) / kChunk : 0;
 }
 
+// The kernel of a tree launch: units of `rows` query rows, 4 or 8 (paged_kv.hpp, with
+// `buffers` in a wave's ring) or 16, 32 or 48 (paged_rows.hpp, `buffers` 0).
+struct TreeVariant {
+    int rows, buffers;
+};
+
+// Which one a launch of at most `chunks` chunks takes on a device of `cus` CUs; `rows`:
+// query rows of a KV head that one request has at most.
+TreeVariant tree_variant(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows, int64_t cus);
+
 // The chunk kernel of a launch of at most `chunks` chunks, at padded head dim
 // DK (64, 128, 256 or 512, a source file each).
 template <int DK>
 hipError_t launch_paged_kv(const PagedParams &p, bool bf16, int64_t chunks, hipStream_t stream);
 template <int DK>
-hipError_t launch_paged_tree(const TreeParams &p, bool bf16, int64_t chunks, hipStream_t stream);
-// Rows of a KV head and request up to which one wave's MFMAs hold a unit (paged_kv.hpp).
-constexpr int64_t kFewRows = 8;
-// Whether units of `unit` rows leave a tree launch at most an item per CU, each with a
-// CU to itself; `whole`: the head dim is one that needs no padding. `items`: at one
-// unit, `rows`: of a KV head that one request has at most. Such launches split their
-// rows over more workgroups of paged_kv.hpp (one request of 8 new tokens behind 1000
-// keys, f32: 21 us and 26 in units of sixteen rows at 16 x 8 x 256 heads, 29 and 54 at
-// 16 x 2 x 512, 21 and 27 at 32 x 8 x 128, both 23 at 16 x 4 x 64; of 40 behind 500: 26
-// and 45, 36 and 57, both 43, 31 and 37).
-bool few_items(bool whole, int64_t items, int64_t rows, int64_t unit);
-// Whether such a launch takes the kernels of many rows (paged_rows.hpp).
-bool many_rows(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows);
-// `rows`: query rows of a KV head that one request has at most, above eight.
+hipError_t launch_paged_tree(const TreeParams &p, const TreeVariant &v, bool bf16, int64_t rows,
+                             int64_t chunks, hipStream_t stream);
 template <int DK>
-hipError_t launch_paged_rows(const TreeParams &p, bool bf16, int64_t rows, int64_t chunks,
-                             hipStream_t stream);
+hipError_t launch_paged_rows(const TreeParams &p, int unit, bool bf16, int64_t rows,
+                             int64_t chunks, hipStream_t stream);
 
 } // namespace pcl

@@ -452,6 +452,10 @@ __device__ __forceinline__ TreeItem chunk_item(const PlanItem &i, int k)
 
 // Four waves a SIMD, two workgroups a CU, where one 16 of rows leaves room for them
 // (128 registers; 64 trees of bf16 219 us, 254 us at the 148 that the compiler took).
+// (48 rows at padded head dim 128, bf16, spill 4 registers at 256; with the one workgroup
+// that the LDS holds as the bound the compiler holds sums in AGPRs and copies them: prompt
+// parts of 512 tokens at 32 x 8 x 112, bf16, 2276 us and 2180, at 128 2262 and 2124; units
+// of 32 rows 2350.)
 template <int DK, typename T, bool FULL, int U, int NB>
 __global__ __launch_bounds__((RowsCfg<DK, T, U>::kThreads),
                              (DK == 256 && U == 1 ? 4 : 2)) void tree_rows_kernel(TreeParams p)
@@ -1132,40 +1136,27 @@ static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks,
     return hipGetLastError();
 }
 
-// 16s of rows of the largest unit: what the LDS of a CU holds beside the rings (512),
-// and what its registers do (four at head dim 128 spilled 43 to 157 of them: prompt parts
-// 2290 us, 2146 with three; trees of 12 at 32 x 8 x 128, f32, 513 and 385 us). Units of two
-// instead of three at head dim 256, with two buffers: prompt parts 2250 us (2064).
-constexpr int most_groups(int dk)
-{
-    return dk == 512 ? 2 : 3;
-}
-
-// The fewest units that hold a request's rows, and the smallest such units: no matrix
-// instruction runs on rows that none has (64 trees of 16 at 32 x 8 x 128, 64 rows in two
-// units of 32: 577 us; as 48 and 16: 759 us).
 template <int DK, typename T, bool FULL>
-static hipError_t launch_rows(const TreeParams &p, int64_t rows, int64_t chunks, hipStream_t stream)
+static hipError_t launch_rows(const TreeParams &p, int unit, int64_t rows, int64_t chunks,
+                              hipStream_t stream)
 {
-    constexpr int most = 16 * most_groups(DK);
-    const int64_t units = (rows + most - 1) / most, unit = (rows + units - 1) / units;
-    if constexpr (most_groups(DK) > 2) {
-        if (unit > 32)
+    if constexpr (DK < 512) { // (tree_variant)
+        if (unit == 48)
             return launch_rows<DK, T, FULL, 3>(p, rows, chunks, stream);
     }
-    return unit > 16 ? launch_rows<DK, T, FULL, 2>(p, rows, chunks, stream)
-                     : launch_rows<DK, T, FULL, 1>(p, rows, chunks, stream);
+    return unit == 32 ? launch_rows<DK, T, FULL, 2>(p, rows, chunks, stream)
+                      : launch_rows<DK, T, FULL, 1>(p, rows, chunks, stream);
 }
 
 template <int DK>
-hipError_t launch_paged_rows(const TreeParams &p, bool bf16, int64_t rows, int64_t chunks,
-                             hipStream_t stream)
+hipError_t launch_paged_rows(const TreeParams &p, int unit, bool bf16, int64_t rows,
+                             int64_t chunks, hipStream_t stream)
 {
     if (p.dim == DK)
-        return bf16 ? launch_rows<DK, __bf16, true>(p, rows, chunks, stream)
-                    : launch_rows<DK, float, true>(p, rows, chunks, stream);
-    return bf16 ? launch_rows<DK, __bf16, false>(p, rows, chunks, stream)
-                : launch_rows<DK, float, false>(p, rows, chunks, stream);
+        return bf16 ? launch_rows<DK, __bf16, true>(p, unit, rows, chunks, stream)
+                    : launch_rows<DK, float, true>(p, unit, rows, chunks, stream);
+    return bf16 ? launch_rows<DK, __bf16, false>(p, unit, rows, chunks, stream)
+                : launch_rows<DK, float, false>(p, unit, rows, chunks, stream);
 }
 
 } // namespace pcl

@@ -1,5 +1,5 @@
 // The chunk kernels of many query rows of a step's new tokens at padded head dim 512.
 #include "paged_rows.hpp"
 
-template hipError_t pcl::launch_paged_rows<512>(const TreeParams &, bool, int64_t, int64_t,
+template hipError_t pcl::launch_paged_rows<512>(const TreeParams &, int, bool, int64_t, int64_t,
                                                 hipStream_t);

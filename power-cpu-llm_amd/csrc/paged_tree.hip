@@ -83,15 +83,32 @@ static int64_t most_rows(const pcl_paged_tree_desc &d)
     return std::min(d.q_rows, d.requests * std::min(d.max_new, d.max_length));
 }
 
-bool few_items(bool whole, int64_t items, int64_t rows, int64_t unit)
-{
-    return whole && items * ((rows + unit - 1) / unit) <= device_cus();
-}
+// Query rows of a KV head and request up to which no launch is one of many rows.
+constexpr int64_t kFewRows = 8;
 
-bool many_rows(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows)
+// Units of 4 or 8 rows where a request has no more, or where they leave at most an item
+// per CU, each with a CU to itself (one request of 8 new tokens behind 1000 keys, f32: 21
+// us and 26 in units of sixteen rows at 16 x 8 x 256 heads, 29 and 54 at 16 x 2 x 512, 21
+// and 27 at 32 x 8 x 128, both 23 at 16 x 4 x 64; of 40 behind 500: 26 and 45, 36 and 57,
+// both 43, 31 and 37); two buffers of the ring where an item has a CU to itself (PagedCfg
+// has both sides). Otherwise the fewest units that hold a request's rows, and the smallest
+// such units: no matrix instruction runs on rows that none has (64 trees of 16 at 32 x 8 x
+// 128, 64 rows in two units of 32: 577 us; as 48 and 16: 759 us). The largest unit is what
+// the LDS of a CU holds beside the rings (512) and what its registers do (64 rows at head
+// dim 128 spilled 43 to 157 of them: prompt parts 2290 us, 2146 with 48; trees of 12 at 32
+// x 8 x 128, f32, 513 and 385 us). Units of 32 instead of 48 at head dim 256, with two
+// buffers: prompt parts 2250 us (2064).
+TreeVariant tree_variant(int64_t dim, int64_t chunks, int64_t kvheads, int64_t rows, int64_t cus)
 {
-    const bool whole = dim == 64 || dim == 128 || dim == 256 || dim == 512;
-    return rows > kFewRows && !few_items(whole, chunks * kvheads, rows, kFewRows);
+    const bool whole = dim == 64 || dim == 128 || dim == 256 || dim == 512; // not padded
+    for (const int unit : {4, (int)kFewRows}) {
+        const bool few = whole && chunks * kvheads * ((rows + unit - 1) / unit) <= cus;
+        if (rows <= unit || few)
+            return {unit, few ? 2 : 1};
+    }
+    const int64_t most = dim > 256 ? 32 : 48;
+    const int64_t units = (rows + most - 1) / most, unit = (rows + units - 1) / units;
+    return {unit > 32 ? 48 : unit > 16 ? 32 : 16, 0};
 }
 
 static int check_tree(const pcl_paged_tree_desc &d)
@@ -196,8 +213,11 @@ int pcl_paged_tree_attention(pcl_context *ctx, const pcl_paged_tree_desc *desc)
     p.o_stride = d.o_stride;
     const int64_t items = pcl::most_items(d);
     p.max_items = (int)items;
-    const bool many = pcl::many_rows(s.dim, d.requests * each, s.kvheads,
-                                     std::min(d.max_new, d.max_length) * (d.qheads / s.kvheads));
+    const int64_t rows = std::min(d.max_new, d.max_length) * (d.qheads / s.kvheads);
+    const int64_t chunks = d.requests * each;
+    const pcl::TreeVariant v =
+        pcl::tree_variant(s.dim, chunks, s.kvheads, rows, pcl::device_cus());
+    const bool many = !v.buffers;
     p.plan = many ? reinterpret_cast<pcl::PlanHead *>(body) : nullptr;
     p.split = many ? reinterpret_cast<int32_t *>(body + 16 * (1 + items)) : nullptr;
     body += items ? 16 * (1 + items) + pcl::split_bytes(d) / sizeof(float) : 0;
@@ -229,13 +249,13 @@ int pcl_paged_tree_attention(pcl_context *ctx, const pcl_paged_tree_desc *desc)
     p.by_group = pcl::divisor((uint32_t)p.group);
     p.by_kvheads = pcl::divisor((uint32_t)p.kvheads);
     p.by_page_tokens = pcl::divisor(p.page_tokens);
-    const int64_t chunks = d.requests * each;
     const bool bf16 = s.type == PCL_CACHE_BF16;
     int span = pcl::open_timed_span(ctx, 0);
-    hipError_t e = p.dim <= 64    ? pcl::launch_paged_tree<64>(p, bf16, chunks, ctx->stream)
-                   : p.dim <= 128 ? pcl::launch_paged_tree<128>(p, bf16, chunks, ctx->stream)
-                   : p.dim <= 256 ? pcl::launch_paged_tree<256>(p, bf16, chunks, ctx->stream)
-                                  : pcl::launch_paged_tree<512>(p, bf16, chunks, ctx->stream);
+    const auto launch = p.dim <= 64    ? pcl::launch_paged_tree<64>
+                        : p.dim <= 128 ? pcl::launch_paged_tree<128>
+                        : p.dim <= 256 ? pcl::launch_paged_tree<256>
+                                       : pcl::launch_paged_tree<512>;
+    hipError_t e = launch(p, v, bf16, rows, chunks, ctx->stream);
     pcl::close_timed_span(ctx, span);
     if (e == hipSuccess && each > 1) {
         span = pcl::open_timed_span(ctx, 1);

@@ -1,9 +1,117 @@
-"""The compiled kernels of pcl_paged_tree_attention: their registers."""
+"""Every compiled kernel of pcl_paged_tree_attention: which launch takes which, its
+bits and error on that launch, and its registers.
+
+A launch's kernel follows from the head dim, the page type, the rows of a KV head that
+a request has at most and the items (tree_variant of csrc/paged_tree.hip, which the
+tests ask, so that a change of the rule cannot leave a kernel without its test).
+"""
+import ctypes
 import os
 import re
 import subprocess
 
+import numpy as np
 import pytest
+
+import test_paged as tp
+from test_paged import bits, ctx, torch  # noqa: F401
+from test_paged_tree import TreeCache, random_trees
+
+CUS = 256  # of an MI355X
+
+
+class Variant(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int), ("buffers", ctypes.c_int)]
+
+
+def variant_of(pcl, dim, chunks, kvheads, rows, cus=CUS):
+    fn = pcl.load()._ZN3pcl12tree_variantElllll
+    fn.restype = Variant
+    fn.argtypes = [ctypes.c_int64] * 5
+    v = fn(dim, chunks, kvheads, rows, cus)
+    return v.rows, v.buffers
+
+
+# query heads of a KV head and the most new tokens of a request, for each unit of rows
+SHAPES = {4: (2, 2), 8: (3, 2), 16: (4, 4), 32: (8, 3), 48: (5, 8)}
+DIMS = [64, 48, 128, 80, 256, 208, 512, 272]  # whole and padded
+KVHEADS = 4
+# held tokens around tiles, pages and chunks: of few items, of few in units of eight rows
+# (192 over the KV heads) and of many (288)
+FEW = [0, 255, 300]
+EIGHTS = [33, 200, 255, 256, 500, 700, 1000, 1500]
+MANY = [0, 0, 1, 31] + EIGHTS
+
+
+def padded(dim):
+    return next(d for d in (64, 128, 256, 512) if dim <= d)
+
+
+def cases():
+    """(dim, dtype, rows of the unit, buffers, held tokens)."""
+    out = []
+    for dim in DIMS:
+        for dtype in ("f32", "bf16"):
+            for unit in SHAPES:
+                if unit == 48 and dim > 256:
+                    continue
+                if unit <= 8 and dim == padded(dim):
+                    out.append((dim, dtype, unit, 2, FEW if unit == 4 else EIGHTS))
+                out.append((dim, dtype, unit, 1 if unit <= 8 else 0, MANY))
+    return out
+
+
+def launch_of(unit, held):
+    """(query heads, new tokens of each request, max_length, chunks of the launch)."""
+    group, most = SHAPES[unit]
+    counts = [1 + (5 * b + most - 1) % most for b in range(len(held))]
+    counts[len(held) // 2] = 0
+    counts[1] = most
+    length = max(a + n for a, n in zip(held, counts))
+    return group * KVHEADS, counts, length, len(held) * -(-length // 256)
+
+
+def kernel_of(dim, dtype, unit, buffers):
+    """A kernel's name without the ring of the many-row ones."""
+    kind = "f" if dtype == "f32" else "DF16b"
+    whole = int(dim == padded(dim))
+    if buffers:
+        return "paged_tree %d %s %d %d %d" % (padded(dim), kind, whole, unit // 4, buffers)
+    return "tree_rows %d %s %d %d" % (padded(dim), kind, whole, unit // 16)
+
+
+def test_a_case_for_every_compiled_kernel(pcl):
+    pcl.load()
+    symbols = subprocess.run(["nm", "-D", "--defined-only", pcl.LIB_PATH], check=True,
+                             capture_output=True, text=True).stdout
+    compiled = set()
+    for name, dk, kind, whole, n, nb in re.findall(
+            r"_ZN3pcl\d+(paged_tree|tree_rows)_kernelILi(\d+)E(f|DF16b)Lb([01])ELi(\d)ELi(\d)E",
+            symbols):
+        compiled.add(" ".join((name, dk, kind, whole, n) + ((nb,) if name == "paged_tree" else ())))
+    assert len(compiled) == 48 + 44
+    reached = set()
+    for dim, dtype, unit, buffers, held in cases():
+        group, most = SHAPES[unit]
+        chunks = launch_of(unit, held)[3]
+        assert variant_of(pcl, dim, chunks, KVHEADS, group * most) == (unit, buffers)
+        reached.add(kernel_of(dim, dtype, unit, buffers))
+    assert reached == compiled
+
+
+def test_variants_of_launches(pcl):
+    # rows of one unit and of several; few items, of whole head dims alone
+    for rows, unit in ((1, 4), (4, 4), (5, 8), (8, 8), (9, 16), (16, 16), (17, 32), (32, 32),
+                       (33, 48), (48, 48), (49, 32), (64, 32), (65, 48), (97, 48), (1 << 20, 48)):
+        assert variant_of(pcl, 256, 1 << 20, 8, rows) == (unit, 0 if unit > 8 else 1)
+        assert variant_of(pcl, 80, 1, 1, rows) == (unit, 0 if unit > 8 else 1)
+    for rows, unit in ((9, 16), (16, 16), (17, 32), (33, 32), (49, 32), (1 << 20, 32)):
+        assert variant_of(pcl, 512, 1 << 20, 8, rows) == (unit, 0)
+    assert variant_of(pcl, 64, 64, 4, 4) == (4, 2)
+    assert variant_of(pcl, 64, 65, 4, 4) == (4, 1)
+    assert variant_of(pcl, 64, 8, 4, 32) == (4, 2)
+    assert variant_of(pcl, 64, 16, 4, 32) == (8, 2)
+    assert variant_of(pcl, 64, 17, 4, 32) == (32, 0)
 
 
 def resources(source):
@@ -43,3 +151,84 @@ def test_no_kernel_of_few_rows_keeps_its_words_in_memory():
     kernels = {n: w for n, w in found.items() if "paged_tree_kernel" in n}
     assert len(kernels) == 48
     assert {n: w for n, w in kernels.items() if w != (0, 0)} == {}
+
+
+# registers that spill where both ways around it were slower: 48 rows at padded head dim
+# 128 with bf16 pages (the compiler holds 256; a bound of 512 puts sums into AGPRs)
+SPILLS = {"_ZN3pcl16tree_rows_kernelILi128EDF16bLb0ELi3ELi3EEEvNS_10TreeParamsE": (32, 8)}
+
+
+def test_no_kernel_of_many_rows_keeps_its_words_in_memory():
+    from concurrent.futures import ThreadPoolExecutor
+    if not os.path.exists("/opt/rocm/bin/hipcc"):
+        pytest.skip("hipcc absent")
+    with ThreadPoolExecutor(4) as pool:
+        found = dict(x for r in pool.map(resources, ["paged_rows_d%d.hip" % dk for dk in
+                                                     (512, 64, 128, 256)]) for x in r.items())
+    kernels = {n: w for n, w in found.items() if "tree_rows_kernel" in n}
+    assert len(kernels) == 44 and set(SPILLS) <= set(kernels)
+    for name, words in kernels.items():
+        most = SPILLS.get(name, (0, 0))
+        assert words[0] <= most[0] and words[1] <= most[1], (name, words)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,dtype,unit,buffers,held", cases(),
+                         ids=lambda x: None if isinstance(x, list) else str(x))
+def test_each_kernel_has_the_contiguous_bits(pcl, torch, ctx, dim, dtype, unit, buffers, held):
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    qheads, counts, length, chunks = launch_of(unit, held)
+    group, most = SHAPES[unit]
+    assert variant_of(pcl, dim, chunks, KVHEADS, group * most, cus) == (unit, buffers)
+    masks, positions = random_trees(np.random.default_rng(dim + unit), held, counts)
+    for tree in (None, masks):
+        cache = TreeCache(pcl, torch, (qheads, KVHEADS, dim), held, counts, 16, dtype, dim, tree,
+                          positions if tree else None)
+        q = cache.queries()
+        for window, softcap in ((0, 0.0), (100, 0.0), (0, 1.5)):
+            out = cache.tree_attend(ctx, q, window=window, softcap=softcap, max_length=length,
+                                    max_new=most)
+            assert ctx.sync() == 0
+            cache.check(ctx, q, out, window=window, softcap=softcap, exact=tree is not None)
+            assert bool((out[cache.rows - 3:] == 9.5).all())
+    assert ctx.sync() == 0
+
+
+# Whole spans of chunks are items from as many chunks on (over the units and KV heads) as
+# the longest span has, for each workgroup: at most four on a CU. Requests of one span of
+# three chunks, 3072 to 3456 of them in all; and of a whole span of sixteen and a part of
+# the next, 8640 chunks for two workgroups a CU (8192).
+SPANS = [((32, 8, 64), "f32", 16, [513 + i for i in range(128)]),
+         ((32, 8, 128), "f32", 16, [600 - 7 * i % 80 for i in range(128)]),
+         ((16, 8, 256), "bf16", 16, [600 + i for i in range(144)]),
+         ((16, 8, 256), "f32", 32, [590 + i % 40 for i in range(144)]),
+         ((32, 8, 128), "bf16", 32, [513 + i for i in range(128)]),
+         ((32, 8, 64), "bf16", 16, [4360 + 3 * i for i in range(60)])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dtype,unit,held", SPANS, ids=lambda x: None
+                         if isinstance(x, list) else str(x))
+@pytest.mark.parametrize("tree", [False, True], ids=["chain", "tree"])
+def test_spans_of_small_units_as_items(pcl, torch, ctx, heads, dtype, unit, held, tree):
+    qheads, kvheads, dim = heads
+    group = qheads // kvheads
+    most = unit // group
+    counts = [most - i % 3 for i in range(len(held))]
+    masks = positions = None
+    if tree:
+        masks, positions = random_trees(np.random.default_rng(dim), held, counts)
+    cache = TreeCache(pcl, torch, heads, held, counts, 64, dtype, 29, masks, positions)
+    length = max(cache.lengths)
+    chunks = len(held) * -(-length // 256)
+    assert chunks * kvheads >= 3 * 4 * CUS
+    assert variant_of(pcl, dim, chunks, kvheads, group * most) == (unit, 0)
+    q = cache.queries()
+    out = cache.tree_attend(ctx, q, max_length=length)
+    assert ctx.sync() == 0
+    again = cache.tree_attend(ctx, q, max_length=length)
+    assert np.array_equal(bits(out), bits(again))
+    cache.check(ctx, q, out, requests=[0, 1, len(held) // 2, len(held) - 2, len(held) - 1],
+                exact=False)
+    assert bool((out[cache.rows - 3:] == 9.5).all())
+    assert ctx.sync() == 0
