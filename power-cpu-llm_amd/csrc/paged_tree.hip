@@ -90,8 +90,10 @@ constexpr int64_t kFewRows = 8;
 // per CU, each with a CU to itself (one request of 8 new tokens behind 1000 keys, f32: 21
 // us and 26 in units of sixteen rows at 16 x 8 x 256 heads, 29 and 54 at 16 x 2 x 512, 21
 // and 27 at 32 x 8 x 128, both 23 at 16 x 4 x 64; of 40 behind 500: 26 and 45, 36 and 57,
-// both 43, 31 and 37); two buffers of the ring where an item has a CU to itself (PagedCfg
-// has both sides). Otherwise the fewest units that hold a request's rows, and the smallest
+// both 43, 31 and 37; padded, the 8 behind 1000: 23 and 35 at 10 x 2 x 80, 22 and 27 at 16 x
+// 8 x 144, 35 and 56 at 16 x 2 x 400, but 25 and 24 at 16 x 4 x 48 and the same at 16 and 32
+// dims, of 40 behind 500 33 and 29: not below 64). Two buffers of the ring where an item of
+// a whole head dim has a CU to itself (PagedCfg has both sides). Otherwise the fewest units that hold a request's rows, and the smallest
 // such units: no matrix instruction runs on rows that none has (64 trees of 16 at 32 x 8 x
 // 128, 64 rows in two units of 32: 577 us; as 48 and 16: 759 us). The largest unit is what
 // the LDS of a CU holds beside the rings (512) and what its registers do (64 rows at head
@@ -102,9 +104,9 @@ TreeVariant tree_variant(int64_t dim, int64_t chunks, int64_t kvheads, int64_t r
 {
     const bool whole = dim == 64 || dim == 128 || dim == 256 || dim == 512; // not padded
     for (const int unit : {4, (int)kFewRows}) {
-        const bool few = whole && chunks * kvheads * ((rows + unit - 1) / unit) <= cus;
-        if (rows <= unit || few)
-            return {unit, few ? 2 : 1};
+        const bool few = chunks * kvheads * ((rows + unit - 1) / unit) <= cus;
+        if (rows <= unit || (few && dim >= 64))
+            return {unit, few && whole ? 2 : 1};
     }
     const int64_t most = dim > 256 ? 32 : 48;
     const int64_t units = (rows + most - 1) / most, unit = (rows + units - 1) / units;

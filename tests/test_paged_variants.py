@@ -100,11 +100,11 @@ def test_a_case_for_every_compiled_kernel(pcl):
 
 
 def test_variants_of_launches(pcl):
-    # rows of one unit and of several; few items, of whole head dims alone
+    # rows of one unit and of several
     for rows, unit in ((1, 4), (4, 4), (5, 8), (8, 8), (9, 16), (16, 16), (17, 32), (32, 32),
                        (33, 48), (48, 48), (49, 32), (64, 32), (65, 48), (97, 48), (1 << 20, 48)):
         assert variant_of(pcl, 256, 1 << 20, 8, rows) == (unit, 0 if unit > 8 else 1)
-        assert variant_of(pcl, 80, 1, 1, rows) == (unit, 0 if unit > 8 else 1)
+        assert variant_of(pcl, 48, 1, 1, rows) == (unit, 0 if unit > 8 else 1)
     for rows, unit in ((9, 16), (16, 16), (17, 32), (33, 32), (49, 32), (1 << 20, 32)):
         assert variant_of(pcl, 512, 1 << 20, 8, rows) == (unit, 0)
     assert variant_of(pcl, 64, 64, 4, 4) == (4, 2)
@@ -112,6 +112,37 @@ def test_variants_of_launches(pcl):
     assert variant_of(pcl, 64, 8, 4, 32) == (4, 2)
     assert variant_of(pcl, 64, 16, 4, 32) == (8, 2)
     assert variant_of(pcl, 64, 17, 4, 32) == (32, 0)
+    # few items of padded head dims above 64 have one buffer
+    for dim in (80, 112, 144, 208, 272, 496):
+        assert variant_of(pcl, dim, 8, 4, 32) == (4, 1)
+        assert variant_of(pcl, dim, 16, 4, 32) == (8, 1)
+        assert variant_of(pcl, dim, 17, 4, 32) == (32, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(10, 2, 80), (16, 8, 144), (6, 3, 208), (16, 2, 400),
+                                   (4, 1, 112), (16, 4, 48)],
+                         ids=lambda h: "x".join(map(str, h)))
+def test_few_items_of_padded_head_dims(pcl, torch, ctx, dtype, heads):
+    qheads, kvheads, dim = heads
+    rng = np.random.default_rng(dim)
+    for held, counts in (([100], [6]), ([1000], [8]), ([500], [40]), ([64, 2, 700], [9, 4, 12])):
+        masks, positions = random_trees(rng, held, counts)
+        for tree in (None, masks):
+            cache = TreeCache(pcl, torch, heads, held, counts, 16, dtype, sum(held), tree,
+                              positions if tree else None)
+            q = cache.queries()
+            length = max(cache.lengths)
+            rows = max(counts) * qheads // kvheads
+            variant = variant_of(pcl, dim, len(held) * -(-length // 256), kvheads, rows)
+            assert variant[1] == (1 if dim > 64 or rows <= 8 else 0)
+            for window, softcap in ((0, 0.0), (70, 0.0), (0, 1.5)):
+                out = cache.tree_attend(ctx, q, window=window, softcap=softcap,
+                                        max_length=length)
+                assert ctx.sync() == 0
+                cache.check(ctx, q, out, window=window, softcap=softcap)
+    assert ctx.sync() == 0
 
 
 def resources(source):
