@@ -348,6 +348,8 @@ int zero_tag_region(pcl_context *ctx, void *ws, size_t bytes, uint32_t *gen)
 {
     const int nwords = (int)std::min<size_t>(kTagFloats, bytes / sizeof(uint32_t));
     *gen = current_generation(ctx->device);
+    if (nwords == 0) // (a workspace of less than a word)
+        return PCL_OK;
     zero_words_kernel<<<(nwords + 255) / 256, 256, 0, ctx->stream>>>(
         static_cast<uint32_t *>(ws), nwords);
     const hipError_t e = hipGetLastError();
