@@ -736,13 +736,15 @@ int pcl_paged_copy(pcl_context *ctx, const pcl_page_pools *pools, int64_t layers
  * token attends only keys whose position is less than `window` before its own (the
  * new tokens' by positions, which lie from lengths[b] to step_lengths[b] - 1).
  * Requests without new tokens or with a negative newest are left out, and a token
- * that attends no key too: their output rows stay as they were. Queries are scaled and scores capped as in
- * pcl_attention_desc. A token's output has the bits that pcl_attention_launch gives
- * for the request's keys and values in one segment (the chain: causal, first_key 0,
- * first_query lengths[b]; masks: with the same mask as bytes), whatever else is in
- * the batch; only a zero's sign may differ. Keys that no token attends may hold
- * anything. A key that one token attends and another one does not may make the
- * latter a NaN where its value is not finite; the former sets the error flag then.
+ * that attends no key too: their output rows stay as they were. Queries are scaled and
+ * scores capped as in pcl_attention_desc. A token's output has the bits that
+ * pcl_attention_launch gives for the request's keys and values in one segment (the
+ * chain: causal, first_key 0, first_query lengths[b]; masks: with the same mask as
+ * bytes), whatever else is in the batch; only a zero's sign may differ. Keys that no
+ * token attends may hold anything. A key that one token attends and another one does not
+ * may make the latter a NaN where its value is not finite; the former sets the error
+ * flag then. A token whose attended scores are all -infinity, which is bit 0 of the
+ * flag, keeps its output row too.
  * max_length bounds step_lengths, max_new the new tokens of a request (they size the
  * workspace with q_rows). A request past them or whose rows do not lie in q_rows,
  * or with more new tokens than its masks have bits, is left out with bit 5 of the

@@ -263,3 +263,68 @@ def test_spans_of_small_units_as_items(pcl, torch, ctx, heads, dtype, unit, held
                 exact=False)
     assert bool((out[cache.rows - 3:] == 9.5).all())
     assert ctx.sync() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(4, 2, 64), (32, 2, 128), (48, 3, 80)],
+                         ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("tree", [False, True], ids=["chain", "tree"])
+def test_scores_of_minus_infinity(pcl, torch, ctx, dtype, heads, tree):
+    # a token whose every score is -infinity keeps its row; for one that attends other
+    # keys too that key counts for nothing; both set bit 0
+    qheads, kvheads, dim = heads
+    held, counts = [0, 0, 300], [1, 5, 4]
+    masks = positions = None
+    if tree:
+        masks = [np.tril(np.ones((n, n), bool)) for n in counts]
+        positions = [[a + i for i in range(n)] for a, n in zip(held, counts)]
+    cache = TreeCache(pcl, torch, heads, held, counts, 16, dtype, 3, masks, positions)
+    q = cache.queries()
+    q.view(cache.rows, qheads, dim)[:, :, 3] = 1.0
+    outs = []
+    for bad in (-1e30, float("-inf")):  # (scores far below the others': weights of 0 too)
+        for b, at in ((0, 0), (1, 0), (2, 17)):
+            slot = int(cache.table[b, at // 16]) * 16 + at % 16
+            cache.pools.k.view(-1, kvheads, dim)[slot, :, 3] = bad
+        outs.append(cache.tree_attend(ctx, q))
+        assert ctx.sync() == (0 if bad > -float("inf") else 1)
+    want, out = outs
+    alone = [cache.first[0], cache.first[1]]
+    assert bool(torch.isfinite(out).all()) and bool((out[alone] == 9.5).all())
+    want[alone] = 9.5
+    assert np.array_equal(bits(out + 0.0), bits(want + 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(4096, 1, 16), (4096, 4096, 16), (4095, 3, 16)],
+                         ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("tree", [False, True], ids=["chain", "tree"])
+def test_heads_at_their_bounds(pcl, torch, ctx, heads, tree):
+    held, counts = [300, 0, 5], [2, 3, 1]
+    masks = positions = None
+    if tree:
+        masks, positions = random_trees(np.random.default_rng(7), held, counts)
+    cache = TreeCache(pcl, torch, heads, held, counts, 16, "bf16", 3, masks, positions)
+    q = cache.queries()
+    for window in (0, 260):
+        out = cache.tree_attend(ctx, q, window=window)
+        assert ctx.sync() == 0
+        cache.check(ctx, q, out, window=window)
+        assert bool((out[cache.rows - 3:] == 9.5).all())
+    assert ctx.sync() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,new", [((1, 1, 16), 3), ((12, 1, 16), 2)], ids=str)
+def test_a_length_bound_far_above_the_lengths(pcl, torch, ctx, heads, new):
+    # chunks, partials and items counted from 2^28 and more tokens
+    cache = TreeCache(pcl, torch, heads, [700], [new], 16, "f32", 3, rows=new)
+    q = cache.queries()
+    want = cache.tree_attend(ctx, q)
+    for length in (1 << 26, (1 << 28) + 7):
+        out = cache.tree_attend(ctx, q, max_length=length, table_stride=1 << 25)
+        assert ctx.sync() == 0
+        assert np.array_equal(bits(out), bits(want)), length
+    cache.check(ctx, q, want)
+    assert ctx.sync() == 0
