@@ -13,11 +13,12 @@
 //   pages that go back: those of the finished requests' tables that no other
 //   request's holds.
 // All but the copies are short, bound by their chains of dependent loads and by the
-// launch (MI355X): masks of 16 trees of 12 and of 256 of 64, 3.2 and 3.6 us; accepted
-// branches 3.2; a fork 4.6 (8 from 4 of up to 512 tokens) and 6.2 (480 from 16 of up to
-// 8192); a release 8.0 in one workgroup, 2.2 + 4.4 + 4.4 of its three launches. Copies
-// of 192 part-filled pages of three layers, 402 MB read and written, 89 us (4.5 TB/s; a
-// plain copy of 4 GiB 4.7), of 64 branches of up to 5 rows in six layers 6.2 us.
+// launch (MI355X, profiled durations): masks of 16 trees of 12 and of 256 of 64, 3.0 and
+// 3.8 us; accepted branches 3.2 and 3.4; a fork 4.4 (32 requests from 8 of up to 4000
+// tokens, pages of 16) and 6.0 (480 from 16 of up to 8192, pages of 8); their releases 8.0
+// in one workgroup, 1.8 + 4.4 + 4.4 in three launches. Copies of 192 part-filled pages of
+// 64 tokens in four layers of 2 x 512, f32, 402 MB read and written, 89 us (4.5 TB/s; a
+// plain copy of 4 GiB 4.7), of 64 branches of up to 5 rows in six layers 6.3 us.
 #include "context.hpp"
 #include "page_batch.hpp"
 #include "paged.hpp"
@@ -359,8 +360,8 @@ constexpr int kReleaseBits = 1 << 17, kReleaseEntries = 1 << 14;
 
 // Small batches: one workgroup, the marks as bits in LDS. The requests' words are read
 // at once, then a wave takes the tables of kReleaseAhead requests at a time, so that
-// their loads do not wait for each other's (8 forks of 4 prompts of up to 512 tokens: 8.0
-// us, 8.9 with a table after another).
+// their loads do not wait for each other's (32 forks of 8 prompts of up to 4000 tokens,
+// pages of 16: 8.0 us, 8.9 with a table after another).
 constexpr int kReleaseAhead = 4;
 
 __global__ __launch_bounds__(kReleaseThreads) void release_small_kernel(PageParams p)
@@ -565,9 +566,11 @@ int64_t mark_bytes(const pcl_page_batch *b)
     return (b->pages + 31) / 32 * 32;
 }
 
-// One workgroup does as long as it has some 16 pages a thread to look at: 40
-// requests of 250 pages 5 us against 13 of the three launches and 20 with their calls;
-// 496 requests of 1024 pages would be 0.3 ms.
+// One workgroup does as long as it has some 16 table entries a thread to look at. Calls in
+// a row, one workgroup and three launches, of a release in which nobody ended and of a
+// fork with its commit and release: 40 requests of 250 entries 6.2 and 8.5, 16.0 and 16.6
+// us; of 32 entries 5.0 and 9.1, 13.0 and 17; at the border 64 of 250 7.6 and 9.1, 17.4 and
+// 16.9, 16 of 1000 (the lives alone) 18.2 and 17.7, 8 of 1875 22 and 19.7.
 bool release_is_small(const pcl_page_batch *b)
 {
     return b->pages <= pcl::kReleaseBits &&

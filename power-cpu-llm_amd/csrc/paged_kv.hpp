@@ -22,9 +22,9 @@
 // Tree launches (paged_tree_kernel) have several new tokens' rows in a unit, each with
 // its own keys: four rows (new token, query head of the KV head) or eight. More rows
 // than eight take paged_rows.hpp, except where units of at most eight leave no more
-// items than CUs: one request of 6 new tokens behind 200 keys, 16 x 8 x 256, f32, 16 us
+// items than CUs: one request of 6 new tokens behind 200 keys, 16 x 8 x 256, f32, 15.6 us
 // in 24 items of four rows, bound by the chain of an item (64 KiB of K and 50 of V
-// through each wave; four buffers instead of two: 16.4 us).
+// through each wave; four buffers instead of two were 0.4 us slower).
 //
 // Bound by HBM where the lengths add up to some hundred MB (MI355X, cold inputs;
 // a call with its combine, the figures in brackets without): 64 requests of up

@@ -15,17 +15,17 @@
 // in paged_kv.hpp, takes five). The probabilities of all waves meet in LDS: three
 // barriers a chunk.
 //
-// Bound by the matrix instructions and the phases between them (MI355X, cold inputs; a
-// call with its plan and merge, this kernel in brackets, and the multiply-adds of
+// Bound by the matrix instructions and the phases between them (MI355X, cold inputs;
+// calls in a row, each with its plan and merge, and in brackets the multiply-adds of
 // whole units at 154 TFLOP/s, which a large f32 product of the library reaches):
-//   64 trees of up to 8 over up to 8192 keys, 16 x 8 x 256 heads, bf16, 0.86 GB: 245 us
-//     (222; 96), matrix pipes 45 % busy; 220 us where all pages are the same one;
-//   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 193 us (177; 106);
-//   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 890 us (840; 537);
-//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 162 us (147;
-//     62);
-//   4 prompt parts of up to 512 over up to 8192 keys, 16 x 8 x 256, bf16: 1.86 ms (1.75;
-//     1.16).
+//   64 trees of up to 8 over up to 8192 keys, 16 x 8 x 256 heads, bf16, 0.86 GB: 246 us
+//     (96), matrix pipes 47 % busy; 203 us where all pages are the same one;
+//   32 trees of up to 24, 1024-key window, 16 x 8 x 256, f32, 0.54 GB: 193 us (106);
+//   16 trees of up to 12 over up to 32K keys, 16 x 2 x 512, f32, 1.7 GB: 897 us (537);
+//   256 chains of up to 4 over up to 2048 keys, 32 x 8 x 128, bf16, 0.44 GB: 165 us (62);
+//   4 prompt parts of up to 512 over up to 8192 keys, 16 x 8 x 256, bf16: 1.87 ms (1.16).
+// The launch's words, two items and two chunks' words take more scalar registers than a
+// wave has: 136 to 208 of them lie in lanes of vector registers.
 // Of a chunk at 48 rows the scores take 43 % (83 % of it matrix instructions), the
 // softmax 10 %, P.V 45 % (79 %) and the output 2 %.
 //
@@ -34,9 +34,9 @@
 // with which two workgroups have a CU's registers at one 16 of rows, and the query
 // copied into LDS as it is, 222, 168 and 2054 us; a chunk's softmax from one read of
 // its maxima and items as workgroups come to them 237, 170 and 1881 us with their plan;
-// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us, 890 since), half lines
+// whole spans as items 248, 173 and 1857 us (the third case 1002 -> 882 us), half lines
 // of K up to head dim 128 165 us; an item's claim and the next chunk's words behind the
-// scores 245 and 162 us.
+// scores 245 and 162 us (246, 165 and 1868 since, the third case 897).
 #pragma once
 
 #include "paged_kv.hpp"

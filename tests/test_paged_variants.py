@@ -172,14 +172,24 @@ def resources(source):
     return {name: (w["S"], w["V"]) for name, w in found.items()}
 
 
-def test_no_kernel_of_few_rows_keeps_its_words_in_memory():
+@pytest.fixture(scope="module")
+def compiled():
+    """The same of every kernel of the tree attention, by source."""
     from concurrent.futures import ThreadPoolExecutor
     if not os.path.exists("/opt/rocm/bin/hipcc"):
         pytest.skip("hipcc absent")
-    with ThreadPoolExecutor(4) as pool:
-        found = dict(x for r in pool.map(resources, ["paged_tree_d%d.hip" % dk for dk in
-                                                     (512, 64, 128, 256)]) for x in r.items())
-    kernels = {n: w for n, w in found.items() if "paged_tree_kernel" in n}
+    sources = ["paged_%s_d%d.hip" % (kind, dk) for kind in ("rows", "tree")
+               for dk in (512, 64, 128, 256)]
+    with ThreadPoolExecutor(8) as pool:
+        return dict(zip(sources, pool.map(resources, sources)))
+
+
+def kernels_of(compiled, kind, name):
+    return {n: w for s, r in compiled.items() if kind in s for n, w in r.items() if name in n}
+
+
+def test_no_kernel_of_few_rows_keeps_its_words_in_memory(compiled):
+    kernels = kernels_of(compiled, "paged_tree", "paged_tree_kernel")
     assert len(kernels) == 48
     assert {n: w for n, w in kernels.items() if w != (0, 0)} == {}
 
@@ -189,14 +199,8 @@ def test_no_kernel_of_few_rows_keeps_its_words_in_memory():
 SPILLS = {"_ZN3pcl16tree_rows_kernelILi128EDF16bLb0ELi3ELi3EEEvNS_10TreeParamsE": (32, 8)}
 
 
-def test_no_kernel_of_many_rows_keeps_its_words_in_memory():
-    from concurrent.futures import ThreadPoolExecutor
-    if not os.path.exists("/opt/rocm/bin/hipcc"):
-        pytest.skip("hipcc absent")
-    with ThreadPoolExecutor(4) as pool:
-        found = dict(x for r in pool.map(resources, ["paged_rows_d%d.hip" % dk for dk in
-                                                     (512, 64, 128, 256)]) for x in r.items())
-    kernels = {n: w for n, w in found.items() if "tree_rows_kernel" in n}
+def test_no_kernel_of_many_rows_keeps_its_words_in_memory(compiled):
+    kernels = kernels_of(compiled, "paged_rows", "tree_rows_kernel")
     assert len(kernels) == 44 and set(SPILLS) <= set(kernels)
     for name, words in kernels.items():
         most = SPILLS.get(name, (0, 0))
