@@ -231,13 +231,13 @@ def test_each_kernel_has_the_contiguous_bits(pcl, torch, ctx, dim, dtype, unit, 
 
 # Whole spans of chunks are items from as many chunks on (over the units and KV heads) as
 # the longest span has, for each workgroup: at most four on a CU. Requests of one span of
-# three chunks, 3072 to 3456 of them in all; and of a whole span of sixteen and a part of
-# the next, 8640 chunks for two workgroups a CU (8192).
-SPANS = [((32, 8, 64), "f32", 16, [513 + i for i in range(128)]),
-         ((32, 8, 128), "f32", 16, [600 - 7 * i % 80 for i in range(128)]),
+# three chunks, enough for four workgroups on each CU; and of a whole span of sixteen and a
+# part of the next, 8640 chunks for two workgroups a CU (8192).
+SPANS = [((32, 8, 64), "f32", 16, [513 + i for i in range(140)]),
+         ((32, 8, 128), "f32", 16, [600 - 7 * i % 80 for i in range(140)]),
          ((16, 8, 256), "bf16", 16, [600 + i for i in range(144)]),
          ((16, 8, 256), "f32", 32, [590 + i % 40 for i in range(144)]),
-         ((32, 8, 128), "bf16", 32, [513 + i for i in range(128)]),
+         ((32, 8, 128), "bf16", 32, [513 + i for i in range(140)]),
          ((32, 8, 64), "bf16", 16, [4360 + 3 * i for i in range(60)])]
 
 
